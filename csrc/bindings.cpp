@@ -699,6 +699,141 @@ void kv_dequant_blocks_py(torch::Tensor cache, torch::Tensor scales, torch::Tens
                            cache.size(0), cache.size(2), cache.size(4), cache.size(3), dst.data_ptr(), cur_stream());
 }
 
+// ---- block-scaled 8-bit KV cache (int8, or uint8 with e4m3 bit patterns)
+static bool check_block8(const torch::Tensor& cache, const torch::Tensor& scales, bool layers) {
+  const int o = layers ? 1 : 0;
+  check_cuda(cache, "kv_cache");
+  TORCH_CHECK(cache.scalar_type() == at::kChar || cache.scalar_type() == at::kByte,
+              "block-scaled cache: int8, or uint8 with e4m3 bit patterns");
+  TORCH_CHECK(cache.dim() == 5 + o && cache.size(1 + o) == 2 && cache.is_contiguous(),
+              "block-scaled cache: contiguous [", layers ? "layers, " : "", "blocks, 2, Hk, block_size, D]");
+  check_same_device(cache, scales);
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.is_contiguous() && scales.dim() == 3 + o,
+              "block scales: contiguous fp32 [", layers ? "layers, " : "", "blocks, 2, Hk]");
+  for (int d = 0; d < 3 + o; ++d)
+    TORCH_CHECK(scales.size(d) == cache.size(d), "block scales do not match the cache");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0, "block-scaled cache: 16-byte alignment");
+  TORCH_CHECK(cache.size(o) <= INT32_MAX, "block-scaled cache: too many blocks");
+  return cache.scalar_type() == at::kByte;
+}
+static float* check_mass(const c10::optional<torch::Tensor>& mass, const torch::Tensor& cache, int o) {
+  if (!mass.has_value()) return nullptr;
+  check_same_device(cache, *mass);
+  TORCH_CHECK(mass->scalar_type() == at::kFloat && mass->is_contiguous() && mass->dim() == 3 + o &&
+                  mass->size(o) == cache.size(o) && mass->size(1 + o) == cache.size(2 + o) &&
+                  mass->size(2 + o) == cache.size(3 + o) && (o == 0 || mass->size(0) == cache.size(0)),
+              "mass: contiguous fp32 [", o ? "layers, " : "", "blocks, Hk, block_size] like the cache");
+  return mass->data_ptr<float>();
+}
+static void check_rows(const torch::Tensor& tables, const torch::Tensor& lens, const torch::Tensor& cache, int64_t rows) {
+  check_i32(tables, "block_tables");
+  check_i32(lens, "seq_lens");
+  check_same_device(tables, cache);
+  check_same_device(lens, cache);
+  TORCH_CHECK(tables.dim() == 2 && (tables.size(1) <= 1 || tables.stride(1) == 1) && tables.size(0) >= rows,
+              "block_tables [B, max_blocks] row-major");
+  TORCH_CHECK(lens.dim() == 1 && lens.is_contiguous() && lens.numel() >= rows, "seq_lens [B]");
+  TORCH_CHECK(tables.size(1) * cache.size(cache.dim() - 2) <= INT32_MAX - 256, "block_tables: too wide");
+}
+
+void kv_quant_blocks_py(torch::Tensor kv, torch::Tensor slots, torch::Tensor cache, torch::Tensor scales,
+                        c10::optional<torch::Tensor> mass) {
+  const bool e4m3 = check_block8(cache, scales, false);
+  check_bf16(kv, "kv");
+  check_i32(slots, "slots");
+  check_same_device(kv, cache);
+  check_same_device(slots, cache);
+  TORCH_CHECK(kv.dim() == 4 && kv.size(1) == 2 && kv.size(2) == cache.size(2) && kv.size(3) == cache.size(4),
+              "kv must be [T, 2, Hk, D] like the cache");
+  TORCH_CHECK(kv.stride(3) == 1 && kv.stride(0) % 4 == 0 && kv.stride(1) % 4 == 0 && kv.stride(2) % 4 == 0 &&
+                  reinterpret_cast<uintptr_t>(kv.data_ptr()) % 8 == 0,
+              "kv: unit stride over D, rows at multiples of 8 bytes");
+  TORCH_CHECK(slots.dim() == 1 && slots.is_contiguous() && slots.numel() >= kv.size(0), "one slot per token");
+  float* mp = check_mass(mass, cache, 0);
+  c10::cuda::CUDAGuard guard(cache.device());
+  launch_kv_quant_blocks(kv.data_ptr(), kv.stride(0), kv.stride(1), kv.stride(2), slots.data_ptr<int>(),
+                         cache.data_ptr(), scales.data_ptr<float>(), mp, kv.size(0), cache.size(2), cache.size(4),
+                         cache.size(3), (int)cache.size(0), e4m3, cur_stream());
+}
+
+void kv_dequant_scaled_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor tables,
+                          c10::optional<torch::Tensor> lens, torch::Tensor dst) {
+  const bool e4m3 = check_block8(cache, scales, false);
+  check_i32(tables, "block_tables");
+  check_bf16(dst, "dst");
+  check_same_device(tables, cache);
+  check_same_device(dst, cache);
+  if (lens.has_value()) check_rows(tables, *lens, cache, tables.size(0));
+  TORCH_CHECK(tables.dim() == 2 && (tables.size(1) <= 1 || tables.stride(1) == 1), "block_tables [B, max_blocks] row-major");
+  TORCH_CHECK(dst.is_contiguous() && dst.dim() == 5 && dst.size(0) * 16 >= tables.numel() * cache.size(3) &&
+                  dst.size(1) == 2 && dst.size(2) == cache.size(2) && dst.size(3) == 16 && dst.size(4) == cache.size(4),
+              "dst bf16 [B * max_blocks * block_size / 16, 2, Hk, 16, D]");
+  c10::cuda::CUDAGuard guard(cache.device());
+  launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>(), tables.stride(0),
+                           lens.has_value() ? lens->data_ptr<int>() : nullptr, tables.size(0), tables.size(1),
+                           (int)cache.size(0), cache.size(2), cache.size(4), cache.size(3), e4m3, dst.data_ptr(),
+                           cur_stream());
+}
+
+void block8_decode_py(torch::Tensor out, torch::Tensor q, torch::Tensor cache, torch::Tensor scales,
+                      torch::Tensor tables, torch::Tensor lens, double scale, int64_t splits,
+                      c10::optional<torch::Tensor> workspace, int64_t window, double softcap,
+                      c10::optional<torch::Tensor> mass) {
+  const bool e4m3 = check_block8(cache, scales, false);
+  check_bf16(q, "q");
+  check_bf16(out, "out");
+  check_same_device(q, cache);
+  check_same_device(out, cache);
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) == q.size(2) && q.size(2) == cache.size(4),
+              "q must be [B, H, D] with packed heads of the cache's D");
+  TORCH_CHECK(q.stride(0) % 4 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0, "q: rows at multiples of 8 bytes");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes(), "out must be contiguous like q");
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = cache.size(2);
+  TORCH_CHECK(Hk > 0 && H % Hk == 0, "H must be a multiple of Hk");
+  TORCH_CHECK(splits >= 1 && splits <= 64, "block-scaled decode attention: 1 to 64 splits");
+  check_rows(tables, lens, cache, B);
+  float* mp = check_mass(mass, cache, 0);
+  float *po = nullptr, *pml = nullptr, *sc = nullptr;
+  const int64_t n_o = splits > 1 ? B * H * splits * D : 0, n_ml = (splits > 1 || mp) ? B * H * splits * 2 : 0;
+  const int64_t n_sc = mp ? B * H * tables.size(1) * cache.size(3) : 0;
+  if (n_o + n_ml + n_sc > 0) {
+    TORCH_CHECK(workspace.has_value() && workspace->is_cuda() && workspace->scalar_type() == at::kFloat &&
+                    workspace->is_contiguous() && workspace->numel() >= n_o + n_ml + n_sc,
+                "decode attention: fp32 workspace of ", std::to_string(n_o + n_ml + n_sc), " elements needed");
+    check_same_device(*workspace, cache);
+    po = workspace->data_ptr<float>();
+    pml = po + n_o;
+    sc = pml + n_ml;
+  }
+  c10::cuda::CUDAGuard guard(cache.device());
+  launch_block8_decode(out.data_ptr(), q.data_ptr(), q.stride(0), cache.data_ptr(), scales.data_ptr<float>(),
+                       tables.data_ptr<int>(), tables.stride(0), tables.size(1), lens.data_ptr<int>(), B, H, Hk, D,
+                       cache.size(3), (int)cache.size(0), (int)splits, (float)scale, (int)window, (float)softcap, po,
+                       pml, sc, mp, e4m3, cur_stream());
+}
+
+void kv_evict_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor mass, torch::Tensor tables,
+                 torch::Tensor lens, torch::Tensor keep, torch::Tensor kept, int64_t sink, int64_t recent) {
+  const bool e4m3 = check_block8(cache, scales, true);
+  float* mp = check_mass(mass, cache, 1);
+  check_i32(keep, "keep_lens");
+  check_i32(kept, "kept");
+  check_same_device(keep, cache);
+  check_same_device(kept, cache);
+  const int64_t B = tables.size(0);
+  check_rows(tables, lens, cache, B);
+  TORCH_CHECK(keep.dim() == 1 && keep.is_contiguous() && keep.numel() >= B, "keep_lens [B]");
+  TORCH_CHECK(sink >= 0 && recent >= 0 && sink <= INT32_MAX && recent <= INT32_MAX, "kv_evict: sink and recent are token counts >= 0");
+  TORCH_CHECK(kept.is_contiguous() && kept.dim() == 4 && kept.size(0) == cache.size(0) && kept.size(1) == B &&
+                  kept.size(2) == cache.size(3),
+              "kept int32 [layers, B, Hk, max_keep]");
+  c10::cuda::CUDAGuard guard(cache.device());
+  launch_kv_evict(cache.data_ptr(), scales.data_ptr<float>(), mp, tables.data_ptr<int>(), tables.stride(0),
+                  tables.size(1), lens.data_ptr<int>(), keep.data_ptr<int>(), kept.data_ptr<int>(), cache.size(0), B,
+                  cache.size(3), cache.size(5), cache.size(4), (int)cache.size(1), (int)sink, (int)recent,
+                  (int)kept.size(3), e4m3, cur_stream());
+}
+
 // Grouped (per-expert) GEMM: out = a · b_g^T per M tile (tile_group names g); epi 0 none, 2 SwiGLU,
 // 5 scatter (`out` is then the uint64 per-row destination table).
 void gemm_grouped_py(torch::Tensor out, torch::Tensor a, torch::Tensor b, int64_t N, int64_t groups, int64_t epi,
@@ -965,6 +1100,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_q4k_splits", [](int64_t M, int64_t N, int64_t K) { return gemm_q4k_splits((int)M, (int)N, (int)K); },
         "split-K factor of the fused Q4_K GEMM");
   m.def("gemm_retile", &gemm_retile_py, "(tile width, whole-wave tiles, narrow tail tile width or 0) of a GEMM");
+  m.def("kv_quant_blocks", &kv_quant_blocks_py);
+  m.def("kv_dequant_scaled", &kv_dequant_scaled_py);
+  m.def("block8_decode", &block8_decode_py);
+  m.def("block8_decode_splits", &block8_decode_splits);
+  m.def("kv_evict", &kv_evict_py);
   m.def("num_sms", &device_num_sms);
   m.def("moe_forward", &moe_forward_out, "MoE layer: route, permute, grouped tcgen05 expert GEMMs, combine (K12)",
         py::arg("out"), py::arg("x"), py::arg("router"), py::arg("w_gu"), py::arg("w_down"), py::arg("ws"),

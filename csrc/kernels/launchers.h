@@ -245,6 +245,26 @@ void launch_kv_quant_fp8(const void* kv, const int* slots, void* cache, float* s
 void launch_kv_dequant_blocks(const void* cache, const float* scales, const int* ids, int n, int num_blocks, int Hk,
                               int D, int block_size, void* dst, cudaStream_t s);
 
+// ---- block-scaled 8-bit paged KV cache (csrc/kernels/kv_block8.cu): codes [NB, 2, Hk, bs, D] int8 or e4m3,
+// scales fp32 [NB, 2, Hk], mass fp32 [NB, Hk, bs]
+void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, const int* slots, void* cache,
+                            float* scales, float* mass, int T, int Hk, int D, int bs, int num_blocks, bool e4m3,
+                            cudaStream_t s);
+void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
+                              const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
+                              void* dst, cudaStream_t s);
+int block8_decode_splits(int B, int Hk, int G, int D, int64_t max_len);
+// part_o / part_ml: fp32 [B * H, splits, D] and [B * H, splits, 2] (splits > 1, or mass); scores: fp32
+// [B * Hk, mb * bs, G] (mass)
+void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void* cache, const float* scales,
+                          const int* tables, int64_t bt_stride, int mb, const int* lens, int B, int H, int Hk, int D,
+                          int bs, int num_blocks, int splits, float scale, int window, float softcap, float* part_o,
+                          float* part_ml, float* scores, float* mass, bool e4m3, cudaStream_t s);
+// cache [layers, NB, 2, Hk, bs, D]; kept int32 [layers, B, Hk, max_keep]
+void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
+                     const int* lens, const int* keep, int* kept, int layers, int B, int Hk, int D, int bs,
+                     int num_blocks, int sink, int recent, int max_keep, bool e4m3, cudaStream_t s);
+
 // ---- NVLS (multimem) collectives over a multicast-bound symmetric region (csrc/comm/nvls.cu)
 // mode: 0 one-shot, 1 two-shot (x gathered into every rank's x buffer), 2 reduce-scatter (owned rows local)
 void launch_tp_nvls_ar_rmsnorm(uint64_t uc, uint64_t mc, int rank, int world, int64_t p0, int64_t p1, int64_t x_off,

@@ -46,6 +46,7 @@ CUDA_SOURCES = [
     "kernels/moe.cu",
     "kernels/kv_transfer.cu",
     "kernels/kv_fp8.cu",
+    "kernels/kv_block8.cu",
     "kernels/int4.cu",
     "kernels/gdn.cu",
 ]

@@ -109,11 +109,13 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
                   num_heads: int, num_kv_heads: int, head_dim: int,
                   q_out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                   q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
-                  norm_eps: float = 1e-6, kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  norm_eps: float = 1e-6, kv_scales: Optional[torch.Tensor] = None,
+                  mass: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Split fused QKV (+ projection bias), per-head RMSNorm of q and k (QK-norm) when weights
     are given, NeoX RoPE of q and k, paged KV-cache write; returns q [T, H, D]. With ``kv_scales``
-    the cache is fp8 e4m3 (uint8 storage): the step's K/V rows go through a bf16 scratch and are
-    quantized into their slots with one scale per token and head (``kv_quant_fp8``)."""
+    the cache holds 8-bit codes: the step's K/V rows go through a bf16 scratch and are quantized
+    into their slots, with one scale per token and head (4-D scales: ``kv_quant_fp8``) or per block
+    and head (3-D scales: ``kv_quant_blocks``, which takes ``mass`` along)."""
     if kv_scales is not None and kv_cache is not None:
         T = qkv.shape[0]
         step = torch.empty(T, 2, num_kv_heads, 1, head_dim, dtype=torch.bfloat16 if qkv.is_cuda else qkv.dtype,
@@ -121,7 +123,11 @@ def rope_kv_write(qkv: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Ten
         ident = torch.arange(T, dtype=torch.int32, device=qkv.device)
         q = rope_kv_write(qkv, positions, cos_sin, step, ident, num_heads, num_kv_heads, head_dim, q_out, bias,
                           q_norm, k_norm, norm_eps)
-        kv_quant_fp8(step.view(T, 2, num_kv_heads, head_dim), slot_mapping, kv_cache, kv_scales)
+        step = step.view(T, 2, num_kv_heads, head_dim)
+        if kv_scales.dim() == 3:
+            kv_quant_blocks(step, slot_mapping, kv_cache, kv_scales, mass=mass)
+        else:
+            kv_quant_fp8(step, slot_mapping, kv_cache, kv_scales)
         return q
     if not qkv.is_cuda:
         return _cpu(ref.rope_kv_write(qkv, positions, cos_sin, kv_cache, slot_mapping,
@@ -172,12 +178,24 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
                            out: Optional[torch.Tensor] = None,
                            workspace: Optional[torch.Tensor] = None, tensor_cores: bool = True,
                            window: int = 0, softcap: float = 0.0,
-                           kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+                           kv_scales: Optional[torch.Tensor] = None,
+                           mass: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One query token per sequence: q [B, H, D]. head_dim 128 runs the tensor-core kernel
     (``tensor_cores=False`` selects the CUDA-core kernel, used for other head sizes).
     ``window`` > 0: sliding-window attention; ``softcap`` > 0: tanh soft-capped scores.
-    ``kv_scales`` (fp32 [NB, 2, Hk, bs]): ``kv_cache`` holds fp8 e4m3 values (uint8 storage), value =
-    e4m3 * scale of its token and head (head_dim 128)."""
+    ``kv_scales`` fp32 [NB, 2, Hk, bs]: ``kv_cache`` holds fp8 e4m3 values (uint8 storage), value =
+    e4m3 * scale of its token and head (head_dim 128).
+
+    ``kv_scales`` fp32 [NB, 2, Hk]: block-scaled cache (see ``kv_quant_blocks``; head_dim 32, 64, 96,
+    128 or 256). A sequence of length 0 gives zeros. ``num_splits`` 0 lets the kernel choose from the
+    shapes. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
+    heads of its KV head, is added to it; where rows share a block all of them are added, and only
+    then the last bits depend on their order."""
+    if kv_scales is not None and kv_scales.dim() == 3:
+        return _decode_block8(q, kv_cache, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap,
+                              kv_scales, mass)
+    if mass is not None:
+        raise ValueError("paged_decode_attention: mass needs a block-scaled cache (kv_scales [NB, 2, Hk])")
     if kv_scales is not None and not q.is_cuda:
         kv_cache = kv_dequant_fp8(kv_cache, kv_scales)
         kv_scales = None
@@ -192,6 +210,25 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
     _C(2 if num_splits > 1 else 1).paged_decode_attention(out, q, kv_cache, block_tables, seq_lens, float(scale),
                                                           int(num_splits), workspace, bool(tensor_cores),
                                                           int(window), float(softcap), kv_scales)
+    return out
+
+
+def _decode_block8(q, cache, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap, scales, mass):
+    if not q.is_cuda:
+        return _cpu(ref.block8_decode(q, cache, scales, block_tables, seq_lens, scale, window, softcap, mass), out)
+    B, H, D = q.shape
+    ext = cuda_ext()
+    width = block_tables.shape[1] * cache.shape[3]
+    if num_splits <= 0:
+        num_splits = ext.block8_decode_splits(B, cache.shape[2], H // max(1, cache.shape[2]), D, width)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+    # fp32 partial outputs and softmax sums of the splits, and the scores that become weights
+    n = B * H * ((num_splits * D if num_splits > 1 else 0) + (2 * num_splits if num_splits > 1 or mass is not None else 0)
+                 + (width if mass is not None else 0))
+    if n and workspace is None:
+        workspace = torch.empty(n, dtype=torch.float32, device=q.device)
+    _C(2 if n else 1).block8_decode(out, q, cache, scales, block_tables, seq_lens, float(scale), int(num_splits),
+                                    workspace, int(window), float(softcap), mass)
     return out
 
 
@@ -224,10 +261,23 @@ def kv_quant_fp8(kv: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor, sca
         scales[s // bs, :, :, s % bs] = scl[t]
 
 
-def kv_dequant_blocks(cache: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor):
-    """bf16 copy of the blocks an fp8 cache's ``block_tables`` [n, mb] reference, as a [n * mb]-block
-    cache, with the matching [n, mb] table (prefill attention over an fp8 cache)."""
+def kv_dequant_blocks(cache: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor,
+                      seq_lens: Optional[torch.Tensor] = None):
+    """bf16 copy of the blocks an 8-bit cache's ``block_tables`` [n, mb] reference, as a cache of its
+    own, with the matching table (prefill attention over an 8-bit cache). Scales per token ([NB, 2,
+    Hk, bs]): n * mb blocks of the cache's size. Scales per block ([NB, 2, Hk]): blocks of 16
+    tokens, the table [n, mb * bs / 16]; with ``seq_lens``, tokens behind a row's length read as zero
+    up to a multiple of 128 and are left unwritten beyond."""
     n, mb = block_tables.shape
+    if scales.dim() == 3:
+        bs = cache.shape[3]
+        mb16 = mb * bs // 16
+        if not cache.is_cuda:
+            tmp = ref.block8_gather(cache, scales, block_tables, seq_lens)
+        else:
+            tmp = torch.empty(n * mb16, 2, cache.shape[2], 16, cache.shape[4], dtype=torch.bfloat16, device=cache.device)
+            _C().kv_dequant_scaled(cache, scales, block_tables, seq_lens, tmp)
+        return tmp, torch.arange(n * mb16, dtype=torch.int32, device=cache.device).view(n, mb16)
     ids = block_tables.reshape(-1).contiguous()
     if not cache.is_cuda:
         NB = cache.shape[0]
@@ -238,6 +288,59 @@ def kv_dequant_blocks(cache: torch.Tensor, scales: torch.Tensor, block_tables: t
         _C().kv_dequant_blocks(cache, scales, ids, tmp)
     table = torch.arange(n * mb, dtype=torch.int32, device=cache.device).view(n, mb)
     return tmp, table
+
+
+# ---------------------------------------------------------------------------- block-scaled 8-bit KV cache
+def kv_quant_blocks(kv: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
+                    mass: Optional[torch.Tensor] = None) -> None:
+    """Write the step's K/V rows kv [T, 2, Hk, D] into a block-scaled 8-bit cache at ``slots`` (< 0:
+    skipped). ``cache`` [NB, 2, Hk, bs, D] holds codes (int8, or uint8 with e4m3 bit patterns), ``scales``
+    fp32 [NB, 2, Hk] one power of two (at least 2^-100) per block, K/V and head; value = code * scale.
+
+    A write to a block's first slot starts the block anew: its scale is the smallest that holds the
+    written rows. Any other write can only raise the scale; the codes already there are then rounded
+    to it. NaN is stored as 0, infinities as the largest bf16. ``mass`` (fp32 [NB, Hk, bs]), the
+    attention weight the tokens have drawn, becomes 0 at the written slots. The rows of one block must be
+    neighbours in ``slots`` (skipped rows aside), as the engine's batches are; of two rows with the
+    same slot the later one stays."""
+    if kv.is_cuda:
+        _C().kv_quant_blocks(kv, slots, cache, scales, mass)
+        return
+    ref.block8_write(kv, slots, cache, scales, mass)
+
+
+def kv_evict(cache: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor, block_tables: torch.Tensor,
+             seq_lens: torch.Tensor, keep_lens: torch.Tensor, sink: int, recent: int,
+             max_keep: Optional[int] = None) -> torch.Tensor:
+    """Shrink sequences of a block-scaled 8-bit cache to the tokens that drew the most attention.
+
+    Of a sequence (row of ``block_tables`` [B, mb]) with L = ``seq_lens[b]`` tokens and K = ``keep_lens[b]``
+    < L, every KV head (and layer) keeps the first ``sink`` tokens, the last ``recent`` and those of the
+    rest with the largest ``mass`` (ties: the earlier token; NaN counts as 0), K in all. They move in
+    order to the front of the sequence's blocks, in place, codes, mass and block scales with them
+    (each block gets the smallest scale that holds its tokens), so the first ceil(K / bs) blocks hold the
+    sequence and the caller may release the others. Sequences with K >= L stay as they are. No block
+    may belong to two rows.
+
+    ``cache`` [(layers,) NB, 2, Hk, bs, D] with ``scales`` [(layers,) NB, 2, Hk] and ``mass`` [(layers,) NB, Hk,
+    bs]. Returns the kept tokens' former places, int32 [(layers,) B, Hk, max_keep], padded with -1;
+    ``max_keep`` (default: the table's width in tokens) must be at least the largest K below its L: a larger
+    one is cut to it."""
+    bs = cache.shape[-2]
+    one = cache.dim() == 5
+    if max_keep is None:
+        max_keep = block_tables.shape[1] * bs
+    if max_keep < 0:
+        raise ValueError("kv_evict: max_keep must be >= 0")
+    if one:
+        cache, scales, mass = cache.unsqueeze(0), scales.unsqueeze(0), mass.unsqueeze(0)
+    if not cache.is_cuda:
+        kept = ref.block8_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, sink, recent, max_keep)
+    else:
+        kept = torch.empty(cache.shape[0], block_tables.shape[0], cache.shape[3], max_keep, dtype=torch.int32,
+                           device=cache.device)
+        _C(2 if max_keep else 1).kv_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, kept, int(sink), int(recent))
+    return kept[0] if one else kept
 
 
 def prefill_block_m(head_dim: int, tensor_cores: bool = True) -> int:
@@ -312,10 +415,11 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     """Varlen causal attention of new tokens q [T, H, D] over the paged KV (prefix + new).
     head_dim 64 / 128 runs on tcgen05/TMEM (the two-tile kernel when ``tiles`` is a ``prefill_schedule``
     work list); other sizes on mma.sync (64-row tiles). ``window`` > 0: sliding-window attention;
-    ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (fp8 cache) the referenced blocks
-    are dequantized into a bf16 copy first."""
+    ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (8-bit cache, scales per token or per
+    block) the referenced blocks are dequantized into a bf16 copy first."""
     if kv_scales is not None:
-        kv_cache, block_tables = kv_dequant_blocks(kv_cache, kv_scales, block_tables)
+        kv_cache, block_tables = kv_dequant_blocks(kv_cache, kv_scales, block_tables,
+                                                   seq_lens if kv_scales.dim() == 3 else None)
     if not q.is_cuda:
         return _cpu(ref.paged_attention(q, kv_cache, block_tables, seq_lens, query_start, scale, window, softcap),
                     out)

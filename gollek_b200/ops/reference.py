@@ -120,6 +120,160 @@ def paged_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch
     return out
 
 
+# ---- block-scaled 8-bit KV cache: codes [NB, 2, Hk, bs, D], scales [NB, 2, Hk], mass [NB, Hk, bs]
+BLOCK8_FLOOR = -100                       # the smallest scale is 2^-100
+_BF16_MAX = 3.3895313892515355e38
+
+
+def block8_decode_codes(codes: torch.Tensor) -> torch.Tensor:
+    """fp32 numbers of 8-bit codes (int8, or uint8 with e4m3 bit patterns)."""
+    return codes.float() if codes.dtype == torch.int8 else codes.view(torch.float8_e4m3fn).float()
+
+
+def block8_encode(y: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """8-bit codes of y = value / scale, to nearest, ties to even, saturating."""
+    if dtype == torch.int8:
+        return y.round().clamp(-127, 127).to(torch.int8)
+    return y.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+
+
+def block8_scale(amax: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The smallest power of two s >= 2^-100 with amax <= qmax * s (qmax 127 for int8, 448 for e4m3)."""
+    m, e = torch.frexp(amax.float())
+    bits, top = (7, 127 / 128) if dtype == torch.int8 else (9, 0.875)
+    e = (e - bits + (m > top).int()).clamp(min=BLOCK8_FLOOR)
+    e = torch.where(amax > 0, e, torch.full_like(e, BLOCK8_FLOOR))
+    return ((e + 127) << 23).view(torch.float32)
+
+
+def _block8_check(cache, scales, mass, layers: bool = False) -> None:
+    o = 1 if layers else 0
+    if cache.dtype not in (torch.int8, torch.uint8) or cache.dim() != 5 + o or cache.shape[1 + o] != 2:
+        raise ValueError("block-scaled cache: int8 or uint8 [blocks, 2, Hk, block_size, D]")
+    if cache.shape[3 + o] not in (16, 32, 64):
+        raise ValueError("block-scaled KV cache: block size 16, 32 or 64")
+    if scales.dtype != torch.float32 or tuple(scales.shape) != tuple(cache.shape[:3 + o]):
+        raise ValueError("block scales: fp32 [blocks, 2, Hk] like the cache")
+    want = tuple(cache.shape[:1 + o]) + tuple(cache.shape[2 + o:4 + o])
+    if mass is not None and (mass.dtype != torch.float32 or tuple(mass.shape) != want):
+        raise ValueError("mass: fp32 [blocks, Hk, block_size] like the cache")
+
+
+def block8_write(kv: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor,
+                 mass: Optional[torch.Tensor] = None) -> None:
+    """Rows kv [T, 2, Hk, D] into their slots, block by block (see ``ops.kv_quant_blocks``)."""
+    _block8_check(cache, scales, mass)
+    NB, bs = cache.shape[0], cache.shape[3]
+    if kv.dim() != 4 or tuple(kv.shape[1:]) != (2, cache.shape[2], cache.shape[4]) or slots.numel() < kv.shape[0]:
+        raise ValueError("kv must be [T, 2, Hk, D] like the cache, with one slot per token")
+    x = kv.float().nan_to_num(0.0, _BF16_MAX, -_BF16_MAX).clamp(-_BF16_MAX, _BF16_MAX)
+    runs, last = [], None
+    for t, s in enumerate(slots[: kv.shape[0]].tolist()):
+        if s < 0:
+            continue
+        if s // bs >= NB:
+            raise ValueError(f"slot {s} beyond the pool")
+        if s // bs != last:
+            if any(r[0] == s // bs for r in runs):
+                raise ValueError("kv_quant_blocks: the rows of one block must be neighbours")
+            runs.append((s // bs, [], []))
+            last = s // bs
+        runs[-1][1].append(t)
+        runs[-1][2].append(s % bs)
+    for blk, ts, offs in runs:
+        need = block8_scale(x[ts].abs().amax((0, -1)), cache.dtype)
+        if 0 not in offs:
+            new = torch.maximum(scales[blk], need)
+            grown = (new > scales[blk])[..., None, None]
+            y = block8_decode_codes(cache[blk]) * (scales[blk] / new)[..., None, None]
+            cache[blk] = torch.where(grown, block8_encode(y, cache.dtype), cache[blk])
+        else:
+            new = need
+        scales[blk] = new
+        for t, o in zip(ts, offs):
+            cache[blk, :, :, o] = block8_encode(x[t] / new[..., None], cache.dtype)
+        if mass is not None:
+            mass[blk, :, offs] = 0.0
+
+
+def block8_gather(cache: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor,
+                  seq_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fp32 copy of the tables' blocks, [n * mb * bs / 16, 2, Hk, 16, D]; zero behind each row's length."""
+    _block8_check(cache, scales, None)
+    NB, _, Hk, bs, D = cache.shape
+    n, mb = block_tables.shape
+    ids = block_tables.long().clamp(0, NB - 1)
+    x = block8_decode_codes(cache[ids]) * scales[ids][..., None, None]          # [n, mb, 2, Hk, bs, D]
+    if seq_lens is not None:
+        pos = torch.arange(mb * bs).view(1, mb, 1, 1, bs, 1)
+        x = torch.where(pos < seq_lens[:n].long().view(n, 1, 1, 1, 1, 1), x, torch.zeros(()))
+    return x.view(n, mb, 2, Hk, bs // 16, 16, D).permute(0, 1, 4, 2, 3, 5, 6).reshape(-1, 2, Hk, 16, D)
+
+
+def block8_decode(q: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor, block_tables: torch.Tensor,
+                  seq_lens: torch.Tensor, scale: float, window: int = 0, softcap: float = 0.0,
+                  mass: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One query per sequence over a block-scaled cache; adds the softmax weights to ``mass``."""
+    _block8_check(cache, scales, mass)
+    B, H, D = q.shape
+    Hk, bs = cache.shape[2], cache.shape[3]
+    if H % Hk or D != cache.shape[4]:
+        raise ValueError("q must be [B, H, D] with H a multiple of Hk and the cache's D")
+    out = torch.zeros_like(q)
+    for b in range(B):
+        L = min(max(int(seq_lens[b]), 0), block_tables.shape[1] * bs)
+        lo = max(0, L - window) if window > 0 else 0
+        if L == 0:
+            continue
+        at = torch.arange(lo, L)
+        ids = block_tables[b].long()[at // bs]
+        kv = block8_decode_codes(cache[ids, :, :, at % bs]) * scales[ids][..., None]   # [n, 2, Hk, D]
+        s = torch.einsum("kgd,nkd->kgn", q[b].float().view(Hk, H // Hk, D), kv[:, 0]) * scale
+        if softcap > 0:
+            s = softcap * torch.tanh(s / softcap)
+        p = torch.softmax(s, -1)
+        out[b] = torch.einsum("kgn,nkd->kgd", p, kv[:, 1]).reshape(H, D).to(q.dtype)
+        if mass is not None:
+            mass[ids, :, at % bs] += p.sum(1).T
+    return out
+
+
+def block8_evict(cache: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor, block_tables: torch.Tensor,
+                 seq_lens: torch.Tensor, keep_lens: torch.Tensor, sink: int, recent: int, max_keep: int) -> torch.Tensor:
+    """Keep the tokens with the most attention weight (see ``ops.kv_evict``); cache [layers, NB, ...]."""
+    _block8_check(cache, scales, mass, layers=True)
+    if sink < 0 or recent < 0:
+        raise ValueError("kv_evict: sink and recent are token counts >= 0")
+    Ly, _, _, Hk, bs, D = cache.shape
+    B = block_tables.shape[0]
+    kept = torch.full((Ly, B, Hk, max_keep), -1, dtype=torch.int32)
+    for b in range(B):
+        L = min(max(int(seq_lens[b]), 0), block_tables.shape[1] * bs)
+        K = min(max(int(keep_lens[b]), 0), L)
+        if K == L:
+            kept[:, b, :, : min(L, max_keep)] = torch.arange(min(L, max_keep), dtype=torch.int32)
+            continue
+        K = min(K, max_keep)
+        a = min(sink, K)
+        r = min(recent, K - a)
+        at = torch.arange(L)
+        ids, off = block_tables[b].long()[at // bs], at % bs
+        for ly in range(Ly):
+            for h in range(Hk):
+                w = mass[ly, ids, h, off]
+                mid = w[a:L - r].nan_to_num(0.0).sort(descending=True, stable=True).indices[: K - a - r].sort().values + a
+                src = torch.cat([at[:a], mid, at[L - r:]])
+                kept[ly, b, h, :K] = src.int()
+                x = block8_decode_codes(cache[ly, ids[src], :, h, off[src]]) * scales[ly, ids[src], :, h][..., None]
+                for j in range(0, K, bs):
+                    blk, n = ids[j], min(bs, K - j)
+                    s = block8_scale(x[j:j + n].abs().amax((0, 2)), cache.dtype)               # [2]
+                    cache[ly, blk, :, h, :n] = block8_encode(x[j:j + n] / s[:, None], cache.dtype).transpose(0, 1)
+                    scales[ly, blk, :, h] = s
+                mass[ly, ids[:K], h, off[:K]] = w[src]
+    return kept
+
+
 def gemm(a: torch.Tensor, b: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y = a @ b.T (+ residual); a [M, K], b [N, K] (nn.Linear layout)."""
     y = a.float() @ b.float().t()

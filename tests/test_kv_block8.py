@@ -1,0 +1,629 @@
+"""Block-scaled 8-bit KV cache (int8 / e4m3 codes, one power-of-two scale per block and head): write, decode
+attention with accumulated weights, prompt attention, eviction; against plain 64-bit restatements.
+
+Tolerances, where the result is rounded: an output element is sum(p v) with p held in f16 (half a step 2^-11, the
+products and sums in fp32) and stored in bf16 (half a step 2^-8 relative), so
+|error| <= 2^-8 |out| + 2^-10 sum(p |v|). A softmax weight comes from an fp32 score of D products (each
+rounded by at most D 2^-24 of sum |q k|) and an exponential of relative error 2^-20 at most."""
+import math
+
+import pytest
+import torch
+
+from gollek_b200 import ops
+from gollek_b200.ops import reference as ref
+
+KINDS = {"int8": torch.int8, "e4m3": torch.uint8}
+
+
+def numbers(codes):
+    """64-bit numbers of the codes, from their bits."""
+    if codes.dtype == torch.int8:
+        return codes.double()
+    c = codes.long()
+    e, m = (c >> 3) & 15, (c & 7).double()
+    v = torch.where(e == 0, m * 2.0 ** -9, (1 + m / 8) * torch.exp2((e - 7).double()))
+    v = torch.where((c & 127) == 127, torch.full_like(v, math.nan), v)
+    return torch.where(c >= 128, -v, v)
+
+
+def values(cache, scales):
+    return numbers(cache) * scales.double()[..., None, None]
+
+
+def least_scale(top, kind):
+    y = max(top / (127.0 if kind == "int8" else 448.0), 2.0 ** -100)
+    m, e = math.frexp(y)
+    return 2.0 ** (e - 1 if m == 0.5 else e)
+
+
+def nearest(y, kind):
+    """y rounded to the type's numbers, ties to even."""
+    if kind == "int8":
+        return y.round().clamp(-127, 127)
+    step = torch.exp2(torch.frexp(y).exponent.clamp(min=-5).double() - 4)
+    return ((y / step).round() * step).clamp(-448, 448)
+
+
+def tables_for(lens, bs, gen, spare=4):
+    nb = [(l + bs - 1) // bs for l in lens]
+    NB = sum(nb) + spare
+    ids = (torch.randperm(NB - 1, generator=gen) + 1).int()   # block 0 belongs to nobody: tables are padded with it
+    bt = torch.zeros(len(lens), max(1, max(nb)), dtype=torch.int32)
+    k = 0
+    for b, n in enumerate(nb):
+        bt[b, :n] = ids[k:k + n]
+        k += n
+    return bt, NB
+
+
+def filled(kind, lens, Hk, D, bs, seed, layers=1):
+    """A cache whose tokens are random; everything behind a sequence's end is poison."""
+    g = torch.Generator().manual_seed(seed)
+    bt, NB = tables_for(lens, bs, g)
+    code = torch.randint(-127, 128, (layers, NB, 2, Hk, bs, D), generator=g)
+    cache = code.to(torch.int8) if kind == "int8" else (code.float() / 8).to(torch.float8_e4m3fn).view(torch.uint8)
+    scales = torch.exp2(torch.randint(-9, -4, (layers, NB, 2, Hk), generator=g).float())
+    if kind == "e4m3":
+        scales *= 8
+    used = set(bt.flatten().tolist()) - {0}
+    for i in range(NB):
+        if i not in used:
+            scales[:, i] = math.nan
+    for b, l in enumerate(lens):
+        if l % bs:
+            cache[:, bt[b, l // bs].item(), :, :, l % bs:] = 127     # e4m3: NaN
+    mass = torch.rand(layers, NB, Hk, bs, generator=g)
+    return cache, scales, mass, bt, torch.tensor(lens, dtype=torch.int32)
+
+
+def attend(q, cache, scales, bt, lens, scale, window=0, softcap=0.0):
+    """64-bit attention of one query per row: out, weights per (row, kv head, token), sum(p |v|), sum |q k|."""
+    B, H, D = q.shape
+    Hk, bs = cache.shape[2], cache.shape[3]
+    out = torch.zeros(B, H, D, dtype=torch.float64)
+    absv = torch.zeros_like(out)
+    weights, big = [], 0.0
+    for b in range(B):
+        L = int(lens[b])
+        lo = max(0, L - window) if window else 0
+        at = torch.arange(lo, L)
+        w = torch.zeros(Hk, L, dtype=torch.float64)
+        if L:
+            ids = bt[b].long()[at // bs]
+            x = numbers(cache[ids, :, :, at % bs]) * scales[ids].double()[..., None]
+            for h in range(H):
+                k, v, qq = x[:, 0, h // (H // Hk)], x[:, 1, h // (H // Hk)], q[b, h].double()
+                s = k @ qq * scale
+                big = max(big, float((k.abs() @ qq.abs()).max()) * scale)
+                if softcap:
+                    s = softcap * torch.tanh(s / softcap)
+                p = torch.softmax(s, 0)
+                out[b, h], absv[b, h] = p @ v, p @ v.abs()
+                w[h // (H // Hk), lo:] += p
+        weights.append(w)
+    return out, weights, absv, big
+
+
+def check_out(got, out, absv):
+    err = (got.double().cpu() - out).abs()
+    assert bool((err <= 2.0 ** -8 * out.abs() + 2.0 ** -10 * absv + 1e-30).all()), float((err / (absv + 1e-30)).max())
+
+
+def check_mass(got, before, weights, bt, lens, bs, D, big, cap=0.0):
+    """The weights' sums; everything else untouched to the bit."""
+    want, seen = before.double().clone(), torch.zeros_like(before, dtype=torch.bool)
+    # the cap's tanh has an absolute error of 2^-20 at most, times the cap
+    rel = 2.0 ** -20 + 2 * D * 2.0 ** -24 * big + cap * 2.0 ** -20
+    tol = torch.zeros_like(want)
+    for b, w in enumerate(weights):
+        for t in range(w.shape[1]):
+            blk = int(bt[b, t // bs])
+            want[blk, :, t % bs] += w[:, t]
+            tol[blk, :, t % bs] += rel * w[:, t] + 2.0 ** -23 * want[blk, :, t % bs]
+            seen[blk, :, t % bs] |= w[:, t] > 0
+    got = got.double().cpu()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() - tol).max())
+    assert torch.equal(got[~seen], before.double()[~seen])
+
+
+# ------------------------------------------------------------------------------------------- write
+def write_oracle(kv, slots, cache, scales, mass, kind):
+    num, sc, ms = numbers(cache), scales.double().clone(), mass.clone()
+    bs = cache.shape[3]
+    by = {}
+    for t, s in enumerate(slots.tolist()):
+        if s >= 0:
+            by.setdefault(s // bs, []).append((t, s % bs))
+    x = kv.double().nan_to_num(0.0, 3.3895313892515355e38, -3.3895313892515355e38)
+    for blk, rows in by.items():
+        for w in range(2):
+            for h in range(kv.shape[2]):
+                need = least_scale(max(float(x[t, w, h].abs().max()) for t, _ in rows), kind)
+                old = float(sc[blk, w, h])
+                s = need if any(o == 0 for _, o in rows) else max(old, need)
+                if s > old and not any(o == 0 for _, o in rows):
+                    num[blk, w, h] = nearest(num[blk, w, h] * (old / s), kind)
+                sc[blk, w, h] = s
+                for t, o in rows:
+                    num[blk, w, h, o] = nearest(x[t, w, h] / s, kind)
+        for _, o in rows:
+            ms[blk, :, o] = 0
+    return num, sc, ms
+
+
+def write_case(kind, Hk, D, bs, seed):
+    """Rows that fill blocks from their start, go on in the middle, sit alone; skipped rows; odd values."""
+    g = torch.Generator().manual_seed(seed)
+    cache, scales, mass, bt, _ = filled(kind, [3 * bs + 5, 2 * bs], Hk, D, bs, seed)
+    scales = scales.nan_to_num(0.25)
+    if kind == "e4m3":
+        cache = torch.where((cache & 127) == 127, torch.zeros_like(cache), cache)
+    slots = []
+    slots += [int(bt[0, 0]) * bs + i for i in range(bs)]                   # a whole block
+    slots += [-1, int(bt[0, 1]) * bs + 0, -1, int(bt[0, 1]) * bs + 1]      # a block begun, skipped rows around
+    slots += [int(bt[0, 2]) * bs + i for i in (3, 4, 5)]                   # in the middle
+    slots += [int(bt[0, 3]) * bs + 7, int(bt[1, 0]) * bs + 9, int(bt[1, 1]) * bs + bs - 1, -1]
+    kv = torch.randn(len(slots), 2, Hk, D, generator=g)
+    kv[-2] *= 1000.0                                                       # its block's scale has to grow
+    kv[-3] = 0.0                                                           # nothing to add
+    kv[2, 0, 0, :4] = torch.tensor([math.nan, math.inf, -math.inf, -0.0])
+    kv[5, 1] = 1e-38
+    return kv.bfloat16(), torch.tensor(slots, dtype=torch.int32), cache[0], scales[0], mass[0]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("Hk,D,bs", [(2, 64, 16), (1, 96, 32), (3, 32, 64)])
+def test_write_cpu(kind, Hk, D, bs):
+    kv, slots, cache, scales, mass = write_case(kind, Hk, D, bs, 1)
+    num, sc, ms = write_oracle(kv, slots, cache, scales, mass, kind)
+    ops.kv_quant_blocks(kv, slots, cache, scales, mass=mass)
+    assert torch.equal(numbers(cache), num) and torch.equal(scales.double(), sc) and torch.equal(mass, ms)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("Hk,D,bs", [(2, 64, 16), (1, 96, 32), (3, 32, 64), (8, 128, 16), (2, 256, 32)])
+def test_write_gpu(kind, Hk, D, bs):
+    kv, slots, cache, scales, mass = write_case(kind, Hk, D, bs, 2)
+    num, sc, ms = write_oracle(kv, slots, cache, scales, mass, kind)
+    c, s, m = cache.cuda(), scales.cuda(), mass.cuda()
+    wide = torch.zeros(kv.shape[0], 3, Hk + 1, D + 8, dtype=torch.bfloat16, device="cuda")
+    wide[:, 1:, 1:, :D] = kv.cuda()
+    ops.kv_quant_blocks(wide[:, 1:, 1:, :D], slots.cuda(), c, s, mass=m)     # a strided view of K / V
+    assert torch.equal(numbers(c.cpu()), num) and torch.equal(s.cpu().double(), sc) and torch.equal(m.cpu(), ms)
+    c2, s2 = cache.cuda(), scales.cuda()
+    ops.kv_quant_blocks(kv.cuda(), slots.cuda(), c2, s2)                     # without weights
+    assert torch.equal(c2, c) and torch.equal(s2, s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("T", [0, 1, 1023, 1024, 2500])
+def test_write_long_runs_gpu(kind, T):
+    """Prompts of many blocks, the last one part-filled, starting in the middle of a block."""
+    Hk, D, bs = 2, 128, 16
+    g = torch.Generator().manual_seed(T)
+    lens = [T + 21, 40]
+    cache, scales, mass, bt, _ = filled(kind, lens, Hk, D, bs, 3)
+    scales = scales.nan_to_num(0.5)
+    if kind == "e4m3":
+        cache = torch.where((cache & 127) == 127, torch.zeros_like(cache), cache)
+    pos = torch.arange(21, 21 + T)
+    slots = torch.cat([bt[0].long()[pos // bs] * bs + pos % bs, torch.full((5,), -1)]).int()
+    kv = torch.randn(T + 5, 2, Hk, D, generator=g).bfloat16()
+    want = [x[0].clone() for x in (cache, scales, mass)]
+    ops.kv_quant_blocks(kv, slots, *want[:2], mass=want[2])
+    got = [x[0].cuda() for x in (cache, scales, mass)]
+    ops.kv_quant_blocks(kv.cuda(), slots.cuda(), *got[:2], mass=got[2])
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------- decode
+LENS = [0, 1, 15, 16, 17, 31, 300, 700]
+
+
+def test_decode_cpu():
+    cache, scales, mass, bt, lens = filled("int8", LENS, 2, 32, 16, 5)
+    q = torch.randn(len(LENS), 6, 32, generator=torch.Generator().manual_seed(1))
+    m = mass[0].clone()
+    got = ops.paged_decode_attention(q, cache[0], bt, lens, 0.2, kv_scales=scales[0], mass=m, window=100, softcap=5.0)
+    out, w, absv, big = attend(q, cache[0], scales[0], bt, lens, 0.2, 100, 5.0)
+    check_out(got, out, absv)
+    check_mass(m, mass[0], w, bt, lens, 16, 32, big, 5.0)
+    assert bool((got[0] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D,G,bs", [(128, 4, 16), (64, 8, 32), (96, 1, 16), (32, 7, 64), (256, 2, 16), (256, 12, 32),
+                                    (128, 16, 16), (64, 24, 16), (96, 9, 16), (128, 1, 64)])
+@pytest.mark.parametrize("splits,weigh", [(0, True), (1, False), (1, True), (5, True), (64, False)])
+def test_decode_gpu(kind, D, G, bs, splits, weigh):
+    Hk = 2
+    cache, scales, mass, bt, lens = filled(kind, LENS, Hk, D, bs, D + G)
+    g = torch.Generator().manual_seed(D * G)
+    q = (torch.randn(len(LENS), Hk * G, D, generator=g) * 0.5).bfloat16()
+    q[3] = 0.0
+    q[5] *= 2.0 ** -30
+    scale = 1 / math.sqrt(D)
+    m = mass[0].cuda()
+    dev = [x.cuda() for x in (q, cache[0], bt, lens)]
+    got = ops.paged_decode_attention(*dev, scale, num_splits=splits, kv_scales=scales[0].cuda(),
+                                     mass=m if weigh else None)
+    out, w, absv, big = attend(q, cache[0], scales[0], bt, lens, scale)
+    check_out(got, out, absv)
+    assert bool((got[0] == 0).all())
+    if weigh:
+        check_mass(m, mass[0], w, bt, lens, bs, D, big)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("window,softcap", [(1, 0.0), (16, 0.0), (33, 3.0), (5000, 30.0), (0, 0.5)])
+def test_decode_window_and_cap_gpu(kind, window, softcap):
+    cache, scales, mass, bt, lens = filled(kind, LENS, 2, 64, 16, 9)
+    q = torch.randn(len(LENS), 8, 64, generator=torch.Generator().manual_seed(2)).bfloat16()
+    m = mass[0].cuda()
+    got = ops.paged_decode_attention(q.cuda(), cache[0].cuda(), bt.cuda(), lens.cuda(), 0.125, num_splits=0,
+                                     kv_scales=scales[0].cuda(), mass=m, window=window, softcap=softcap)
+    out, w, absv, big = attend(q, cache[0], scales[0], bt, lens, 0.125, window, softcap)
+    check_out(got, out, absv)
+    check_mass(m, mass[0], w, bt, lens, 16, 64, big, softcap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_decode_uneven_scales_gpu(kind):
+    """Value scales 2^-100 .. 2^90 apart from block to block, a dominant token in a block of tiny values, all-zero
+    blocks, scores of +-200: nothing may overflow or drown."""
+    Hk, D, bs = 2, 64, 16
+    cache, scales, _, bt, lens = filled(kind, [90, 64, 48], Hk, D, bs, 11)
+    cache, scales = cache[0], scales[0]
+    q = torch.randn(3, 8, D, generator=torch.Generator().manual_seed(3)).bfloat16() * 8
+    scales[bt[0, 0], 1] = 2.0 ** -100
+    scales[bt[0, 2], 1] = 2.0 ** 90
+    cache[bt[1, 1], 1] = 0
+    scales[bt[1, 1], 1] = 2.0 ** -100
+    scales[bt[2, 0], 1] = 2.0 ** -60
+    scales[bt[2, 0], 0] *= 64                        # its scores decide the softmax
+    got = ops.paged_decode_attention(q.cuda(), cache.cuda(), bt.cuda(), lens.cuda(), 1.0, num_splits=0,
+                                     kv_scales=scales.cuda())
+    out, _, absv, _ = attend(q, cache, scales, bt, lens, 1.0)
+    # scores of up to some thousand: an fp32 score is off by up to 2 D 2^-24 of sum |q k|, and so is a weight
+    big = max(attend(q[b:b + 1], cache, scales, bt[b:b + 1], lens[b:b + 1], 1.0)[3] for b in range(3))
+    err = (got.double().cpu() - out).abs()
+    # p * scale is held in f16 over a reference no larger than its largest value among the tokens: below
+    # 2^-14 of it f16 steps are 2^-24, so a token's term is off by up to 2^-25 qmax max(p scale) even where its
+    # own p is far smaller (sums in which only such tokens have a non-zero code)
+    floor = torch.zeros_like(out)
+    for b in range(3):
+        at = torch.arange(int(lens[b]))
+        ids = bt[b].long()[at // bs]
+        for h in range(8):
+            k = numbers(cache[ids, 0, h // 4, at % bs]) * scales[ids, 0, h // 4].double()[:, None]
+            p = torch.softmax(k @ q[b, h].double(), 0)
+            floor[b, h] = len(at) * 2.0 ** -25 * 448 * float((p * scales[ids, 1, h // 4].double()).max())
+    tol = 2.0 ** -8 * out.abs() + (2.0 ** -10 + 4 * D * 2.0 ** -24 * big) * absv + floor
+    assert bool((err <= tol).all())
+
+
+@pytest.mark.gpu
+def test_decode_strides_stream_graph_and_shared_blocks_gpu():
+    cache, scales, mass, bt, lens = filled("int8", [200, 333, 64], 2, 128, 16, 13)
+    qkv = torch.randn(3, (8 + 4) * 128, generator=torch.Generator().manual_seed(4)).bfloat16().cuda()
+    q = qkv[:, :8 * 128].view(3, 8, 128)
+    wide = torch.zeros(5, bt.shape[1] + 9, dtype=torch.int32, device="cuda")
+    wide[:3, :bt.shape[1]] = bt.cuda()
+    c, s, l = cache[0].cuda(), scales[0].cuda(), lens.cuda()
+    base = ops.paged_decode_attention(q, c, wide[:, :bt.shape[1]], l, 0.09, num_splits=0, kv_scales=s)
+    out, w, absv, big = attend(q.cpu(), cache[0], scales[0], bt, lens, 0.09)
+    check_out(base, out, absv)
+    # another stream gives the same bits
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        other = ops.paged_decode_attention(q, c, wide, l, 0.09, num_splits=3, kv_scales=s)
+    torch.cuda.current_stream().wait_stream(st)
+    check_out(other, out, absv)
+    # captured with other lengths, replayed twice, weights added twice
+    m = mass[0].cuda()
+    lg = torch.zeros_like(l)
+    g = torch.cuda.CUDAGraph()
+    res = ops.paged_decode_attention(q, c, wide, lg, 0.09, num_splits=0, kv_scales=s, mass=m)
+    with torch.cuda.graph(g):
+        res = ops.paged_decode_attention(q, c, wide, lg, 0.09, num_splits=0, kv_scales=s, mass=m)
+    lg.copy_(l)
+    g.replay()
+    g.replay()
+    check_out(res, out, absv)
+    check_mass(m, mass[0], [2 * x for x in w], bt, lens, 16, 128, big)
+    # two rows over the same blocks: both rows' weights arrive
+    bt2, l2 = bt.clone(), torch.tensor([200, 200, 64], dtype=torch.int32)
+    bt2[1] = bt2[0]
+    m = mass[0].cuda()
+    got = ops.paged_decode_attention(q, c, bt2.cuda(), l2.cuda(), 0.09, num_splits=0, kv_scales=s, mass=m)
+    out, w, absv, big = attend(q.cpu(), cache[0], scales[0], bt2, l2, 0.09)
+    check_out(got, out, absv)
+    check_mass(m, mass[0], w, bt2, l2, 16, 128, big)
+
+
+@pytest.mark.gpu
+def test_large_pool_offsets_gpu():
+    """Blocks whose byte offsets pass 2^32."""
+    Hk, D, bs = 8, 128, 16
+    NB = (1 << 32) // (2 * Hk * bs * D) + 200
+    cache = torch.zeros(NB, 2, Hk, bs, D, dtype=torch.int8, device="cuda")
+    scales = torch.full((NB, 2, Hk), 0.01, device="cuda")
+    mass = torch.zeros(NB, Hk, bs, device="cuda")
+    small, ssc, _, sbt, lens = filled("int8", [100, 50], Hk, D, bs, 17)
+    bt = torch.where(sbt > 0, NB - 1 - sbt, torch.zeros_like(sbt))
+    for i in set(sbt.flatten().tolist()) - {0}:
+        cache[NB - 1 - i], scales[NB - 1 - i] = small[0, i].cuda(), ssc[0, i].cuda()
+    q = torch.randn(2, 32, D, generator=torch.Generator().manual_seed(5)).bfloat16()
+    got = ops.paged_decode_attention(q.cuda(), cache, bt.cuda(), lens.cuda(), 0.09, num_splits=0, kv_scales=scales,
+                                     mass=mass)
+    out, w, absv, _ = attend(q, small[0], ssc[0], sbt, lens, 0.09)
+    check_out(got, out, absv)
+    assert abs(float(mass.double().sum()) - 64) < 1e-3
+    want = [small, ssc.clone(), torch.zeros(1, small.shape[1], Hk, bs)]
+    for i in set(sbt.flatten().tolist()) - {0}:
+        want[2][0, i] = mass[NB - 1 - i].cpu()
+    keep = torch.tensor([40, 33], dtype=torch.int32)
+    k1 = ops.kv_evict(*want, sbt, lens, keep, 4, 8, max_keep=40)
+    k2 = ops.kv_evict(cache, scales, mass, bt.cuda(), lens.cuda(), keep.cuda(), 4, 8, max_keep=40)
+    assert torch.equal(k2.cpu(), k1[0])
+    for i in set(sbt.flatten().tolist()) - {0}:
+        assert torch.equal(cache[NB - 1 - i].cpu(), want[0][0, i])
+
+
+# ------------------------------------------------------------------------------------------- prompts
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D,G,bs,window", [(128, 4, 16, 0), (64, 7, 16, 0), (128, 2, 32, 0), (64, 1, 64, 50),
+                                           (32, 2, 16, 0), (256, 2, 16, 0)])
+def test_prefill_gpu(kind, D, G, bs, window):
+    Hk = 2
+    lens, new = [1, 130, 257, 40, 500], [1, 130, 2, 17, 133]
+    cache, scales, _, bt, sl = filled(kind, lens, Hk, D, bs, 19)
+    cache, scales = cache[0], scales[0]
+    qs = torch.tensor([0] + new).cumsum(0).int()
+    q = (torch.randn(int(qs[-1]), Hk * G, D, generator=torch.Generator().manual_seed(6)) * 0.5).bfloat16()
+    scale = 1 / math.sqrt(D)
+    got = ops.paged_prefill_attention(q.cuda(), cache.cuda(), bt.cuda(), sl.cuda(), qs.cuda(), scale, window=window,
+                                      kv_scales=scales.cuda()).double().cpu()
+    for b, n in enumerate(new):
+        rows = torch.arange(lens[b] - n + 1, lens[b] + 1, dtype=torch.int32)
+        out, _, absv, _ = attend(q[qs[b]:qs[b + 1]], cache, scales, bt[b:b + 1].expand(n, -1), rows, scale, window)
+        # the prompt kernels hold p in bf16 (half a step 2^-8)
+        err = (got[qs[b]:qs[b + 1]] - out).abs()
+        assert bool((err <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all()), (b, float((err / absv).max()))
+
+
+def test_gather_cpu_behind_the_end():
+    cache, scales, _, bt, lens = filled("e4m3", [5, 70], 2, 32, 32, 23)
+    tmp, table = ops.kv_dequant_blocks(cache[0], scales[0], bt, lens)
+    x = tmp[table.long()].permute(0, 3, 2, 1, 4, 5)                    # [n, Hk, 2, mb16, 16, D]
+    flat = x.reshape(2, 2, 2, -1, 32)
+    want = values(cache[0], scales[0])[bt.long()].permute(0, 3, 2, 1, 4, 5).reshape(2, 2, 2, -1, 32)
+    for b, l in enumerate([5, 70]):
+        assert torch.equal(flat[b, :, :, :l].double(), want[b, :, :, :l]) and not bool(flat[b, :, :, l:].any())
+
+
+# ------------------------------------------------------------------------------------------- eviction
+def evict_oracle(cache, scales, mass, bt, lens, keep, sink, recent, max_keep, kind):
+    num, sc, ms = numbers(cache), scales.double().clone(), mass.clone()
+    n0, s0, m0 = num.clone(), sc.clone(), ms.clone()
+    Ly, _, _, Hk, bs, D = cache.shape
+    kept = torch.full((Ly, len(lens), Hk, max_keep), -1, dtype=torch.int32)
+    for b, L in enumerate(lens.tolist()):
+        K = min(max(int(keep[b]), 0), L)
+        if K == L:
+            kept[:, b, :, : min(L, max_keep)] = torch.arange(min(L, max_keep), dtype=torch.int32)
+            continue
+        K = min(K, max_keep)
+        a = min(sink, K)
+        r = min(recent, K - a)
+        for ly in range(Ly):
+            for h in range(Hk):
+                w = [float(m0[ly, bt[b, t // bs], h, t % bs]) for t in range(L)]
+                mid = sorted(range(a, L - r), key=lambda t: (-(w[t] if w[t] == w[t] else 0.0), t))[: K - a - r]
+                take = list(range(a)) + sorted(mid) + list(range(L - r, L))
+                kept[ly, b, h, :K] = torch.tensor(take, dtype=torch.int32)
+                for j0 in range(0, K, bs):
+                    part = take[j0:j0 + bs]
+                    blk = int(bt[b, j0 // bs])
+                    for kvi in range(2):
+                        v = torch.stack([n0[ly, bt[b, t // bs], kvi, h, t % bs] * s0[ly, bt[b, t // bs], kvi, h] for t in part])
+                        s = least_scale(float(v.abs().max()), kind)
+                        sc[ly, blk, kvi, h] = s
+                        num[ly, blk, kvi, h, : len(part)] = nearest(v / s, kind)
+                    for i, t in enumerate(part):
+                        ms[ly, blk, h, i] = m0[ly, bt[b, t // bs], h, t % bs]
+    return kept, num, sc, ms
+
+
+def same(a, b):
+    return torch.equal(a.nan_to_num(1.25e33), b.nan_to_num(1.25e33))
+
+
+def evict_case(kind, D, bs, seed, layers=2, Hk=2):
+    lens = [5 * bs + 3, 40, 1, 0, 2 * bs, 100]
+    keep = [2 * bs + 5, 39, 0, 0, 5 * bs, 1]
+    cache, scales, mass, bt, sl = filled(kind, lens, Hk, D, bs, seed, layers)
+    g = torch.Generator().manual_seed(seed)
+    mass = torch.where(torch.rand(mass.shape, generator=g) < 0.4, torch.round(mass * 4) / 4, mass)   # many ties
+    mass[0, bt[0, 1], 0, 2] = math.nan
+    mass[0, bt[0, 2], 1, 1] = math.inf
+    mass[0, bt[0, 2], 0, 3] = -0.0
+    return cache, scales, mass, bt, sl, torch.tensor(keep, dtype=torch.int32)
+
+
+EVICT = [(4, 8, None), (0, 0, None), (1000, 3, None), (2, 1000, None), (3, 5, 20)]
+
+
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("sink,recent,max_keep", EVICT)
+def test_evict_cpu(kind, sink, recent, max_keep):
+    c = evict_case(kind, 32, 16, 29)
+    want = evict_oracle(*c, sink, recent, max_keep or c[3].shape[1] * 16, kind)
+    got = ops.kv_evict(*c, sink, recent, max_keep=max_keep)
+    assert torch.equal(got, want[0]) and same(numbers(c[0]), want[1])
+    assert same(c[1].double(), want[2]) and same(c[2], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (96, 16), (256, 64), (32, 16)])
+@pytest.mark.parametrize("sink,recent,max_keep", EVICT)
+def test_evict_gpu(kind, D, bs, sink, recent, max_keep):
+    c = evict_case(kind, D, bs, 31)
+    want = evict_oracle(*c, sink, recent, max_keep or c[3].shape[1] * bs, kind)
+    d = [x.cuda() for x in c]
+    got = ops.kv_evict(*d, sink, recent, max_keep=max_keep)
+    assert torch.equal(got.cpu(), want[0]) and same(numbers(d[0].cpu()), want[1])
+    assert same(d[1].cpu().double(), want[2]) and same(d[2].cpu(), want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("L,K,ties", [(3000, 2000, False), (20000, 5000, True), (40000, 39999, False)])
+def test_evict_long_gpu(L, K, ties):
+    """Many chunks moved over one another; sequences whose weights do not fit on chip; a single layer's tensors."""
+    Hk, D, bs = 1, 64, 16
+    c = filled("int8", [L], Hk, D, bs, 37)
+    cache, scales, mass, bt, sl = c[0][0], c[1][0], c[2][0], c[3], c[4]
+    mass = torch.round(mass * 50) / 50 if ties else mass
+    keep = torch.tensor([K], dtype=torch.int32)
+    d = [x.cuda() for x in (cache, scales, mass, bt, sl, keep)]
+    want = ops.kv_evict(cache, scales, mass, bt, sl, keep, 16, 100, max_keep=K)
+    got = ops.kv_evict(*d, 16, 100, max_keep=K)
+    assert torch.equal(got.cpu(), want) and torch.equal(d[0].cpu(), cache)
+    assert same(d[1].cpu(), scales) and same(d[2].cpu(), mass)
+
+
+# ------------------------------------------------------------------------------------------- together
+def together(kind, dev, steps=40):
+    """A sequence grows token by token, is weighed, evicted and grows on; returns every output and the final cache."""
+    Hk, G, D, bs = 2, 4, 64, 16
+    g = torch.Generator().manual_seed(41)
+    NB = 12
+    cache = torch.zeros(NB, 2, Hk, bs, D, dtype=KINDS[kind], device=dev)
+    scales = torch.zeros(NB, 2, Hk, device=dev)
+    mass = torch.zeros(NB, Hk, bs, device=dev)
+    bt = torch.tensor([[7, 3, 9, 1, 5, 2]], dtype=torch.int32)
+    n, outs = 0, []
+
+    def put(k):
+        nonlocal n
+        pos = torch.arange(n, n + k)
+        slots = (bt[0].long()[pos // bs] * bs + pos % bs).int()
+        kv = (torch.randn(k, 2, Hk, D, generator=g) * torch.exp2(torch.rand(k, 2, Hk, 1, generator=g) * 4)).bfloat16()
+        ops.kv_quant_blocks(kv.to(dev), slots.to(dev), cache, scales, mass=mass)
+        n += k
+
+    put(37)
+    for i in range(steps):
+        q = (torch.randn(1, Hk * G, D, generator=g) * 0.3).bfloat16()
+        outs.append(ops.paged_decode_attention(q.to(dev), cache, bt.to(dev), torch.tensor([n], dtype=torch.int32).to(dev),
+                                               0.125, num_splits=0, kv_scales=scales, mass=mass).float().cpu())
+        if n > 60:
+            kept = ops.kv_evict(cache, scales, mass, bt.to(dev), torch.tensor([n], dtype=torch.int32).to(dev),
+                                torch.tensor([35], dtype=torch.int32).to(dev), 4, 10, max_keep=35)
+            outs.append(kept.float().cpu())
+            n = 35
+        put(1)
+    return outs, cache.cpu(), scales.cpu(), mass.cpu()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_write_weigh_evict_together_gpu(kind):
+    a, b = together(kind, "cpu"), together(kind, "cuda")
+    # the same tokens stay (weights differ in their last bits only), so codes and scales are equal
+    assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+    torch.testing.assert_close(b[3], a[3], rtol=1e-4, atol=1e-6)
+    for x, y in zip(b[0], a[0]):
+        # both sides round to bf16 (half a step 2^-8 each)
+        torch.testing.assert_close(x, y, rtol=2 * 2.0 ** -8, atol=2.0 ** -6)
+
+
+# ------------------------------------------------------------------------------------------- refusals
+def refusals(dev):
+    cache, scales, mass, bt, lens = [x.to(dev) for x in filled("int8", [20, 30], 2, 64, 16, 43)]
+    cache, scales, mass = cache[0], scales[0], mass[0]
+    dt = torch.bfloat16
+    q, kv = torch.zeros(2, 4, 64, dtype=dt, device=dev), torch.zeros(2, 2, 2, 64, dtype=dt, device=dev)
+    slots = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    keep = torch.tensor([5, 5], dtype=torch.int32, device=dev)
+    bad = (ValueError, RuntimeError)
+
+    def no(f, *a, **k):
+        with pytest.raises(bad):
+            f(*a, **k)
+
+    dec, wr, ev = ops.paged_decode_attention, ops.kv_quant_blocks, ops.kv_evict
+    no(dec, q, cache.float(), bt, lens, 1.0, kv_scales=scales)                      # not 8 bits
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales[:-1].contiguous())            # fewer blocks
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales.double())
+    no(dec, q[..., :32].contiguous(), cache, bt, lens, 1.0, kv_scales=scales)       # another head size
+    no(dec, q[:, :3].contiguous(), cache, bt, lens, 1.0, kv_scales=scales)          # heads not a multiple
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales, mass=mass[:, :1].contiguous())
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales, mass=mass.half())
+    no(dec, q, torch.zeros(8, 2, 2, 16, 64, dtype=dt, device=dev), bt, lens, 1.0, mass=mass)   # weights of a bf16 cache
+    no(dec, q, cache[:, :, :, :8].contiguous(), bt, lens, 1.0, kv_scales=scales)    # blocks of 8 tokens
+    no(wr, kv[..., :32].contiguous(), slots, cache, scales)
+    no(wr, kv, slots[:1], cache, scales)
+    no(wr, kv, slots, cache.float(), scales)
+    no(wr, kv, slots, cache, scales, mass=mass[:-1].contiguous())
+    no(ev, cache, scales, mass, bt, lens, keep, -1, 3)
+    no(ev, cache, scales, mass, bt, lens, keep, 1, -3)
+    no(ev, cache, scales, mass, bt, lens, keep, 1, 3, max_keep=-1)
+    no(ev, cache, scales, mass.double(), bt, lens, keep, 1, 3)
+    no(ev, cache, scales[None], mass, bt, lens, keep, 1, 3)
+    return cache, scales, mass, bt, lens, q, kv, slots, keep, no
+
+
+def test_refusals_cpu():
+    refusals("cpu")
+    cache, scales, mass, bt, lens = filled("int8", [40], 2, 64, 16, 43)
+    with pytest.raises(ValueError):      # rows of one block that are not neighbours
+        ops.kv_quant_blocks(torch.zeros(3, 2, 2, 64), torch.tensor([16, 32, 17], dtype=torch.int32), cache[0], scales[0])
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    cache, scales, mass, bt, lens, q, kv, slots, keep, no = refusals("cuda")
+    dec = ops.paged_decode_attention
+    no(dec, q.float(), cache, bt, lens, 1.0, kv_scales=scales)
+    no(dec, q, cache, bt.long(), lens, 1.0, kv_scales=scales)
+    no(dec, q, cache, bt, lens.cpu(), 1.0, kv_scales=scales)
+    no(dec, q, cache, bt[:1], lens, 1.0, kv_scales=scales)
+    no(dec, q, cache, bt, lens, 1.0, num_splits=65, kv_scales=scales)
+    no(dec, q, cache, bt, lens, 1.0, num_splits=4, kv_scales=scales, workspace=torch.empty(8, device="cuda"))
+    no(dec, q, cache.transpose(0, 2), bt, lens, 1.0, kv_scales=scales)
+    no(ops.kv_quant_blocks, kv.float(), slots, cache, scales)
+    no(ops.kv_quant_blocks, kv, slots.long(), cache, scales)
+    no(ops.kv_evict, cache, scales, mass, bt, lens, keep.long(), 1, 3)
+    no(ops.kv_evict, cache, scales, mass, bt, lens.cpu(), keep, 1, 3)
+    z = torch.zeros(4, 2, 2, 16, 48, dtype=torch.int8, device="cuda")
+    no(dec, torch.zeros(2, 4, 48, dtype=torch.bfloat16, device="cuda"), z, bt * 0, lens, 1.0, kv_scales=scales[:4].contiguous())
+
+
+@pytest.mark.gpu
+def test_bad_indices_are_reported_gpu():
+    """With bounds checking on, block ids and slots outside the pool are reported and nothing else is written."""
+    cache, scales, mass, bt, lens = [x.cuda() for x in filled("int8", [40, 33], 2, 64, 16, 47)]
+    cache, scales, mass = cache[0], scales[0].nan_to_num(0.5), mass[0]
+    NB = cache.shape[0]
+    before = cache.clone()
+    with ops.BoundsCheck() as bc:
+        kv = torch.randn(2, 2, 2, 64, device="cuda").bfloat16()
+        ops.kv_quant_blocks(kv, torch.tensor([NB * 16, -1], dtype=torch.int32, device="cuda"), cache, scales)
+        torch.cuda.synchronize()
+        assert bc.status() == (4, NB) and torch.equal(cache, before)
+        bc.reset()
+        bad = bt.clone()
+        bad[0, 1] = NB + 7
+        out = ops.paged_decode_attention(torch.randn(2, 4, 64, device="cuda").bfloat16(), cache, bad, lens, 0.1,
+                                         num_splits=0, kv_scales=scales)
+        assert bc.status() == (4, NB + 7) and bool(torch.isfinite(out).all())
