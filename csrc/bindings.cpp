@@ -1,7 +1,9 @@
 // Python bindings of the sm_100a kernels (module gollek_b200_C).
 //
 // All torch-tensor validation happens here (compiled by the host compiler); the .cu files
-// only see raw pointers, strides and the current CUDA stream.
+// only see raw pointers, strides and the current CUDA stream. Messages carry numbers as
+// std::to_string: the module may be linked with a C++ library of its own, and formatting a number through
+// the stream operators of torch's message builder then ends the process instead of raising.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -242,7 +244,7 @@ void gemm_bf16_out(torch::Tensor out, torch::Tensor a, torch::Tensor b, c10::opt
   if (sp > 1) {
     TORCH_CHECK(workspace.has_value() && workspace->is_cuda() && workspace->scalar_type() == at::kFloat &&
                     workspace->numel() >= (int64_t)sp * M * N,
-                "gemm: split-K ", sp, " needs an fp32 workspace of ", (int64_t)sp * M * N, " elements");
+                "gemm: split-K ", std::to_string(sp), " needs an fp32 workspace of ", std::to_string((int64_t)sp * M * N), " elements");
     part = workspace->data_ptr<float>();
   }
   launch_gemm_bf16(out.data_ptr(), out.stride(0), a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), rp, ldr, M,
@@ -309,7 +311,7 @@ void moe_forward_out(torch::Tensor out, torch::Tensor x, torch::Tensor router, t
   if (splits > 1) {
     TORCH_CHECK(ypart.has_value() && ypart->is_cuda() && ypart->scalar_type() == at::kFloat &&
                     ypart->numel() >= (int64_t)splits * cap * H,
-                "moe: split-K down projection needs an fp32 buffer of ", (int64_t)splits * cap * H, " elements");
+                "moe: split-K down projection needs an fp32 buffer of ", std::to_string((int64_t)splits * cap * H), " elements");
     yq = ypart->data_ptr<float>();
   }
   launch_moe_forward(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0), router.data_ptr(), w_gu.data_ptr(),
@@ -934,14 +936,14 @@ void gemm_fp8_py(torch::Tensor out, torch::Tensor a, torch::Tensor sa, torch::Te
   if (sp > 1) {
     TORCH_CHECK(workspace.has_value() && workspace->scalar_type() == at::kFloat &&
                     workspace->numel() >= (int64_t)sp * M * N,
-                "fp8 gemm: split-K ", sp, " needs an fp32 workspace of ", (int64_t)sp * M * N, " elements");
+                "fp8 gemm: split-K ", std::to_string(sp), " needs an fp32 workspace of ", std::to_string((int64_t)sp * M * N), " elements");
     part = workspace->data_ptr<float>();
   }
   int* cnt = nullptr;
   if (sp > 1 && tile_cnt.has_value()) {
     const int64_t tiles = (int64_t)((M + 127) / 128) * (N / 128);
     TORCH_CHECK(tile_cnt->is_cuda() && tile_cnt->scalar_type() == at::kInt && tile_cnt->numel() >= tiles,
-                "fp8 gemm: ", tiles, " zeroed int32 tile counters expected");
+                "fp8 gemm: ", std::to_string(tiles), " zeroed int32 tile counters expected");
     cnt = tile_cnt->data_ptr<int>();
   }
   launch_gemm_fp8(out.data_ptr(), out.stride(0), a.data_ptr(), a.stride(0), sa.data_ptr<float>(), b.data_ptr(),
@@ -999,7 +1001,7 @@ void gemm_q4k_py(torch::Tensor out, torch::Tensor a, torch::Tensor w, int64_t N,
   float* part = nullptr;
   if (sp > 1) {
     TORCH_CHECK(workspace.has_value() && workspace->scalar_type() == at::kFloat && workspace->numel() >= (int64_t)sp * M * N,
-                "q4k gemm: split-K ", sp, " needs an fp32 workspace of ", (int64_t)sp * M * N, " elements");
+                "q4k gemm: split-K ", std::to_string(sp), " needs an fp32 workspace of ", std::to_string((int64_t)sp * M * N), " elements");
     part = workspace->data_ptr<float>();
   }
   launch_gemm_q4k(out.data_ptr(), out.stride(0), a.data_ptr(), a.stride(0), w.data_ptr(), M, (int)N, (int)K, (int)epi,

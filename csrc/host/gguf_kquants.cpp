@@ -418,7 +418,7 @@ Fmt fmt_of(int64_t t) {
     case 11: return {QKK, 110, deq_q3_k, q_q3_k};
     case 13: return {QKK, 176, deq_q5_k, q_q5_k};
     case 14: return {QKK, 210, deq_q6_k, q_q6_k};
-    default: TORCH_CHECK(false, "ggml type ", t, " is not handled here");
+    default: TORCH_CHECK(false, "ggml type ", std::to_string(t), " is not handled here");
   }
 }
 
