@@ -43,8 +43,9 @@ def parse(argv=None):
     p.add_argument("--decode-steps", type=int, default=64)
     p.add_argument("--skip-prefill", action="store_true", help="llama70b-fp8: decode only, no prefill sweep")
     p.add_argument("--scale", type=float, default=1.0, help="shrink batch / lengths (small runs)")
-    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8"],
-                   help="llama70b-fp8: KV cache in the model dtype, or fp8 e4m3 with a scale per token and head")
+    p.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8", "int8", "fp8_block"],
+                   help="llama70b-fp8: KV cache in the model dtype, fp8 e4m3 with a scale per token and head, or "
+                        "int8 / e4m3 with a scale per block and head")
     p.add_argument("--comm", default="fused", choices=["fused", "nccl"],
                    help="TP collectives: fused P2P kernels over the IPC heap, or NCCL")
     return p.parse_args(argv)

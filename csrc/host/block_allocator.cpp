@@ -178,6 +178,19 @@ class SeqTables {
     dropped_[seq] += (int64_t)idx.size() * pool_->block_size();
     return (int64_t)idx.size();
   }
+  // KV eviction by token: of the sequence's `tokens` cached tokens `kept` now lie together at the front of
+  // its blocks. Blocks behind them are released, later tokens keep their logical positions.
+  int64_t compact(int64_t seq, int64_t tokens, int64_t kept) {
+    auto& t = at(seq);
+    const int64_t bs = pool_->block_size();
+    if (kept < 1 || kept > tokens || tokens > (int64_t)t.size() * bs)
+      throw std::out_of_range("SeqTables.compact: 1 <= kept <= tokens <= capacity");
+    const int64_t need = (kept + bs - 1) / bs, freed = (int64_t)t.size() - need;
+    for (int64_t i = (int64_t)t.size() - 1; i >= need; --i) pool_->decref(t[i]);
+    t.resize(need);
+    dropped_[seq] += tokens - kept;
+    return freed;
+  }
   int64_t dropped(int64_t seq) const {
     auto it = dropped_.find(seq);
     return it == dropped_.end() ? 0 : it->second;
@@ -306,5 +319,6 @@ void register_block_allocator(pybind11::module& m) {
       .def("blocks_needed", &SeqTables::blocks_needed)
       .def("build_batch", &SeqTables::build_batch)
       .def("drop", &SeqTables::drop)
+      .def("compact", &SeqTables::compact)
       .def("dropped", &SeqTables::dropped);
 }

@@ -614,13 +614,18 @@ class EngineConfig:
     block_size: int = 16
     num_gpu_blocks: Optional[int] = None      # None => size from memory fraction
     gpu_memory_utilization: float = 0.85
-    kv_cache_dtype: str = "auto"              # auto (= model dtype) | fp8 (e4m3, a scale per token and head)
+    # auto (= model dtype) | fp8 (e4m3, a scale per token and head) | int8 or fp8_block (8-bit codes with one
+    # power-of-two scale per block and head)
+    kv_cache_dtype: str = "auto"
     enable_prefix_caching: bool = True
     # KV eviction under memory pressure (opt-in; changes outputs): when the block pool is more than
     # `kv_eviction_threshold` full, the longest running sequences drop their least important KV
     # blocks (key-norm + recency score) down to `kv_retention_target` of their blocks; the first
     # `kv_protect_sink_blocks` blocks and the most recent `kv_protect_recent` fraction are kept
     kv_eviction: bool = False
+    # what is dropped: "key_norm" drops whole blocks; "attention" keeps, in every layer and KV head, the tokens that
+    # drew the most attention weight while decoding (needs kv_cache_dtype int8 or fp8_block, turns prefix caching off)
+    kv_eviction_policy: str = "key_norm"
     kv_eviction_threshold: float = 0.85
     kv_retention_target: float = 0.6
     kv_protect_sink_blocks: int = 1

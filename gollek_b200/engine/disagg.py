@@ -57,7 +57,7 @@ def export_sequence(engine, seq: Sequence, model_id: str = "") -> KVHandoff:
     blocks = engine.kv.tables.blocks(seq.seq_id)[:nb]
     ids = torch.tensor(blocks, dtype=torch.int32)
     if getattr(engine.model, "kv_scales", None) is not None:
-        raise ValueError("moving KV blocks of an fp8 cache (values + per-token scales) is not supported")
+        raise ValueError("moving KV blocks of an 8-bit cache (codes + scales) is not supported")
     kv = ops.kv_gather_blocks(engine.kv_cache, ids.to(engine.kv_cache.device))
     return KVHandoff(seq.request_id, model_id or str(engine.cfg.model), list(seq.prompt_token_ids),
                      list(seq.output_token_ids), dataclasses.asdict(seq.params), engine.cfg.block_size, kv,
@@ -69,6 +69,8 @@ def import_sequence(engine, h: KVHandoff) -> Sequence:
     freshly allocated blocks; it joins the running batch at its next decode step."""
     if h.block_size != engine.cfg.block_size:
         raise ValueError("prefill and decode engines must use the same KV block size")
+    if getattr(engine.model, "kv_scales", None) is not None:
+        raise ValueError("a hand-off's blocks cannot be adopted by an 8-bit cache (codes + scales)")
     exp = engine.model.kv_cache_shape(h.kv.shape[1], h.block_size)
     if tuple(h.kv.shape) != (exp[0], h.kv.shape[1]) + tuple(exp[2:]):
         raise ValueError(f"KV layout mismatch: got {tuple(h.kv.shape)}, this model stores {exp}")

@@ -95,7 +95,25 @@ class LLMEngine:
             cfg.enable_prefix_caching = False
             cfg.use_cuda_graphs = False
             self.model.alloc_gdn_state(cfg.max_num_seqs + 1)
-        # ---- KV cache (bf16, or fp8 e4m3 with a scale per token and head)
+        # ---- KV cache (bf16; fp8 e4m3 with a scale per token and head; int8 / e4m3 with a scale per block)
+        kv_block8 = {"int8": torch.int8, "fp8_block": torch.uint8}.get(cfg.kv_cache_dtype)
+        weigh = cfg.kv_eviction and cfg.kv_eviction_policy == "attention"
+        if cfg.kv_eviction_policy not in ("key_norm", "attention"):
+            raise ValueError(f"kv_eviction_policy {cfg.kv_eviction_policy!r}: key_norm or attention")
+        if kv_block8 is not None:
+            if model_cfg.is_mla or (self.device.type == "cuda" and self.model.D not in (32, 64, 128, 256)):
+                raise ValueError("block-scaled KV cache: head_dim 32, 64, 128 or 256 (no MLA)")
+            if cfg.block_size not in (16, 32, 64):
+                raise ValueError("block-scaled KV cache: block size 16, 32 or 64")
+            if cfg.kv_eviction and not weigh:
+                raise ValueError("block-scaled KV cache: eviction is by attention weight (kv_eviction_policy attention)")
+            self.model.kv_block8 = True
+        elif weigh:
+            raise ValueError("kv_eviction_policy attention needs a block-scaled KV cache (kv_cache_dtype int8 or fp8_block)")
+        if weigh:
+            if cfg.speculative_method != "none":
+                raise ValueError("kv_eviction_policy attention: rejected drafts would weigh the cache; not supported")
+            cfg.enable_prefix_caching = False  # tokens move between blocks: none may be shared
         kv_fp8 = cfg.kv_cache_dtype in ("fp8", "fp8_e4m3")
         if kv_fp8:
             if self.model.D != 128 or model_cfg.is_mla:
@@ -104,6 +122,8 @@ class LLMEngine:
                 raise ValueError("kv_cache_dtype fp8: KV eviction moves blocks without their scales; not supported")
             self.model.kv_fp8 = True
         bpb = self.model.kv_bytes_per_block(cfg.block_size)
+        if weigh:  # fp32 attention weight per token, layer and KV head
+            bpb += max(1, self.model.num_kv_layers) * self.model.Hk * cfg.block_size * 4
         nb = num_blocks or cfg.num_gpu_blocks
         if nb is None:
             if self.device.type == "cuda":
@@ -116,7 +136,11 @@ class LLMEngine:
             nb = int(t)
         self.num_blocks = nb
         shape = self.model.kv_cache_shape(nb, cfg.block_size)
-        self.kv_cache = allocate_kv_cache(shape, torch.uint8 if kv_fp8 else self.dtype, self.device)
+        self.kv_cache = allocate_kv_cache(shape, kv_block8 or (torch.uint8 if kv_fp8 else self.dtype), self.device)
+        if kv_block8 is not None:
+            self.model.kv_scales = allocate_kv_cache(shape[:4], torch.float32, self.device)
+            if weigh:
+                self.model.kv_mass = allocate_kv_cache((shape[0], nb, *shape[3:5]), torch.float32, self.device)
         if kv_fp8:
             self.model.kv_scales = allocate_kv_cache(shape[:-1], torch.float32, self.device)
         if cfg.speculative_method == "draft" and cfg.enable_prefix_caching:
@@ -145,8 +169,8 @@ class LLMEngine:
         self.runner = ModelRunner(self.model, cfg, self.kv_cache, self.kv)
         if getattr(cfg, "gc_tuning", False):
             _tune_gc()
-        if cfg.kv_cache_dtype not in ("auto", cfg.dtype, "fp8", "fp8_e4m3"):
-            raise ValueError(f"kv_cache_dtype {cfg.kv_cache_dtype!r}: auto (the model dtype) or fp8 (e4m3)")
+        if cfg.kv_cache_dtype not in ("auto", cfg.dtype, "fp8", "fp8_e4m3", "int8", "fp8_block"):
+            raise ValueError(f"kv_cache_dtype {cfg.kv_cache_dtype!r}: auto (the model dtype), fp8 (e4m3), int8 or fp8_block")
         self.evictor = None
         if cfg.kv_eviction:
             from .evicpress import KVEvictor
@@ -155,7 +179,7 @@ class LLMEngine:
             if model_cfg.sliding_window or model_cfg.layer_types:
                 raise ValueError("kv_eviction: not supported with sliding-window layers")
             self.evictor = KVEvictor(cfg.kv_eviction_threshold, cfg.kv_retention_target, cfg.kv_protect_sink_blocks,
-                                     cfg.kv_protect_recent, cfg.kv_eviction_min_blocks)
+                                     cfg.kv_protect_recent, cfg.kv_eviction_min_blocks, cfg.kv_eviction_policy)
         self.seqs: Dict[str, Sequence] = {}
         self.metrics = EngineMetrics()
         self.eos_token_id = model_cfg.eos_token_id

@@ -17,8 +17,12 @@ Design here:
   act      the lowest-importance unprotected blocks are dropped until the sequence keeps
            ``retention_target`` of its blocks. Dropping is a block-table edit in the native
            allocator (``SeqTables.drop``): later tokens keep their positions (RoPE), their KV slots
-           shift down, and attention runs over the kept blocks. Compression to a narrower dtype is
-           not offered: the attention kernels read bf16 blocks only.
+           shift down, and attention runs over the kept blocks.
+With ``policy="attention"`` (block-scaled 8-bit cache) the unit is the token, and every layer and KV
+head chooses for itself: decoding queries add their softmax weights to a mass per cached token
+(``ops.paged_decode_attention(mass=)``; a prompt chunk's last query counts as one), and
+``ops.kv_evict`` keeps the sink and recent tokens plus the rest's heaviest, moved together at the front
+of the sequence's blocks; the blocks behind them are released (``SeqTables.compact``).
 Eviction is approximate attention and off by default. Sequences that lost blocks stop adding blocks
 to the prefix cache (their block hashes no longer describe a contiguous prefix).
 """
@@ -53,6 +57,7 @@ class KVEvictor:
     sink_blocks: int = 1
     recent: float = 0.2
     min_blocks: int = 8
+    policy: str = "key_norm"
     stats: EvictionStats = field(default_factory=EvictionStats)
 
     def __post_init__(self):
@@ -98,6 +103,8 @@ class KVEvictor:
         if not force and not self.over_threshold(kv):
             return 0
         self.stats.cycles += 1
+        if self.policy == "attention":
+            return self._run_attention(engine, force)
         freed = 0
         cache = engine.kv_cache
         running = [q for q in engine.scheduler.running if kv.has(q)]
@@ -117,4 +124,45 @@ class KVEvictor:
             self.stats.sequences += 1
             self.stats.blocks_dropped += len(drop)
             self.stats.blocks_kept += nb - len(drop)
+        return freed
+
+    def _run_attention(self, engine, force: bool) -> int:
+        """The longest sequences (as many as bring the pool under the threshold; with ``force`` all
+        eligible ones) keep ``retention_target`` of their blocks' worth of tokens, chosen by attention
+        weight per layer and head, in one call. Returns blocks freed."""
+        kv = engine.kv
+        bs = kv.block_size
+        rows, used = [], kv.num_blocks - kv.num_free_blocks()
+        running = [q for q in engine.scheduler.running if kv.has(q)]
+        for seq in sorted(running, key=lambda q: -kv.tables.num_blocks(q.seq_id)):
+            if not force and used / max(1, kv.num_blocks) < self.threshold:
+                break
+            nb = kv.tables.num_blocks(seq.seq_id)
+            tokens = seq.num_computed_tokens - kv.dropped_tokens(seq)
+            keep = max(1, math.ceil(self.retention_target * nb)) * bs
+            if nb < self.min_blocks or keep >= tokens:
+                continue
+            rows.append((seq, nb, tokens, keep))
+            used -= nb - keep // bs
+        if not rows:
+            return 0
+        bt = torch.zeros(len(rows), max(nb for _, nb, _, _ in rows), dtype=torch.int32)
+        for i, (seq, nb, _, _) in enumerate(rows):
+            bt[i, :nb] = torch.tensor(kv.tables.blocks(seq.seq_id), dtype=torch.int32)
+        dev = engine.kv_cache.device
+        lens = torch.tensor([r[2] for r in rows], dtype=torch.int32)
+        keep = torch.tensor([r[3] for r in rows], dtype=torch.int32)
+        # one recent window for the call: the shortest sequence's share
+        recent = max(1, min(math.ceil(self.recent * r[2]) for r in rows))
+        m = engine.model
+        ops.kv_evict(engine.kv_cache, m.kv_scales, m.kv_mass, bt.to(dev), lens.to(dev), keep.to(dev),
+                     self.sink_blocks * bs, recent, max_keep=int(keep.max()))
+        freed = 0
+        for seq, nb, tokens, kept in rows:
+            got = kv.compact(seq, tokens, kept)
+            freed += got
+            self.stats.sequences += 1
+            self.stats.blocks_scored += nb
+            self.stats.blocks_dropped += got
+            self.stats.blocks_kept += nb - got
         return freed

@@ -117,6 +117,11 @@ class KVCacheManager:
         del seq.block_hashes[min(idx):]
         return n
 
+    def compact(self, seq: Sequence, tokens: int, kept: int) -> int:
+        """KV eviction by token: of the sequence's ``tokens`` cached tokens ``kept`` now lie together at the
+        front of its blocks; the blocks behind them are released. Returns blocks freed."""
+        return self.tables.compact(seq.seq_id, tokens, kept)
+
     def dropped_tokens(self, seq: Sequence) -> int:
         return self.tables.dropped(seq.seq_id) if self.tables.has(seq.seq_id) else 0
 

@@ -86,6 +86,7 @@ class ModelRunner:
         self.is_cuda = self.device.type == "cuda"
         self.block_size = cfg.block_size
         self.max_blocks = (cfg.max_model_len + cfg.block_size - 1) // cfg.block_size
+        self.pad_len = 0 if model.kv_block8 else 1  # KV length of padding rows in captured batches
         k_spec = cfg.num_speculative_tokens if cfg.speculative_method != "none" else 0
         max_tokens = cfg.max_num_batched_tokens + cfg.max_num_seqs * (1 + k_spec)
         self.host = _Pinned(max_tokens, cfg.max_num_seqs, self.max_blocks, self.is_cuda,
@@ -610,7 +611,8 @@ class ModelRunner:
         g.positions = torch.zeros(bs, dtype=torch.int32, device=dev)
         g.slots = torch.full((bs,), -1, dtype=torch.int32, device=dev)
         g.block_tables = torch.zeros(bs, self.max_blocks, dtype=torch.int32, device=dev)
-        g.seq_lens = torch.ones(bs, dtype=torch.int32, device=dev)
+        # the warm-up rows own no block: length 1 reads block 0, or length 0 where reading would also weigh it
+        g.seq_lens = torch.full((bs,), self.pad_len, dtype=torch.int32, device=dev)
         splits = self._decode_splits(bs, self.cfg.max_model_len)
         g.workspace = torch.empty(bs * self.model.H * max(1, splits) * (self.model.D + 2),
                                   dtype=torch.float32, device=dev)
@@ -640,11 +642,11 @@ class ModelRunner:
         bs = g.bs
         self.h2d_bytes += 4 * bs * (4 + self.max_blocks)
         self.d2h_bytes += 8 * bs
-        # pad rows: slot -1 (no KV write), length 1, block 0
+        # pad rows: slot -1 (no KV write), length 1 (0 with a block-scaled cache), block 0
         if nd < bs:
             h.positions[nd:bs] = 0
             h.slots[nd:bs] = -1
-            h.seq_lens[nd:bs] = 1
+            h.seq_lens[nd:bs] = self.pad_len
             h.block_tables[nd:bs] = 0
             h.input_ids[nd:bs] = 0
         g.input_ids.copy_(h.input_ids[:bs], non_blocking=True)

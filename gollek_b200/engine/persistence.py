@@ -77,7 +77,7 @@ def save_prefix_cache(engine, path: str, max_blocks: int = 0, compress: str = ""
     hashes = torch.tensor([h for h, _ in items], dtype=torch.int64)
     ids = torch.tensor([b for _, b in items], dtype=torch.int32)
     if getattr(engine.model, "kv_scales", None) is not None:
-        raise ValueError("moving KV blocks of an fp8 cache (values + per-token scales) is not supported")
+        raise ValueError("moving KV blocks of an 8-bit cache (codes + scales) is not supported")
     kv = ops.kv_gather_blocks(engine.kv_cache, ids.to(engine.kv_cache.device))  # [L, n, 2, Hk, bs, D]
     meta = {"signature": json.dumps(_signature(engine))}
     if compress == "turboquant":
@@ -102,6 +102,8 @@ def load_prefix_cache(engine, path: str) -> int:
         hashes = f.get("hashes").tolist()
         if not hashes:
             return 0
+        if getattr(engine.model, "kv_scales", None) is not None:
+            raise ValueError("a snapshot's blocks cannot be adopted by an 8-bit cache (codes + scales)")
         compressed = f.metadata.get("compress") == "turboquant"
         kv = None if compressed else f.get("kv")  # [n, L, 2, Hk, bs, D]
         taken, rows = [], []

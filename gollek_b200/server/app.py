@@ -457,6 +457,7 @@ def create_app(aengine: AsyncEngine, model_name: str = "gollek-b200", api_keys: 
              "kv_utilization": e.kv.usage(), "eviction_enabled": ev is not None}
         if ev is not None:
             d.update({"eviction_threshold": ev.threshold, "retention_target": ev.retention_target,
+                      "eviction_policy": ev.policy,
                       **{f"total_{k}": v for k, v in ev.stats.as_dict().items()}})
         return d
 
