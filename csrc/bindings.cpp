@@ -777,41 +777,44 @@ void kv_dequant_scaled_py(torch::Tensor cache, torch::Tensor scales, torch::Tens
                            cur_stream());
 }
 
-void block8_decode_py(torch::Tensor out, torch::Tensor q, torch::Tensor cache, torch::Tensor scales,
-                      torch::Tensor tables, torch::Tensor lens, double scale, int64_t splits,
-                      c10::optional<torch::Tensor> workspace, int64_t window, double softcap,
-                      c10::optional<torch::Tensor> mass) {
+torch::Tensor block8_decode_py(torch::Tensor q, torch::Tensor cache, torch::Tensor scales, torch::Tensor tables,
+                               torch::Tensor lens, double scale, int64_t splits, c10::optional<torch::Tensor> out_opt,
+                               c10::optional<torch::Tensor> workspace, int64_t window, double softcap,
+                               c10::optional<torch::Tensor> mass) {
   const bool e4m3 = check_block8(cache, scales, false);
   check_bf16(q, "q");
-  check_bf16(out, "out");
   check_same_device(q, cache);
-  check_same_device(out, cache);
   TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) == q.size(2) && q.size(2) == cache.size(4),
               "q must be [B, H, D] with packed heads of the cache's D");
-  TORCH_CHECK(q.stride(0) % 4 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0, "q: rows at multiples of 8 bytes");
-  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes(), "out must be contiguous like q");
+  TORCH_CHECK(q.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q: rows at multiples of 16 bytes");
   const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = cache.size(2);
-  TORCH_CHECK(Hk > 0 && H % Hk == 0, "H must be a multiple of Hk");
-  TORCH_CHECK(splits >= 1 && splits <= 64, "block-scaled decode attention: 1 to 64 splits");
+  TORCH_CHECK(splits >= 0 && splits <= 64, "block-scaled decode attention: 0 (automatic) to 64 splits");
+  TORCH_CHECK(B <= INT32_MAX / 1024, "block-scaled decode attention: too many rows");
   check_rows(tables, lens, cache, B);
   float* mp = check_mass(mass, cache, 0);
-  float *po = nullptr, *pml = nullptr, *sc = nullptr;
-  const int64_t n_o = splits > 1 ? B * H * splits * D : 0, n_ml = (splits > 1 || mp) ? B * H * splits * 2 : 0;
-  const int64_t n_sc = mp ? B * H * tables.size(1) * cache.size(3) : 0;
-  if (n_o + n_ml + n_sc > 0) {
-    TORCH_CHECK(workspace.has_value() && workspace->is_cuda() && workspace->scalar_type() == at::kFloat &&
-                    workspace->is_contiguous() && workspace->numel() >= n_o + n_ml + n_sc,
-                "decode attention: fp32 workspace of ", std::to_string(n_o + n_ml + n_sc), " elements needed");
-    check_same_device(*workspace, cache);
-    po = workspace->data_ptr<float>();
-    pml = po + n_o;
-    sc = pml + n_ml;
-  }
   c10::cuda::CUDAGuard guard(cache.device());
+  const int64_t width = tables.size(1) * cache.size(3);
+  const Block8Plan plan = block8_plan((int)B, (int)H, (int)Hk, (int)D, width, (int)splits, mp != nullptr);
+  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({B, H, D}, q.options());
+  check_bf16(out, "out");
+  check_same_device(out, cache);
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes(), "out must be contiguous like q");
+  torch::Tensor ws;
+  if (workspace.has_value()) {
+    ws = *workspace;
+    TORCH_CHECK(ws.is_cuda() && ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.numel() >= plan.floats() &&
+                    reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0,
+                "decode attention: fp32 workspace of ", std::to_string(plan.floats()), " elements needed");
+    check_same_device(ws, cache);
+  } else {
+    ws = torch::empty({plan.floats()}, q.options().dtype(at::kFloat));
+  }
   launch_block8_decode(out.data_ptr(), q.data_ptr(), q.stride(0), cache.data_ptr(), scales.data_ptr<float>(),
-                       tables.data_ptr<int>(), tables.stride(0), tables.size(1), lens.data_ptr<int>(), B, H, Hk, D,
-                       cache.size(3), (int)cache.size(0), (int)splits, (float)scale, (int)window, (float)softcap, po,
-                       pml, sc, mp, e4m3, cur_stream());
+                       tables.data_ptr<int>(), tables.stride(0), tables.size(1), lens.data_ptr<int>(), (int)B, (int)H,
+                       (int)Hk, (int)D, cache.size(3), (int)cache.size(0), plan, (float)scale, (int)window,
+                       (float)softcap, ws.data_ptr<float>(), mp, e4m3, cur_stream());
+  return out;
 }
 
 void kv_evict_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor mass, torch::Tensor tables,
@@ -1105,7 +1108,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_quant_blocks", &kv_quant_blocks_py);
   m.def("kv_dequant_scaled", &kv_dequant_scaled_py);
   m.def("block8_decode", &block8_decode_py);
-  m.def("block8_decode_splits", &block8_decode_splits);
+  m.def("block8_workspace", [](int64_t B, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t splits, bool mass) {
+    return block8_plan((int)B, (int)H, (int)Hk, (int)D, width, (int)splits, mass).floats();
+  });
   m.def("kv_evict", &kv_evict_py);
   m.def("num_sms", &device_num_sms);
   m.def("moe_forward", &moe_forward_out, "MoE layer: route, permute, grouped tcgen05 expert GEMMs, combine (K12)",

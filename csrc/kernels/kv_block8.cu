@@ -234,29 +234,48 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------------------------
 // Decode attention.
 //
-// One CTA takes a range of 16-token tiles of one (sequence, kv head); its 8 warps take the tiles in
-// turn, each with its own ring of cp.async stages in shared memory, so no barrier stands in the loop. Heads are the
-// N = 8 columns of mma.m16n8k16 and tokens (for S^T = K Q^T) or dims (for O^T = V^T P^T) the 16 rows, so a group of up
-// to 8 heads wastes no row. Codes turn into f16 inside the fragments, exactly:
+// The work is cut into steps of T tokens of one (sequence, kv head, head tile); all steps of the
+// batch form one list (sequence by sequence) and every CTA of a grid that just fills the GPU takes an
+// equal stretch of it, whatever the lengths: no tail, one prologue per CTA, and loads that run ahead over the
+// borders of sequences. A stretch's first and last sequence may be shared with its neighbours: their partial sums
+// meet in a second kernel (block8_join_kernel).
+//
+// A step: warp w (of W) takes the scores of its 16 tokens, S^T = K Q^T, then all warps exchange the
+// probabilities in shared memory and warp w takes dims [w D / W, (w + 1) D / W) of O^T = V^T P^T over all T
+// tokens, so O is never reduced across warps. Heads are the N = 8 columns of mma.m16n8k16, tokens and
+// dims its 16 rows: a group of up to 8 heads wastes no row. Codes turn into f16 inside the fragments, exactly:
 //   K: a lane's four consecutive bytes of a 16-byte chunk are two k-pairs of a k16 step. Any order of dims will
-//      do as long as Q follows it, so Q is gathered in that order once.
+//      do as long as Q follows it, so Q is gathered in that order once per sequence.
 //   V: ldmatrix.trans moves byte pairs; a byte permute splits them into the fragments of the even and the odd dims.
 // Scores get the key scale, probabilities the value scale. The running reference m of the softmax
 // covers score + exponent of the value scale, so p * scale fits f16 whatever the scales; the sum l
-// uses p alone. m only moves when a score passes it by 2^8 (one vote per tile instead of a reduction).
+// uses p alone. m only moves when a score passes it by 2^8: the vote rides on the barrier that the
+// exchange needs anyway.
 // ---------------------------------------------------------------------------------------------
-constexpr int kDecWarps = 8;
 constexpr float kSlack = 8.f;  // p * scale <= 2^9: within f16
 
-template <int D>
+template <int D, int NT>
 struct DecShape {
-  static constexpr int kChunks = D / 16;                        // 16-byte chunks of a token row
-  static constexpr int kRow = (kChunks | 1) * 16;               // row pitch: an odd number of chunks, so 8 rows of one chunk hit 8 bank groups
-  static constexpr int kTile = 16 * kRow;
-  static constexpr int kStage = 2 * kTile + 16;                 // K, V, two scales
+  static constexpr int kChunks = D / 16;                            // 16-byte chunks of a token row
+  static constexpr int kWarps = D == 256 ? 4 : D / 16;              // D = 256: 4 warps of 4 chunks, two CTAs per SM
+  static constexpr int kTokens = 16 * kWarps;                       // of a step
+  static constexpr int kOwn = kChunks / kWarps;                     // chunks of O a warp owns
+  static constexpr bool kSwizzle = kChunks % 8 == 0;
+  // rows of 8 chunks are swizzled, others padded to an odd number: 8 rows of one chunk hit 8 bank groups
+  static constexpr int kRow = kSwizzle ? D : (kChunks | 1) * 16;
+  static constexpr int kSide = kTokens * kRow;                      // K (or V) of a step
+  static constexpr int kQRow = 2 * D + 16;
+  static constexpr bool kStageQ = NT == 1;                          // a head tile's Q arrives with its first step
+  static constexpr int kQ = kStageQ ? 8 * kQRow : 0;                // (two column tiles leave no room for it)
+  static constexpr int kStage = (2 * kSide + kQ + 8 * kWarps + 15) / 16 * 16;  // K, V, Q, tile scales
   static constexpr int kStages = D <= 64 ? 4 : 3;
-  static constexpr int kRing = kStages * kStage;
-  static constexpr int kCtas = D <= 128 ? 2 : 1;
+  static constexpr int kPRow = 2 * kTokens + 16;
+  static constexpr int kP = NT * 8 * kPRow;
+  static constexpr int kSmem = kStages * kStage + kP;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kFit = (227 * 1024) / (kSmem + 1024 + 2 * kWarps * NT * 8 * 4);
+  static constexpr int kRegs = 65536 / (kThreads * (D == 256 ? 168 : NT == 2 ? 120 : 96));
+  static constexpr int kCtas = kFit < kRegs ? kFit : kRegs;         // resident CTAs per SM
 };
 
 struct DecArgs {
@@ -266,18 +285,27 @@ struct DecArgs {
   const int* tables;
   const int* lens;
   __nv_bfloat16* out;
-  float* part_o;       // [B * H, splits, D]
-  float* part_ml;      // [B * H, splits, 2]: reference (log2) and sum
-  float* scores;       // [B * Hk, cap, G] log2 scores
+  float* part_o;       // [grid, 2, HB, D]: sums of a stretch's first and last sequence, where it is shared
+  float* part_ml;      // [grid, 2, HB, 2]: their reference (log2) and sum of probabilities
+  float* row_ml;       // [B * H, 2]: reference and sum of the sequences that one CTA finished (mass)
+  int* spans;          // [B * Hk * NG, 2]: first part and number of parts of each head tile (1: finished)
+  float* scores;       // [B * Hk, mb * bs, G] log2 scores (mass)
   float* mass;
   int64_t q_stride, bt_stride;
-  int B, H, Hk, G, NG, splits, mb, bs_log2, num_blocks, window;
+  int B, H, Hk, G, NG, grid, mb, bs_log2, num_blocks, window;
   float scale_log2, cap, cap_log2;  // softcap (0: none): 2 / softcap, softcap * log2(e)
   uint32_t* bounds;
 };
 
-GOLLEK_DEVICE void cp_async16(uint32_t dst, const void* src, bool full) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+// 16 bytes global -> shared at constant offsets from both addresses; `bytes` 0 writes zeros instead
+template <int DST, int SRC>
+GOLLEK_DEVICE void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
+}
+template <int DST, int SRC>
+GOLLEK_DEVICE void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(DST), "n"(SRC)
+               : "memory");
 }
 GOLLEK_DEVICE void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
@@ -341,123 +369,255 @@ GOLLEK_DEVICE void expand4(uint32_t w, uint32_t& a, uint32_t& b) {
   }
 }
 
+// Tokens of row b that are attended: [lo, L), in steps of T from the tile that holds lo.
+struct DecRow {
+  int L, lo, t0, n;
+};
+GOLLEK_DEVICE DecRow dec_row(const DecArgs& p, int b, int T) {
+  DecRow r;
+  r.L = min(max(p.lens[b], 0), p.mb << p.bs_log2);
+  r.lo = p.window > 0 ? max(0, r.L - p.window) : 0;
+  r.t0 = r.lo & ~15;
+  r.n = (r.L - r.t0 + T - 1) / T;
+  return r;
+}
+// First step of CTA c's stretch, and the CTA whose stretch holds step x. No stretch is empty: with fewer steps
+// than CTAs, the last CTAs take no part (grid is then the number of steps).
+GOLLEK_DEVICE int stretch_grid(const DecArgs& p, int64_t total) { return (int)min((int64_t)p.grid, total); }
+GOLLEK_DEVICE int64_t stretch_begin(int64_t c, int64_t total, int grid) { return c * total / grid; }
+GOLLEK_DEVICE int64_t stretch_of(int64_t x, int64_t total, int grid) { return ((x + 1) * grid - 1) / total; }
+
+// A place in the list of steps: step s of head tile hg of KV head kh of row b.
+struct DecPlace {
+  int b, kh, hg, s;
+  DecRow r;
+};
+GOLLEK_DEVICE void next_head(DecPlace& q, const DecArgs& p, int T) {
+  q.s = 0;
+  if (++q.hg < p.NG) return;
+  q.hg = 0;
+  if (++q.kh < p.Hk) return;
+  q.kh = 0;
+  do {
+    ++q.b;
+    if (q.b < p.B) q.r = dec_row(p, q.b, T);
+  } while (q.b < p.B && q.r.n == 0);
+}
+
 template <int D, int NT, bool E4M3, bool MASS>
-__global__ void __launch_bounds__(kDecWarps * 32, DecShape<D>::kCtas) block8_decode_kernel(const DecArgs p) {
-  using S = DecShape<D>;
-  constexpr int CH = S::kChunks, HB = 8 * NT;  // heads of this CTA
-  extern __shared__ __align__(16) uint8_t dsm[];
-  __shared__ float sm_m[kDecWarps][HB], sm_l[kDecWarps][HB];
+__global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kCtas)
+    block8_decode_kernel(const DecArgs p) {
+  using S = DecShape<D, NT>;
+  constexpr int CH = S::kChunks, HB = 8 * NT, W = S::kWarps, T = S::kTokens, OWN = S::kOwn;
+  extern __shared__ __align__(128) uint8_t dsm[];
+  __shared__ float sm_x[W][HB], sm_l[W][HB];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
-  int idx = blockIdx.x;
-  const int split = idx % p.splits;
-  idx /= p.splits;
-  const int hg = idx % p.NG;
-  const int bk = idx / p.NG;  // b * Hk + kh
-  const int kh = bk % p.Hk, b = bk / p.Hk;
-  const int h0 = hg * HB, nh = min(p.G - h0, HB);  // heads of the group handled here
-  const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2);
-  const int lo = p.window > 0 ? max(0, L - p.window) : 0;
-  const int t_lo = lo >> 4, t_hi = (L + 15) >> 4;
-  const int per = (t_hi - t_lo + p.splits - 1) / p.splits;
-  const int tb = t_lo + split * per, te = min(t_hi, tb + per);
-  const int mine = tb + warp < te ? (te - tb - warp + kDecWarps - 1) / kDecWarps : 0;
-  const int* bt = p.tables + (int64_t)b * p.bt_stride;
-  uint8_t* ring = dsm + warp * S::kRing;
-  const uint32_t ring_u = smem_u32(ring);
+  const int X = p.Hk * p.NG;
+  const uint32_t ring = smem_u32(dsm), psm = ring + S::kStages * S::kStage;
 
-  int ids = 0;  // lane l: pool block of this warp's tile (j & ~31) + l
-  auto issue = [&](int j) {
-    if (j < mine) {
-      if ((j & 31) == 0) {
-        const int t = tb + warp + kDecWarps * (j + lane);
-        ids = t < te ? checked_index(bt[t >> (p.bs_log2 - 4)], p.num_blocks, p.bounds) : 0;
-      }
-      const int64_t id = __shfl_sync(0xffffffffu, ids, j & 31);
-      const int t = tb + warp + kDecWarps * j;
-      const int off = (t << 4) & ((1 << p.bs_log2) - 1);
-      const int64_t rk = (id * 2) * p.Hk + kh, rv = rk + p.Hk;
-      const uint8_t* gk = p.cache + ((rk << p.bs_log2) + off) * D;
-      const uint8_t* gv = p.cache + ((rv << p.bs_log2) + off) * D;
-      const uint32_t st = ring_u + (j % S::kStages) * S::kStage;
+  asm volatile("griddepcontrol.launch_dependents;");
+  // this CTA's stretch of the list: every warp sums the rows' steps, then finds the row it starts in
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? dec_row(p, b0 + lane, T).n : 0);
+  total *= X;
+  const int grid = stretch_grid(p, total);
+  if ((int)blockIdx.x >= grid) return;
+  const int64_t first = stretch_begin(blockIdx.x, total, grid);
+  const int count = (int)(stretch_begin(blockIdx.x + 1, total, grid) - first);
+  DecPlace at;  // of the next step to issue
+  {
+    int64_t before = 0;
+    at.b = 0;
+    for (int b0 = 0;; b0 += 32) {
+      const int n = b0 + lane < p.B ? dec_row(p, b0 + lane, T).n : 0;
+      int sum = n;
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) {
-        const int e = i * 32 + lane, row = e / CH, ch = e % CH;
-        const int tok = (t << 4) + row;
-        const bool full = tok >= lo && tok < L;  // rows outside read as zero
-        cp_async16(st + row * S::kRow + ch * 16, gk + e * 16, full);
-        cp_async16(st + S::kTile + row * S::kRow + ch * 16, gv + e * 16, full);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
       }
-      if (lane < 2) cp_async4(st + 2 * S::kTile + 4 * lane, p.scales + (lane ? rv : rk));
+      const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && before + (int64_t)sum * X > first);
+      if (hit) {
+        const int li = __ffs(hit) - 1;
+        at.b = b0 + li;
+        before += (int64_t)__shfl_sync(0xffffffffu, sum - n, li) * X;
+        break;
+      }
+      before += (int64_t)__shfl_sync(0xffffffffu, sum, 31) * X;
+    }
+    at.r = dec_row(p, at.b, T);
+    const int x = (int)((first - before) / at.r.n);
+    at.kh = x / p.NG, at.hg = x % p.NG;
+    at.s = (int)((first - before) % at.r.n);
+  }
+
+  // block ids of this warp's tiles are read 32 steps at a time, one batch ahead of their use
+  DecPlace ahead = at;
+  auto load_ids = [&]() {
+    int id = 0;
+    if (ahead.b < p.B) {
+      const int t = ahead.r.t0 + (ahead.s + lane) * T + warp * 16;
+      if (t < ahead.r.L)
+        id = checked_index(p.tables[(int64_t)ahead.b * p.bt_stride + (t >> p.bs_log2)], p.num_blocks, p.bounds);
+      ahead.s += 32;
+      if (ahead.s >= ahead.r.n) next_head(ahead, p, T);
+    }
+    return id;
+  };
+  int ids = 0, ids_next = load_ids(), batch = 32;
+  int issued = 0;
+  // a lane's pieces of a tile: 16 bytes at lane * 16 + 512 i, i.e. row lane / CH + 32 / CH i where CH divides 32
+  const uint32_t block_bytes = (uint32_t)(2 * p.Hk << p.bs_log2) * D, v_bytes = block_bytes >> 1;
+  uint32_t st_issue = ring;  // stage of the next step to issue
+  auto issue = [&]() {
+    if (issued < count) {
+      if (batch == 32) ids = ids_next, ids_next = load_ids(), batch = 0;
+      const uint32_t id = __shfl_sync(0xffffffffu, ids, batch);
+      const uint32_t st = st_issue;
+      const int t = at.r.t0 + at.s * T + warp * 16;
+      const int off = t & ((1 << p.bs_log2) - 1);
+      const uint8_t* gk = p.cache + (uint64_t)id * block_bytes + (uint32_t)((at.kh << p.bs_log2) + off) * D;
+      const uint8_t* gv = gk + v_bytes;
+      const uint32_t tail = st + 2 * S::kSide + S::kQ;
+      if (32 % CH == 0 && t >= at.r.lo && t + 16 <= at.r.L) {  // a whole tile
+        constexpr int R = 32 / CH;  // rows per round
+        const int row = lane / CH, ch = lane % CH;
+        const uint8_t *ck = gk + lane * 16, *cv = gv + lane * 16;
+        // with the swizzle a lane's chunk changes with the rounds' row parity bits only
+        const uint32_t d0 = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
+        const uint32_t d1 = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ ((row + R) & 7) : ch) << 4);
+        constexpr int N = CH / 2, RB = R * S::kRow;
+#define GOLLEK_TILE(I)                                                       \
+  if constexpr (I < N) {                                                     \
+    cp_async16<(I) * RB, (I) * 512>(((I) & 1) ? d1 : d0, ck);                \
+    cp_async16<(I) * RB + S::kSide, (I) * 512>(((I) & 1) ? d1 : d0, cv);     \
+  }
+        if constexpr (N <= 4) {
+          GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(2) GOLLEK_TILE(3)
+        } else {  // D = 256: two rows a round, four different chunks
+          const uint32_t d2 = st + (warp * 16 + row) * S::kRow + ((ch ^ ((row + 2 * R) & 7)) << 4);
+          const uint32_t d3 = st + (warp * 16 + row) * S::kRow + ((ch ^ ((row + 3 * R) & 7)) << 4);
+          GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(4) GOLLEK_TILE(5)
+          cp_async16<2 * RB, 1024>(d2, ck);
+          cp_async16<2 * RB + S::kSide, 1024>(d2, cv);
+          cp_async16<6 * RB, 3072>(d2, ck);
+          cp_async16<6 * RB + S::kSide, 3072>(d2, cv);
+          cp_async16<3 * RB, 1536>(d3, ck);
+          cp_async16<3 * RB + S::kSide, 1536>(d3, cv);
+          cp_async16<7 * RB, 3584>(d3, ck);
+          cp_async16<7 * RB + S::kSide, 3584>(d3, cv);
+        }
+#undef GOLLEK_TILE
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < CH / 2; ++i) {
+          const int e = i * 32 + lane, row = e / CH, ch = e % CH;
+          const int bytes = t + row >= at.r.lo && t + row < at.r.L ? 16 : 0;  // rows outside read as zero
+          const uint32_t d = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
+          cp_async16_or_zero<0, 0>(d, gk + e * 16, bytes);
+          cp_async16_or_zero<S::kSide, 0>(d, gv + e * 16, bytes);
+        }
+      }
+      if (lane < 2) cp_async4(tail + 8 * warp + 4 * lane, p.scales + (uint64_t)(id * 2 + lane) * p.Hk + at.kh);
+      if (S::kStageQ && (at.s == 0 || issued == 0)) {
+        const int h0 = at.hg * HB, nh = min(p.G - h0, HB);
+        const __nv_bfloat16* q = p.q + (int64_t)at.b * p.q_stride + (int64_t)(at.kh * p.G + h0) * D;
+        for (int e = threadIdx.x; e < HB * D / 8; e += S::kThreads) {
+          const int hh = e / (D / 8);
+          cp_async16_or_zero<0, 0>(st + 2 * S::kSide + hh * S::kQRow + (e % (D / 8)) * 16, hh < nh ? q + e * 8 : q, hh < nh ? 16 : 0);
+        }
+      }
+      ++issued;
+      ++batch;
+      st_issue = st_issue == ring + (S::kStages - 1) * S::kStage ? ring : st_issue + S::kStage;
+      if (++at.s == at.r.n) {
+        next_head(at, p, T);
+        batch = 32;
+      }
     }
     cp_async_commit();
   };
+  DecPlace cur = at;  // the step being computed
 #pragma unroll
-  for (int j = 0; j < S::kStages - 1; ++j) issue(j);
+  for (int j = 0; j < S::kStages - 1; ++j) issue();
 
-  // Q^T as the B operand, columns = heads: chunk j of the lane's head, dims 16 j + 4 c + {0, 1} and
-  // + {2, 3}. Each head is brought to an amax in [2^11, 2^12) by a power of two: f16 then holds every
-  // bf16 within 2^-28 of it exactly.
   uint32_t qf[NT][CH][2];
   float qmul[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int hh = nt * 8 + g;
-    uint2 raw[CH];
-    float amax = 0.f;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      raw[j] = make_uint2(0u, 0u);
-      if (hh < nh)
-        raw[j] = *reinterpret_cast<const uint2*>(p.q + (int64_t)b * p.q_stride + (int64_t)(kh * p.G + h0 + hh) * D + 16 * j + 4 * c);
-      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[j].x));
-      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[j].y));
-      amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 127) - 11;
-    const float f = __uint_as_float((uint32_t)(127 - e) << 23);
-    const float back = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[j].x));
-      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[j].y));
-      const __half2 hx = __floats2half2_rn(x.x * f, x.y * f), hy = __floats2half2_rn(y.x * f, y.y * f);
-      qf[nt][j][0] = *reinterpret_cast<const uint32_t*>(&hx);
-      qf[nt][j][1] = *reinterpret_cast<const uint32_t*>(&hy);
-    }
-    qmul[nt][0] = __shfl_sync(0xffffffffu, back, 8 * c);      // columns 2 c and 2 c + 1
-    qmul[nt][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
-  }
-
-  float o[CH][NT][4];
+  float o[OWN][NT][4];
   float m[NT][2], l[NT][2];
-#pragma unroll
-  for (int j = 0; j < CH; ++j)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][nt][e] = 0.f;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.f;
-
-  // ldmatrix row of this lane: matrices (rows 0-7, 8-15) of one chunk, then of the next
-  const uint32_t ld_off = ((lane & 7) + ((lane >> 3) & 1) * 8) * S::kRow + (lane >> 4) * 16;
-  for (int j = 0; j < mine; ++j) {
+  const int frow = (lane & 7) + ((lane >> 3) & 1) * 8, fhi = lane >> 4;  // this lane's row and chunk of an x4 ldmatrix
+  bool begun = false;  // whether this stretch holds the current head tile's first step
+  uint32_t st = ring;
+  for (int j = 0; j < count; ++j) {
     cp_async_wait<S::kStages - 2>();
-    __syncwarp();
-    issue(j + S::kStages - 1);  // into the stage read in the previous turn
-    const uint32_t st = ring_u + (j % S::kStages) * S::kStage;
+    __syncthreads();  // the step's data is there, and the previous one's stage is free
+    issue();
+    const uint32_t tail = st + 2 * S::kSide + S::kQ;
+    const int b = cur.b, kh = cur.kh, h0 = cur.hg * HB, nh = min(p.G - h0, HB);
+    const int tok0 = cur.r.t0 + cur.s * T;
+    if (cur.s == 0 || j == 0) {
+      begun = cur.s == 0;
+      // Q^T as the B operand, columns = heads: chunk i of the lane's head, dims 16 i + 4 c + {0, 1} and
+      // + {2, 3}. Each head is brought to an amax in [2^11, 2^12) by a power of two: f16 then holds every
+      // bf16 within 2^-28 of it exactly.
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        uint2 raw[CH];
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          if constexpr (S::kStageQ) {
+            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];"
+                         : "=r"(raw[i].x), "=r"(raw[i].y)
+                         : "r"(st + 2 * S::kSide + (nt * 8 + g) * S::kQRow + 32 * i + 8 * c)
+                         : "memory");
+          } else {
+            raw[i] = make_uint2(0u, 0u);
+            if (nt * 8 + g < nh)
+              raw[i] = *reinterpret_cast<const uint2*>(p.q + (int64_t)b * p.q_stride +
+                                                       (int64_t)(kh * p.G + h0 + nt * 8 + g) * D + 16 * i + 4 * c);
+          }
+          const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].x));
+          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].y));
+          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(v.x), fabsf(v.y))));
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 127) - 11;
+        const float f = __uint_as_float((uint32_t)(127 - e) << 23);
+        const float back = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+          const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].x));
+          const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].y));
+          const __half2 hu = __floats2half2_rn(u.x * f, u.y * f), hv = __floats2half2_rn(v.x * f, v.y * f);
+          qf[nt][i][0] = *reinterpret_cast<const uint32_t*>(&hu);
+          qf[nt][i][1] = *reinterpret_cast<const uint32_t*>(&hv);
+        }
+        qmul[nt][0] = __shfl_sync(0xffffffffu, back, 8 * c);  // columns 2 c and 2 c + 1
+        qmul[nt][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[i][nt][k] = 0.f;
+      }
+    }
+
+    // scores of this warp's 16 tokens
+    const int tile = tok0 + warp * 16, tok = tile + g;
     float s[NT][4], s2[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
+    const uint32_t kb = st + (warp * 16 + frow) * S::kRow;
 #pragma unroll
     for (int j2 = 0; j2 < CH / 2; ++j2) {
       uint32_t r[4], a[4];
-      ldsm4(r, st + ld_off + j2 * 32);
+      ldsm4(r, kb + ((S::kSwizzle ? (2 * j2) ^ (fhi ^ (frow & 7)) : 2 * j2 + fhi) << 4));
       expand4<E4M3, false>(r[0], a[0], a[2]);
       expand4<E4M3, false>(r[1], a[1], a[3]);
 #pragma unroll
@@ -468,159 +628,263 @@ __global__ void __launch_bounds__(kDecWarps * 32, DecShape<D>::kCtas) block8_dec
       for (int nt = 0; nt < NT; ++nt) mma_f16(s2[nt], a, qf[nt][2 * j2 + 1][0], qf[nt][2 * j2 + 1][1]);
     }
     float ks, vs;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs) : "r"(st + 2 * S::kTile) : "memory");
+    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs) : "r"(tail + 8 * warp) : "memory");
+    if (tile >= cur.r.L) vs = 0.f;  // no token here: whatever scale was read, the probabilities are 0
     const float ev = (float)max((int)((__float_as_uint(vs) >> 23) & 0xff) - 127, -100);
-    const int tok = ((tb + warp + kDecWarps * j) << 4) + g;
-    const bool ok0 = tok >= lo && tok < L, ok1 = tok + 8 >= lo && tok + 8 < L;
-    bool up = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float x = (s[nt][e] + s2[nt][e]) * (ks * qmul[nt][e & 1]);
-        // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2 x / cap)))
-        if (p.cap > 0.f) x = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(x * p.cap)));
-        s[nt][e] = (e < 2 ? ok0 : ok1) ? x : -INFINITY;
-        up |= s[nt][e] + ev > m[nt][e & 1] + kSlack;
-      }
-    if constexpr (MASS) {
-      float* sc = p.scores + ((int64_t)bk * (p.mb << p.bs_log2) + tok) * p.G + h0;
+      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (ks * qmul[nt][e & 1]);
+    if (p.cap > 0.f) {  // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2 x / cap)))
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int hh = nt * 8 + 2 * c + (e & 1);
-          if (hh < nh && (e < 2 ? ok0 : ok1)) sc[(e < 2 ? 0 : 8 * p.G) + hh] = s[nt][e];
+        for (int e = 0; e < 4; ++e) s[nt][e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[nt][e] * p.cap)));
+    }
+    bool ok0 = true, ok1 = true;
+    if (tile < cur.r.lo || tile + 16 > cur.r.L) {
+      ok0 = tok >= cur.r.lo && tok < cur.r.L, ok1 = tok + 8 >= cur.r.lo && tok + 8 < cur.r.L;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? ok0 : ok1) ? s[nt][e] : -INFINITY;
+    }
+    bool up = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      up |= fmaxf(s[nt][0], s[nt][2]) + ev > m[nt][0] + kSlack || fmaxf(s[nt][1], s[nt][3]) + ev > m[nt][1] + kSlack;
+    if constexpr (MASS) {
+      float* sc = p.scores + ((int64_t)(b * p.Hk + kh) * (p.mb << p.bs_log2) + tok) * p.G + h0;
+      const bool pairs = (p.G & 1) == 0;  // a token's scores of two heads lie at a multiple of 8 bytes
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const int hh = nt * 8 + 2 * c;
+          float* d = sc + (e < 2 ? 0 : 8 * p.G) + hh;
+          if (!(e < 2 ? ok0 : ok1) || hh >= nh) continue;
+          if (pairs) {
+            *reinterpret_cast<float2*>(d) = make_float2(s[nt][e], s[nt][e + 1]);
+          } else {
+            d[0] = s[nt][e];
+            if (hh + 1 < nh) d[1] = s[nt][e + 1];
+          }
         }
     }
-    if (__any_sync(0xffffffffu, up)) {
+    // probabilities in f16 (2^-11 relative): the output's bf16 rounding is eight times coarser
+    const uint32_t pd = psm + g * S::kPRow + warp * 32 + 4 * c;
+    float e4[NT][4];
+    auto put = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) e4[nt][e] = ex2(s[nt][e] - m[nt][e & 1]);  // a masked score is -inf
+        const __half2 u = __floats2half2_rn(e4[nt][0] * vs, e4[nt][1] * vs);
+        const __half2 v = __floats2half2_rn(e4[nt][2] * vs, e4[nt][3] * vs);
+        const uint32_t x0 = movm_t(*reinterpret_cast<const uint32_t*>(&u));  // now tokens 2 c, 2 c + 1 of head g
+        const uint32_t x1 = movm_t(*reinterpret_cast<const uint32_t*>(&v));
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow), "r"(x0) : "memory");
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow + 16), "r"(x1) : "memory");
+      }
+    };
+    put();
+    if (__syncthreads_or(up)) {  // a score passed the reference: take the step's true maximum
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(s[nt][e], s[nt][e + 2]) + ev;
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, m[nt][e]);
-          const float d = x > m[nt][e] ? m[nt][e] - x : 0.f, al = ex2(d);
-          m[nt][e] = x;
+          float y = fmaxf(s[nt][e], s[nt][e + 2]) + ev;
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+          y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+          if (g == 0) sm_x[warp][nt * 8 + 2 * c + e] = y;
+        }
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float y = m[nt][e];
+#pragma unroll
+          for (int w = 0; w < W; ++w) y = fmaxf(y, sm_x[w][nt * 8 + 2 * c + e]);
+          const float d = y > m[nt][e] ? m[nt][e] - y : 0.f, al = ex2(d);
+          m[nt][e] = y;
           l[nt][e] = shift_sum(l[nt][e], d);
 #pragma unroll
-          for (int jj = 0; jj < CH; ++jj) o[jj][nt][e] *= al, o[jj][nt][e + 2] *= al;
+          for (int i = 0; i < OWN; ++i) o[i][nt][e] *= al, o[i][nt][e + 2] *= al;
         }
-    }
-    uint32_t pb[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float e0 = ok0 ? ex2(s[nt][0] - m[nt][0]) : 0.f, e1 = ok0 ? ex2(s[nt][1] - m[nt][1]) : 0.f;
-      float e2 = ok1 ? ex2(s[nt][2] - m[nt][0]) : 0.f, e3 = ok1 ? ex2(s[nt][3] - m[nt][1]) : 0.f;
-      l[nt][0] += e0 + e2;
-      l[nt][1] += e1 + e3;
-      // probabilities in f16 (2^-11 relative): the output's bf16 rounding is eight times coarser
-      const __half2 x = __floats2half2_rn(e0 * vs, e1 * vs), y = __floats2half2_rn(e2 * vs, e3 * vs);
-      pb[nt][0] = movm_t(*reinterpret_cast<const uint32_t*>(&x));
-      pb[nt][1] = movm_t(*reinterpret_cast<const uint32_t*>(&y));
+      put();
+      __syncthreads();
     }
 #pragma unroll
-    for (int j2 = 0; j2 < CH / 2; ++j2) {
-      uint32_t r[4], a[4];
-      ldsm4_t(r, st + S::kTile + ld_off + j2 * 32);
-      expand4<E4M3, true>(r[0], a[0], a[1]);
-      expand4<E4M3, true>(r[1], a[2], a[3]);
+    for (int nt = 0; nt < NT; ++nt) l[nt][0] += e4[nt][0] + e4[nt][2], l[nt][1] += e4[nt][1] + e4[nt][3];
+
+    // O^T of this warp's dims over the step's tokens, two tiles at a time (tiles behind L are zero)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_f16(o[2 * j2][nt], a, pb[nt][0], pb[nt][1]);
-      expand4<E4M3, true>(r[2], a[0], a[1]);
-      expand4<E4M3, true>(r[3], a[2], a[3]);
+    for (int t2 = 0; t2 < W / 2; ++t2) {
+      uint32_t pb[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_f16(o[2 * j2 + 1][nt], a, pb[nt][0], pb[nt][1]);
+      for (int nt = 0; nt < NT; ++nt) ldsm4(pb[nt], psm + (nt * 8 + (lane & 7)) * S::kPRow + t2 * 64 + (lane >> 3) * 16);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        uint32_t r[4], a[4];
+        const int row = t2 * 32 + (lane & 7) + (lane >> 3) * 8, ch = warp * OWN + i;
+        ldsm4_t(r, st + S::kSide + row * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4));
+        expand4<E4M3, true>(r[0], a[0], a[1]);
+        expand4<E4M3, true>(r[1], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(o[i][nt], a, pb[nt][0], pb[nt][1]);
+        expand4<E4M3, true>(r[2], a[0], a[1]);
+        expand4<E4M3, true>(r[3], a[2], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(o[i][nt], a, pb[nt][2], pb[nt][3]);
+      }
     }
+
+    st = st == ring + (S::kStages - 1) * S::kStage ? ring : st + S::kStage;
+    const int step = cur.s++;
+    const bool last = cur.s == cur.r.n;
+    if (!last && j + 1 < count) continue;
+    // the head tile ends here, or goes on in the next CTA's stretch
+    const bool whole = begun && last;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float y = l[nt][e];
+        y += __shfl_xor_sync(0xffffffffu, y, 4);
+        y += __shfl_xor_sync(0xffffffffu, y, 8);
+        y += __shfl_xor_sync(0xffffffffu, y, 16);
+        if (g == 0) sm_l[warp][nt * 8 + 2 * c + e] = y;
+      }
+    __syncthreads();
+    const uint32_t part = blockIdx.x * 2 + (j > step ? 1 : 0);  // 0: it holds the stretch's first step
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int hh = nt * 8 + 2 * c + e;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += sm_l[w][hh];
+        if (hh >= nh) continue;
+        const int64_t row = (int64_t)b * p.H + kh * p.G + h0 + hh;
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) {
+          const int d = (warp * OWN + i) * 16 + 2 * g;
+          if (whole)
+            *reinterpret_cast<uint32_t*>(p.out + row * D + d) = pack_bf16x2(o[i][nt][e] * inv, o[i][nt][e + 2] * inv);
+          else
+            *reinterpret_cast<float2*>(p.part_o + (part * HB + hh) * D + d) = make_float2(o[i][nt][e], o[i][nt][e + 2]);
+        }
+        if (warp == 0 && g == 0) {
+          if (!whole) *reinterpret_cast<float2*>(p.part_ml + (part * HB + hh) * 2) = make_float2(m[nt][e], sum);
+          else if (MASS) *reinterpret_cast<float2*>(p.row_ml + row * 2) = make_float2(m[nt][e], sum);
+        }
+      }
+    if (begun && threadIdx.x == 0) {  // the CTA that holds the first step says how many parts there are
+      int parts = 1;
+      if (!last) parts = (int)(stretch_of(first + j - step + cur.r.n - 1, total, grid) - blockIdx.x) + 1;
+      *reinterpret_cast<int2*>(p.spans + ((int64_t)b * X + kh * p.NG + cur.hg) * 2) = make_int2((int)part, parts);
+    }
+    if (last) next_head(cur, p, T);
   }
   cp_async_wait<0>();
-  __syncwarp();
-
-  // the warps' partial sums meet in shared memory (each over its own ring)
-  static_assert(HB * D * 4 <= S::kRing, "a warp's partial output fits its ring");
-  float* wo = reinterpret_cast<float*>(ring);
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int hh = nt * 8 + 2 * c + e;
-      float x = l[nt][e];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) sm_m[warp][hh] = m[nt][e], sm_l[warp][hh] = x;
-#pragma unroll
-      for (int j = 0; j < CH; ++j)
-        *reinterpret_cast<float2*>(wo + hh * D + 16 * j + 2 * g) = make_float2(o[j][nt][e], o[j][nt][e + 2]);
-    }
-  __syncthreads();
-  for (int i = threadIdx.x; i < nh * D; i += kDecWarps * 32) {
-    const int hh = i / D;
-    float M = -INFINITY, sum = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm_m[w][hh]);
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      const float d = sm_m[w][hh] - M, f = sm_m[w][hh] == -INFINITY ? 0.f : ex2(d);
-      if (sm_m[w][hh] != -INFINITY) sum += shift_sum(sm_l[w][hh], d);
-      acc += f * reinterpret_cast<const float*>(dsm + w * S::kRing)[i];
-    }
-    const int64_t row = (int64_t)b * p.H + kh * p.G + h0 + hh;
-    if (p.splits == 1)
-      p.out[row * D + i % D] = __float2bfloat16(sum > 0.f ? acc / sum : 0.f);
-    else
-      p.part_o[(row * p.splits + split) * D + i % D] = acc;
-    if ((p.splits > 1 || MASS) && i % D == 0)
-      *reinterpret_cast<float2*>(p.part_ml + (row * p.splits + split) * 2) = make_float2(M, sum);
-  }
 }
 
-// Joins the splits of each (sequence, head): the first B * H CTAs; the others add the softmax weights
-// of 256 tokens of a (sequence, kv head) to mass, summed over the head group in head order. An entry gets one add
-// per call, so sums do not depend on the order of the CTAs unless sequences share a block.
-__global__ void __launch_bounds__(128) block8_join_kernel(const DecArgs p, int D, int mass_tiles) {
+// Part number i of a head tile: its first one, then the first slots of the CTAs that follow.
+GOLLEK_DEVICE int64_t part_slot(int first, int i) { return i == 0 ? first : (first & ~1) + 2 * i; }
+
+// Reference and sum of head hh over a head tile's n parts, by one warp.
+GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh) {
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  const int lane = threadIdx.x & 31;
+  float2 x = make_float2(-INFINITY, 0.f);
+  if (lane < n) x = ml[part_slot(first, lane) * HB + hh];
+  float M = x.x;
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, ml[part_slot(first, i) * HB + hh].x);
+  M = warp_max(M);
+  float sum = x.x == -INFINITY ? 0.f : shift_sum(x.y, x.x - M);
+  for (int i = lane + 32; i < n; i += 32) {
+    const float2 y = ml[part_slot(first, i) * HB + hh];
+    if (y.x != -INFINITY) sum += shift_sum(y.y, y.x - M);
+  }
+  return make_float2(M, warp_sum(sum));
+}
+
+// Joins the parts of the head tiles that several CTAs shared, and zeroes empty rows: the first B * H CTAs, one per
+// (row, head); the others add the softmax weights of 128 tokens of a (row, kv head) to mass, summed over the head group
+// in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows share a block.
+__global__ void __launch_bounds__(128) block8_join_kernel(const DecArgs p, int D, int HB, int mass_tiles) {
   __shared__ float sm[128];
-  const int joins = p.splits > 1 ? p.B * p.H : 0;
-  if ((int)blockIdx.x < joins) {
-    const int64_t row = blockIdx.x;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * p.splits;
-    float M = -INFINITY, sum = 0.f;
-    for (int i = 0; i < p.splits; ++i) M = fmaxf(M, ml[i].x);
-    for (int i = 0; i < p.splits; ++i) sum += ml[i].x == -INFINITY ? 0.f : shift_sum(ml[i].y, ml[i].x - M);
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
-    for (int d = threadIdx.x; d < D; d += 128) {
-      float acc = 0.f;
-      for (int i = 0; i < p.splits; ++i)
-        if (ml[i].x != -INFINITY) acc += ex2(ml[i].x - M) * p.part_o[(row * p.splits + i) * D + d];
-      p.out[row * D + d] = __float2bfloat16(acc * inv);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
+  if ((int)blockIdx.x < p.B * p.H) {
+    const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
+    const int kh = h / p.G, hx = h - kh * p.G, x = kh * p.NG + hx / HB, hh = hx % HB;
+    const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + x];
+    const int L = min(p.lens[b], p.mb << p.bs_log2);
+    __nv_bfloat16* out = p.out + (int64_t)blockIdx.x * D;
+    if (L <= 0) {
+      for (int i = threadIdx.x; i < D; i += 128) out[i] = __float2bfloat16(0.f);
+      return;
     }
+    const int n = span.y;
+    if (n == 1) return;
+    const float2 all = join_ml(p, span.x, n, HB, hh);  // every warp for itself
+    const float inv = all.y > 0.f ? 1.f / all.y : 0.f;
+    float acc[2] = {0.f, 0.f};  // D <= 256
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const int64_t k = part_slot(span.x, i) * HB + hh;
+      const float m = p.part_ml[k * 2], f = m == -INFINITY ? 0.f : ex2(m - all.x);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if ((int)threadIdx.x + 128 * e < D) acc[e] += f * p.part_o[k * D + threadIdx.x + 128 * e];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if ((int)threadIdx.x + 128 * e < D) out[threadIdx.x + 128 * e] = __float2bfloat16(acc[e] * inv);
     return;
   }
-  const int i = blockIdx.x - joins;
-  const int bk = i / mass_tiles, kh = bk % p.Hk, b = bk / p.Hk;
-  const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2);
-  const int lo = p.window > 0 ? max(0, L - p.window) : 0;
-  const int first = (i % mass_tiles) * 256;
-  if (first >= L || first + 256 <= lo) return;
-  for (int h = threadIdx.x; h < p.G; h += 128) {
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + ((int64_t)b * p.H + kh * p.G + h) * p.splits;
-    float M = -INFINITY, sum = 0.f;
-    for (int k = 0; k < p.splits; ++k) M = fmaxf(M, ml[k].x);
-    for (int k = 0; k < p.splits; ++k) sum += ml[k].x == -INFINITY ? 0.f : shift_sum(ml[k].y, ml[k].x - M);
-    sm[h] = M + log2f(sum);
+  const int i = blockIdx.x - p.B * p.H;
+  const int bk = i / mass_tiles, b = bk / p.Hk, kh = bk - b * p.Hk;
+  const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2), lo = p.window > 0 ? max(0, L - p.window) : 0;
+  const int first = (i - bk * mass_tiles) * 128, t = first + threadIdx.x;
+  if (first >= L || first + 128 <= lo) return;
+  const bool mine = t >= lo && t < L;
+  // the token's scores and block are on their way while the heads' sums are joined
+  const float* sc = p.scores + ((int64_t)bk * (p.mb << p.bs_log2) + t) * p.G;
+  float v[8];
+  int id = 0;
+  if (mine) id = checked_index(p.tables[(int64_t)b * p.bt_stride + (t >> p.bs_log2)], p.num_blocks, p.bounds);
+  if (p.G % 4 == 0) {
+#pragma unroll
+    for (int h = 0; h < 8; h += 4)
+      if (mine && h < p.G) {
+        const float4 y = *reinterpret_cast<const float4*>(sc + h);
+        v[h] = y.x, v[h + 1] = y.y, v[h + 2] = y.z, v[h + 3] = y.w;
+      }
+  } else {
+#pragma unroll
+    for (int h = 0; h < 8; ++h)
+      if (mine && h < p.G) v[h] = sc[h];
+  }
+  for (int h = warp; h < p.G; h += 4) {
+    const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
+    const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
+                                  : join_ml(p, span.x, span.y, HB, h % HB);
+    if (lane == 0) sm[h] = ml.x + log2f(ml.y);
   }
   __syncthreads();
-  for (int t = first + threadIdx.x; t < min(first + 256, L); t += 128) {
-    if (t < lo) continue;
-    const float* sc = p.scores + ((int64_t)bk * (p.mb << p.bs_log2) + t) * p.G;
-    float w = 0.f;
-    for (int h = 0; h < p.G; ++h) w += ex2(sc[h] - sm[h]);
-    const int64_t id = checked_index(p.tables[(int64_t)b * p.bt_stride + (t >> p.bs_log2)], p.num_blocks, p.bounds);
-    atomicAdd(p.mass + ((id * p.Hk + kh) << p.bs_log2) + (t & ((1 << p.bs_log2) - 1)), w);
-  }
+  if (!mine) return;
+  float w = 0.f;
+#pragma unroll
+  for (int h = 0; h < 8; ++h)
+    if (h < p.G) w += ex2(v[h] - sm[h]);
+  for (int h = 8; h < p.G; ++h) w += ex2(sc[h] - sm[h]);
+  atomicAdd(p.mass + (((int64_t)id * p.Hk + kh) << p.bs_log2) + (t & ((1 << p.bs_log2) - 1)), w);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -902,21 +1166,51 @@ void launch_kv_dequant_scaled(const void* cache, const float* scales, const int*
   check_launch("kv_dequant_blocks");
 }
 
-// Splits of each (sequence, kv head): enough CTAs for two rounds of the GPU, at least 16 tiles (256
-// tokens) each, as far as the table's width says.
-int block8_decode_splits(int B, int Hk, int G, int D, int64_t max_len) {
-  const int nt = (G > 8 && D <= 128) ? 2 : 1, ng = (G + 8 * nt - 1) / (8 * nt);
-  const int64_t ctas = (int64_t)B * Hk * ng;
-  const int64_t slots = (int64_t)device_num_sms() * (D <= 128 ? 2 : 1);
-  if (ctas == 0 || ctas >= 2 * slots) return 1;
-  const int64_t want = (2 * slots + ctas - 1) / ctas;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, (max_len + 255) / 256), 64));
+namespace {
+
+template <int D, int NT>
+Block8Plan plan_for(int B, int H, int Hk, int64_t width, int splits, bool mass) {
+  using S = DecShape<D, NT>;
+  Block8Plan p;
+  p.nt = NT;
+  p.tokens = S::kTokens;
+  const int G = H / Hk, HB = 8 * NT;
+  p.ng = (G + HB - 1) / HB;
+  const int64_t tiles = (int64_t)B * Hk * p.ng;
+  const int64_t most = tiles * ((width + S::kTokens - 1) / S::kTokens);  // steps, if every row filled its table
+  const int64_t want = splits > 0 ? tiles * splits : (int64_t)device_num_sms() * S::kCtas;
+  p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, most), 1 << 24));
+  p.n_o = (int64_t)p.grid * 2 * HB * D;
+  p.n_ml = (int64_t)p.grid * 2 * HB * 2;
+  p.n_row = mass ? (int64_t)B * H * 2 : 0;
+  p.n_span = tiles * 2;
+  p.n_scores = mass ? (int64_t)B * H * width : 0;  // a multiple of 16, like n_o and n_ml
+  return p;
+}
+
+}  // namespace
+
+// A grid of as many CTAs as the GPU holds at once, or `splits` per (sequence, head tile) on average; never more
+// than there can be steps.
+Block8Plan block8_plan(int B, int H, int Hk, int D, int64_t width, int splits, bool mass) {
+  throw_if(Hk <= 0 || H % Hk != 0, "block-scaled decode attention: H must be a multiple of Hk");
+  throw_if(H / Hk > 128, "block-scaled decode attention: at most 128 query heads per KV head");
+  const bool two = H / Hk > 8;
+#define GOLLEK_B8(DD) \
+  if (D == DD) return two ? plan_for<DD, 2>(B, H, Hk, width, splits, mass) : plan_for<DD, 1>(B, H, Hk, width, splits, mass);
+  GOLLEK_B8(32)
+  GOLLEK_B8(64)
+  GOLLEK_B8(96)
+  GOLLEK_B8(128)
+  GOLLEK_B8(256)
+#undef GOLLEK_B8
+  throw std::runtime_error("block-scaled decode attention: unsupported head_dim " + std::to_string(D));
 }
 
 void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void* cache, const float* scales,
                           const int* tables, int64_t bt_stride, int mb, const int* lens, int B, int H, int Hk, int D,
-                          int bs, int num_blocks, int splits, float scale, int window, float softcap, float* part_o,
-                          float* part_ml, float* scores, float* mass, bool e4m3, cudaStream_t s) {
+                          int bs, int num_blocks, const Block8Plan& plan, float scale, int window, float softcap,
+                          float* workspace, float* mass, bool e4m3, cudaStream_t s) {
   DecArgs p;
   p.bs_log2 = log2_block(bs);
   if (B == 0) return;
@@ -926,54 +1220,60 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.tables = tables;
   p.lens = lens;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
-  p.part_o = part_o;
-  p.part_ml = part_ml;
-  p.scores = scores;
+  p.part_o = workspace;
+  p.part_ml = p.part_o + plan.n_o;
+  p.scores = p.part_ml + plan.n_ml;
+  p.row_ml = p.scores + plan.n_scores;
+  p.spans = reinterpret_cast<int*>(p.row_ml + plan.n_row);
   p.mass = mass;
   p.q_stride = q_stride;
   p.bt_stride = bt_stride;
-  p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.splits = splits, p.mb = mb, p.num_blocks = num_blocks, p.window = window;
-  const int nt = (p.G > 8 && D <= 128) ? 2 : 1;  // D = 256: two column tiles would need 128 accumulators a lane
-  p.NG = (p.G + 8 * nt - 1) / (8 * nt);
+  p.B = B, p.H = H, p.Hk = Hk, p.G = H / Hk, p.NG = plan.ng, p.grid = plan.grid, p.mb = mb, p.num_blocks = num_blocks;
+  p.window = window;
   p.scale_log2 = scale * kLog2e;
   p.cap = softcap > 0.f ? 2.f / softcap : 0.f;  // scores are in log2 units: e^(2 x / cap) = 2^(2 x log2(e) / cap)
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
-  throw_if(p.G > 128, "block-scaled decode attention: at most 128 query heads per KV head");
-  const int64_t grid = (int64_t)B * Hk * p.NG * splits;
-  throw_if(grid > 0x7fffffff, "block-scaled decode attention: grid too large");
-  bool done = false;
-  auto go = [&](auto kern, int smem) {
+  const int mass_tiles = mass ? ((mb << p.bs_log2) + 127) / 128 : 0;
+  const int64_t join = (int64_t)B * H + (int64_t)B * Hk * mass_tiles;
+  throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
+  auto go = [&](auto kern, int threads, int smem) {
     GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<(unsigned)grid, kDecWarps * 32, smem, s>>>(p);
-    done = true;
+    kern<<<(unsigned)plan.grid, threads, smem, s>>>(p);
   };
-#define GOLLEK_B8_M(DD, NN, M)                                                          \
-  if (e4m3) go(block8_decode_kernel<DD, NN, true, M>, kDecWarps * DecShape<DD>::kRing); \
-  else go(block8_decode_kernel<DD, NN, false, M>, kDecWarps * DecShape<DD>::kRing)
-#define GOLLEK_B8_N(DD, NN) \
-  if (mass) { GOLLEK_B8_M(DD, NN, true); } else { GOLLEK_B8_M(DD, NN, false); }
+#define GOLLEK_B8_M(DD, NN, E, M) \
+  go(block8_decode_kernel<DD, NN, E, M>, DecShape<DD, NN>::kThreads, DecShape<DD, NN>::kSmem)
+#define GOLLEK_B8_N(DD, NN)                             \
+  if (e4m3) {                                           \
+    if (mass) GOLLEK_B8_M(DD, NN, true, true);          \
+    else GOLLEK_B8_M(DD, NN, true, false);              \
+  } else {                                              \
+    if (mass) GOLLEK_B8_M(DD, NN, false, true);         \
+    else GOLLEK_B8_M(DD, NN, false, false);             \
+  }
 #define GOLLEK_B8(DD) \
   if (D == DD) {      \
-    if (nt == 1) { GOLLEK_B8_N(DD, 1) } else { GOLLEK_B8_N(DD, 2) } \
+    if (plan.nt == 1) { GOLLEK_B8_N(DD, 1) } else { GOLLEK_B8_N(DD, 2) } \
   }
   GOLLEK_B8(32)
   GOLLEK_B8(64)
   GOLLEK_B8(96)
   GOLLEK_B8(128)
-  if (D == 256) { GOLLEK_B8_N(256, 1) }
+  GOLLEK_B8(256)
 #undef GOLLEK_B8
 #undef GOLLEK_B8_N
 #undef GOLLEK_B8_M
-  throw_if(!done, "block-scaled decode attention: unsupported head_dim " + std::to_string(D));
   check_launch("block8_decode");
-  const int mass_tiles = mass ? ((mb << p.bs_log2) + 255) / 256 : 0;
-  const int64_t join = (splits > 1 ? (int64_t)B * H : 0) + (int64_t)B * Hk * mass_tiles;
-  throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
-  if (join > 0) {
-    block8_join_kernel<<<(unsigned)join, 128, 0, s>>>(p, D, mass_tiles);
-    check_launch("block8_join");
-  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)join);
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its CTAs start as the decode kernel's leave
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, block8_join_kernel, p, D, 8 * plan.nt, mass_tiles));
 }
 
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,

@@ -253,13 +253,18 @@ void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, 
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
                               const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
                               void* dst, cudaStream_t s);
-int block8_decode_splits(int B, int Hk, int G, int D, int64_t max_len);
-// part_o / part_ml: fp32 [B * H, splits, D] and [B * H, splits, 2] (splits > 1, or mass); scores: fp32
-// [B * Hk, mb * bs, G] (mass)
+// Decode attention over it: a grid of CTAs that share the batch's steps evenly, and the fp32 workspace (counts of
+// floats, in this order) for what they share.
+struct Block8Plan {
+  int grid = 1, nt = 1, ng = 1, tokens = 0;
+  int64_t n_o = 0, n_ml = 0, n_scores = 0, n_row = 0, n_span = 0;
+  int64_t floats() const { return n_o + n_ml + n_scores + n_row + n_span; }
+};
+Block8Plan block8_plan(int B, int H, int Hk, int D, int64_t width, int splits, bool mass);
 void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void* cache, const float* scales,
                           const int* tables, int64_t bt_stride, int mb, const int* lens, int B, int H, int Hk, int D,
-                          int bs, int num_blocks, int splits, float scale, int window, float softcap, float* part_o,
-                          float* part_ml, float* scores, float* mass, bool e4m3, cudaStream_t s);
+                          int bs, int num_blocks, const Block8Plan& plan, float scale, int window, float softcap,
+                          float* workspace, float* mass, bool e4m3, cudaStream_t s);
 // cache [layers, NB, 2, Hk, bs, D]; kept int32 [layers, B, Hk, max_keep]
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
                      const int* lens, const int* keep, int* kept, int layers, int B, int Hk, int D, int bs,

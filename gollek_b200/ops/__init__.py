@@ -187,8 +187,9 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
     e4m3 * scale of its token and head (head_dim 128).
 
     ``kv_scales`` fp32 [NB, 2, Hk]: block-scaled cache (see ``kv_quant_blocks``; head_dim 32, 64, 96,
-    128 or 256). A sequence of length 0 gives zeros. ``num_splits`` 0 lets the kernel choose from the
-    shapes. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
+    128 or 256). A sequence of length 0 gives zeros. The CTAs share the batch's tokens evenly:
+    ``num_splits`` 0 fills the GPU, n > 0 takes n CTAs per sequence and KV head on average; without a
+    ``workspace`` one is allocated per call. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
     heads of its KV head, is added to it; where rows share a block all of them are added, and only
     then the last bits depend on their order."""
     if kv_scales is not None and kv_scales.dim() == 3:
@@ -216,20 +217,8 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
 def _decode_block8(q, cache, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap, scales, mass):
     if not q.is_cuda:
         return _cpu(ref.block8_decode(q, cache, scales, block_tables, seq_lens, scale, window, softcap, mass), out)
-    B, H, D = q.shape
-    ext = cuda_ext()
-    width = block_tables.shape[1] * cache.shape[3]
-    if num_splits <= 0:
-        num_splits = ext.block8_decode_splits(B, cache.shape[2], H // max(1, cache.shape[2]), D, width)
-    out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-    # fp32 partial outputs and softmax sums of the splits, and the scores that become weights
-    n = B * H * ((num_splits * D if num_splits > 1 else 0) + (2 * num_splits if num_splits > 1 or mass is not None else 0)
-                 + (width if mass is not None else 0))
-    if n and workspace is None:
-        workspace = torch.empty(n, dtype=torch.float32, device=q.device)
-    _C(2 if n else 1).block8_decode(out, q, cache, scales, block_tables, seq_lens, float(scale), int(num_splits),
-                                    workspace, int(window), float(softcap), mass)
-    return out
+    return _C(2).block8_decode(q, cache, scales, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap,
+                               mass)
 
 
 # ---------------------------------------------------------------------------- fp8 KV cache
