@@ -257,8 +257,9 @@ constexpr float kSlack = 8.f;  // p * scale <= 2^9: within f16
 template <int D, int NT>
 struct DecShape {
   static constexpr int kChunks = D / 16;                            // 16-byte chunks of a token row
-  static constexpr int kWarps = D == 256 ? 4 : D / 16;              // D = 256: 4 warps of 4 chunks, two CTAs per SM
-  static constexpr int kTokens = 16 * kWarps;                       // of a step
+  static constexpr int kWarps = D >= 128 ? 4 : D / 16;              // a warp owns D / (16 W) chunks of O
+  static constexpr int kTiles = D == 128 || D == 64 ? 2 : 1;                   // tiles of 16 tokens a warp scores in a step
+  static constexpr int kTokens = 16 * kWarps * kTiles;              // of a step
   static constexpr int kOwn = kChunks / kWarps;                     // chunks of O a warp owns
   static constexpr bool kSwizzle = kChunks % 8 == 0;
   // rows of 8 chunks are swizzled, others padded to an odd number: 8 rows of one chunk hit 8 bank groups
@@ -267,14 +268,14 @@ struct DecShape {
   static constexpr int kQRow = 2 * D + 16;
   static constexpr bool kStageQ = NT == 1;                          // a head tile's Q arrives with its first step
   static constexpr int kQ = kStageQ ? 8 * kQRow : 0;                // (two column tiles leave no room for it)
-  static constexpr int kStage = (2 * kSide + kQ + 8 * kWarps + 15) / 16 * 16;  // K, V, Q, tile scales
-  static constexpr int kStages = D <= 64 ? 4 : 3;
+  static constexpr int kStage = (2 * kSide + kQ + 8 * kWarps * kTiles + 15) / 16 * 16;  // K, V, Q, tile scales
+  static constexpr int kStages = D < 64 ? 4 : D == 96 ? 3 : 2;
   static constexpr int kPRow = 2 * kTokens + 16;
   static constexpr int kP = NT * 8 * kPRow;
   static constexpr int kSmem = kStages * kStage + kP;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kFit = (227 * 1024) / (kSmem + 1024 + 2 * kWarps * NT * 8 * 4);
-  static constexpr int kRegs = 65536 / (kThreads * (D == 256 ? 168 : NT == 2 ? 120 : 96));
+  static constexpr int kRegs = 65536 / (kThreads * (NT == 2 ? (D >= 128 ? 224 : 128) : D >= 128 ? 168 : D == 64 ? 128 : 96));
   static constexpr int kCtas = kFit < kRegs ? kFit : kRegs;         // resident CTAs per SM
 };
 
@@ -408,7 +409,7 @@ template <int D, int NT, bool E4M3, bool MASS>
 __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kCtas)
     block8_decode_kernel(const DecArgs p) {
   using S = DecShape<D, NT>;
-  constexpr int CH = S::kChunks, HB = 8 * NT, W = S::kWarps, T = S::kTokens, OWN = S::kOwn;
+  constexpr int CH = S::kChunks, HB = 8 * NT, W = S::kWarps, TW = S::kTiles, T = S::kTokens, OWN = S::kOwn;
   extern __shared__ __align__(128) uint8_t dsm[];
   __shared__ float sm_x[W][HB], sm_l[W][HB];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -452,74 +453,77 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
     at.s = (int)((first - before) % at.r.n);
   }
 
-  // block ids of this warp's tiles are read 32 steps at a time, one batch ahead of their use
+  // block ids of this warp's tiles are read 32 at a time, one batch ahead of their use
+  constexpr int BATCH = 32 / TW;  // steps
   DecPlace ahead = at;
   auto load_ids = [&]() {
     int id = 0;
     if (ahead.b < p.B) {
-      const int t = ahead.r.t0 + (ahead.s + lane) * T + warp * 16;
+      const int t = ahead.r.t0 + (ahead.s + lane / TW) * T + (warp * TW + lane % TW) * 16;
       if (t < ahead.r.L)
         id = checked_index(p.tables[(int64_t)ahead.b * p.bt_stride + (t >> p.bs_log2)], p.num_blocks, p.bounds);
-      ahead.s += 32;
+      ahead.s += BATCH;
       if (ahead.s >= ahead.r.n) next_head(ahead, p, T);
     }
     return id;
   };
-  int ids = 0, ids_next = load_ids(), batch = 32;
+  int ids = 0, ids_next = load_ids(), batch = BATCH;
   int issued = 0;
   // a lane's pieces of a tile: 16 bytes at lane * 16 + 512 i, i.e. row lane / CH + 32 / CH i where CH divides 32
   const uint32_t block_bytes = (uint32_t)(2 * p.Hk << p.bs_log2) * D, v_bytes = block_bytes >> 1;
   uint32_t st_issue = ring;  // stage of the next step to issue
   auto issue = [&]() {
     if (issued < count) {
-      if (batch == 32) ids = ids_next, ids_next = load_ids(), batch = 0;
-      const uint32_t id = __shfl_sync(0xffffffffu, ids, batch);
-      const uint32_t st = st_issue;
-      const int t = at.r.t0 + at.s * T + warp * 16;
-      const int off = t & ((1 << p.bs_log2) - 1);
-      const uint8_t* gk = p.cache + (uint64_t)id * block_bytes + (uint32_t)((at.kh << p.bs_log2) + off) * D;
-      const uint8_t* gv = gk + v_bytes;
-      const uint32_t tail = st + 2 * S::kSide + S::kQ;
-      if (32 % CH == 0 && t >= at.r.lo && t + 16 <= at.r.L) {  // a whole tile
-        constexpr int R = 32 / CH;  // rows per round
-        const int row = lane / CH, ch = lane % CH;
-        const uint8_t *ck = gk + lane * 16, *cv = gv + lane * 16;
-        // with the swizzle a lane's chunk changes with the rounds' row parity bits only
-        const uint32_t d0 = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
-        const uint32_t d1 = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ ((row + R) & 7) : ch) << 4);
-        constexpr int N = CH / 2, RB = R * S::kRow;
+      if (batch == BATCH) ids = ids_next, ids_next = load_ids(), batch = 0;
+      const uint32_t st = st_issue, tail = st + 2 * S::kSide + S::kQ;
+#pragma unroll
+      for (int q = 0; q < TW; ++q) {
+        const uint32_t id = __shfl_sync(0xffffffffu, ids, batch * TW + q);
+        const int tile = warp * TW + q, t = at.r.t0 + at.s * T + tile * 16;
+        const int off = t & ((1 << p.bs_log2) - 1);
+        const uint8_t* gk = p.cache + (uint64_t)id * block_bytes + (uint32_t)((at.kh << p.bs_log2) + off) * D;
+        const uint8_t* gv = gk + v_bytes;
+        if (32 % CH == 0 && t >= at.r.lo && t + 16 <= at.r.L) {  // a whole tile
+          constexpr int R = 32 / CH;  // rows per round
+          const int row = lane / CH, ch = lane % CH;
+          const uint8_t *ck = gk + lane * 16, *cv = gv + lane * 16;
+          // with the swizzle a lane's chunk changes with the rounds' row parity bits only
+          const uint32_t d0 = st + (tile * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
+          const uint32_t d1 = st + (tile * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ ((row + R) & 7) : ch) << 4);
+          constexpr int N = CH / 2, RB = R * S::kRow;
 #define GOLLEK_TILE(I)                                                       \
-  if constexpr (I < N) {                                                     \
-    cp_async16<(I) * RB, (I) * 512>(((I) & 1) ? d1 : d0, ck);                \
-    cp_async16<(I) * RB + S::kSide, (I) * 512>(((I) & 1) ? d1 : d0, cv);     \
-  }
-        if constexpr (N <= 4) {
-          GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(2) GOLLEK_TILE(3)
-        } else {  // D = 256: two rows a round, four different chunks
-          const uint32_t d2 = st + (warp * 16 + row) * S::kRow + ((ch ^ ((row + 2 * R) & 7)) << 4);
-          const uint32_t d3 = st + (warp * 16 + row) * S::kRow + ((ch ^ ((row + 3 * R) & 7)) << 4);
-          GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(4) GOLLEK_TILE(5)
-          cp_async16<2 * RB, 1024>(d2, ck);
-          cp_async16<2 * RB + S::kSide, 1024>(d2, cv);
-          cp_async16<6 * RB, 3072>(d2, ck);
-          cp_async16<6 * RB + S::kSide, 3072>(d2, cv);
-          cp_async16<3 * RB, 1536>(d3, ck);
-          cp_async16<3 * RB + S::kSide, 1536>(d3, cv);
-          cp_async16<7 * RB, 3584>(d3, ck);
-          cp_async16<7 * RB + S::kSide, 3584>(d3, cv);
-        }
+    if constexpr (I < N) {                                                     \
+      cp_async16<(I) * RB, (I) * 512>(((I) & 1) ? d1 : d0, ck);                \
+      cp_async16<(I) * RB + S::kSide, (I) * 512>(((I) & 1) ? d1 : d0, cv);     \
+    }
+          if constexpr (N <= 4) {
+            GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(2) GOLLEK_TILE(3)
+          } else {  // D = 256: two rows a round, four different chunks
+            const uint32_t d2 = st + (tile * 16 + row) * S::kRow + ((ch ^ ((row + 2 * R) & 7)) << 4);
+            const uint32_t d3 = st + (tile * 16 + row) * S::kRow + ((ch ^ ((row + 3 * R) & 7)) << 4);
+            GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(4) GOLLEK_TILE(5)
+            cp_async16<2 * RB, 1024>(d2, ck);
+            cp_async16<2 * RB + S::kSide, 1024>(d2, cv);
+            cp_async16<6 * RB, 3072>(d2, ck);
+            cp_async16<6 * RB + S::kSide, 3072>(d2, cv);
+            cp_async16<3 * RB, 1536>(d3, ck);
+            cp_async16<3 * RB + S::kSide, 1536>(d3, cv);
+            cp_async16<7 * RB, 3584>(d3, ck);
+            cp_async16<7 * RB + S::kSide, 3584>(d3, cv);
+          }
 #undef GOLLEK_TILE
-      } else {
+        } else {
 #pragma unroll 1
-        for (int i = 0; i < CH / 2; ++i) {
-          const int e = i * 32 + lane, row = e / CH, ch = e % CH;
-          const int bytes = t + row >= at.r.lo && t + row < at.r.L ? 16 : 0;  // rows outside read as zero
-          const uint32_t d = st + (warp * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
-          cp_async16_or_zero<0, 0>(d, gk + e * 16, bytes);
-          cp_async16_or_zero<S::kSide, 0>(d, gv + e * 16, bytes);
+          for (int i = 0; i < CH / 2; ++i) {
+            const int e = i * 32 + lane, row = e / CH, ch = e % CH;
+            const int bytes = t + row >= at.r.lo && t + row < at.r.L ? 16 : 0;  // rows outside read as zero
+            const uint32_t d = st + (tile * 16 + row) * S::kRow + ((S::kSwizzle ? ch ^ (row & 7) : ch) << 4);
+            cp_async16_or_zero<0, 0>(d, gk + e * 16, bytes);
+            cp_async16_or_zero<S::kSide, 0>(d, gv + e * 16, bytes);
+          }
         }
+        if (lane < 2) cp_async4(tail + 8 * tile + 4 * lane, p.scales + (uint64_t)(id * 2 + lane) * p.Hk + at.kh);
       }
-      if (lane < 2) cp_async4(tail + 8 * warp + 4 * lane, p.scales + (uint64_t)(id * 2 + lane) * p.Hk + at.kh);
       if (S::kStageQ && (at.s == 0 || issued == 0)) {
         const int h0 = at.hg * HB, nh = min(p.G - h0, HB);
         const __nv_bfloat16* q = p.q + (int64_t)at.b * p.q_stride + (int64_t)(at.kh * p.G + h0) * D;
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
       st_issue = st_issue == ring + (S::kStages - 1) * S::kStage ? ring : st_issue + S::kStage;
       if (++at.s == at.r.n) {
         next_head(at, p, T);
-        batch = 32;
+        batch = BATCH;
       }
     }
     cp_async_commit();
@@ -607,84 +611,96 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
     }
 
     // scores of this warp's 16 tokens
-    const int tile = tok0 + warp * 16, tok = tile + g;
-    float s[NT][4], s2[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
-    const uint32_t kb = st + (warp * 16 + frow) * S::kRow;
-#pragma unroll
-    for (int j2 = 0; j2 < CH / 2; ++j2) {
-      uint32_t r[4], a[4];
-      ldsm4(r, kb + ((S::kSwizzle ? (2 * j2) ^ (fhi ^ (frow & 7)) : 2 * j2 + fhi) << 4));
-      expand4<E4M3, false>(r[0], a[0], a[2]);
-      expand4<E4M3, false>(r[1], a[1], a[3]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a, qf[nt][2 * j2][0], qf[nt][2 * j2][1]);
-      expand4<E4M3, false>(r[2], a[0], a[2]);
-      expand4<E4M3, false>(r[3], a[1], a[3]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) mma_f16(s2[nt], a, qf[nt][2 * j2 + 1][0], qf[nt][2 * j2 + 1][1]);
-    }
-    float ks, vs;
-    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs) : "r"(tail + 8 * warp) : "memory");
-    if (tile >= cur.r.L) vs = 0.f;  // no token here: whatever scale was read, the probabilities are 0
-    const float ev = (float)max((int)((__float_as_uint(vs) >> 23) & 0xff) - 127, -100);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = (s[nt][e] + s2[nt][e]) * (ks * qmul[nt][e & 1]);
-    if (p.cap > 0.f) {  // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2 x / cap)))
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[nt][e] * p.cap)));
-    }
-    bool ok0 = true, ok1 = true;
-    if (tile < cur.r.lo || tile + 16 > cur.r.L) {
-      ok0 = tok >= cur.r.lo && tok < cur.r.L, ok1 = tok + 8 >= cur.r.lo && tok + 8 < cur.r.L;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = (e < 2 ? ok0 : ok1) ? s[nt][e] : -INFINITY;
-    }
+    float s[TW][NT][4], vs[TW], ev[TW];
     bool up = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      up |= fmaxf(s[nt][0], s[nt][2]) + ev > m[nt][0] + kSlack || fmaxf(s[nt][1], s[nt][3]) + ev > m[nt][1] + kSlack;
-    if constexpr (MASS) {
-      float* sc = p.scores + ((int64_t)(b * p.Hk + kh) * (p.mb << p.bs_log2) + tok) * p.G + h0;
-      const bool pairs = (p.G & 1) == 0;  // a token's scores of two heads lie at a multiple of 8 bytes
+    for (int q = 0; q < TW; ++q) {
+      const int tile = tok0 + (warp * TW + q) * 16, tok = tile + g;
+      float s2[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const int hh = nt * 8 + 2 * c;
-          float* d = sc + (e < 2 ? 0 : 8 * p.G) + hh;
-          if (!(e < 2 ? ok0 : ok1) || hh >= nh) continue;
-          if (pairs) {
-            *reinterpret_cast<float2*>(d) = make_float2(s[nt][e], s[nt][e + 1]);
-          } else {
-            d[0] = s[nt][e];
-            if (hh + 1 < nh) d[1] = s[nt][e + 1];
+        for (int e = 0; e < 4; ++e) s[q][nt][e] = s2[nt][e] = 0.f;
+      const uint32_t kb = st + ((warp * TW + q) * 16 + frow) * S::kRow;
+#pragma unroll
+      for (int j2 = 0; j2 < CH / 2; ++j2) {
+        uint32_t r[4], a[4];
+        ldsm4(r, kb + ((S::kSwizzle ? (2 * j2) ^ (fhi ^ (frow & 7)) : 2 * j2 + fhi) << 4));
+        expand4<E4M3, false>(r[0], a[0], a[2]);
+        expand4<E4M3, false>(r[1], a[1], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(s[q][nt], a, qf[nt][2 * j2][0], qf[nt][2 * j2][1]);
+        expand4<E4M3, false>(r[2], a[0], a[2]);
+        expand4<E4M3, false>(r[3], a[1], a[3]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma_f16(s2[nt], a, qf[nt][2 * j2 + 1][0], qf[nt][2 * j2 + 1][1]);
+      }
+      float ks;
+      asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs[q]) : "r"(tail + 8 * (warp * TW + q)) : "memory");
+      if (tile >= cur.r.L) vs[q] = 0.f;  // no token here: whatever scale was read, the probabilities are 0
+      ev[q] = (float)max((int)((__float_as_uint(vs[q]) >> 23) & 0xff) - 127, -100);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[q][nt][e] = (s[q][nt][e] + s2[nt][e]) * (ks * qmul[nt][e & 1]);
+      if (p.cap > 0.f) {  // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2 x / cap)))
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[q][nt][e] = p.cap_log2 * (1.f - __fdividef(2.f, 1.f + ex2(s[q][nt][e] * p.cap)));
+      }
+      bool ok0 = true, ok1 = true;
+      if (tile < cur.r.lo || tile + 16 > cur.r.L) {
+        ok0 = tok >= cur.r.lo && tok < cur.r.L, ok1 = tok + 8 >= cur.r.lo && tok + 8 < cur.r.L;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[q][nt][e] = (e < 2 ? ok0 : ok1) ? s[q][nt][e] : -INFINITY;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        up |= fmaxf(s[q][nt][0], s[q][nt][2]) + ev[q] > m[nt][0] + kSlack ||
+              fmaxf(s[q][nt][1], s[q][nt][3]) + ev[q] > m[nt][1] + kSlack;
+      if constexpr (MASS) {
+        float* sc = p.scores + ((int64_t)(b * p.Hk + kh) * (p.mb << p.bs_log2) + tok) * p.G + h0;
+        const bool pairs = (p.G & 1) == 0;  // a token's scores of two heads lie at a multiple of 8 bytes
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const int hh = nt * 8 + 2 * c;
+            float* d = sc + (e < 2 ? 0 : 8 * p.G) + hh;
+            if (!(e < 2 ? ok0 : ok1) || hh >= nh) continue;
+            if (pairs) {
+              *reinterpret_cast<float2*>(d) = make_float2(s[q][nt][e], s[q][nt][e + 1]);
+            } else {
+              d[0] = s[q][nt][e];
+              if (hh + 1 < nh) d[1] = s[q][nt][e + 1];
+            }
           }
-        }
+      }
     }
     // probabilities in f16 (2^-11 relative): the output's bf16 rounding is eight times coarser
-    const uint32_t pd = psm + g * S::kPRow + warp * 32 + 4 * c;
-    float e4[NT][4];
+    const uint32_t pd = psm + g * S::kPRow + warp * TW * 32 + 4 * c;
+    float sum[NT][2];
     auto put = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        sum[nt][0] = sum[nt][1] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) e4[nt][e] = ex2(s[nt][e] - m[nt][e & 1]);  // a masked score is -inf
-        const __half2 u = __floats2half2_rn(e4[nt][0] * vs, e4[nt][1] * vs);
-        const __half2 v = __floats2half2_rn(e4[nt][2] * vs, e4[nt][3] * vs);
-        const uint32_t x0 = movm_t(*reinterpret_cast<const uint32_t*>(&u));  // now tokens 2 c, 2 c + 1 of head g
-        const uint32_t x1 = movm_t(*reinterpret_cast<const uint32_t*>(&v));
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow), "r"(x0) : "memory");
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow + 16), "r"(x1) : "memory");
+        for (int q = 0; q < TW; ++q) {
+          float e4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) e4[e] = ex2(s[q][nt][e] - m[nt][e & 1]);  // a masked score is -inf
+          sum[nt][0] += e4[0] + e4[2];
+          sum[nt][1] += e4[1] + e4[3];
+          const __half2 u = __floats2half2_rn(e4[0] * vs[q], e4[1] * vs[q]);
+          const __half2 v = __floats2half2_rn(e4[2] * vs[q], e4[3] * vs[q]);
+          const uint32_t x0 = movm_t(*reinterpret_cast<const uint32_t*>(&u));  // now tokens 2 c, 2 c + 1 of head g
+          const uint32_t x1 = movm_t(*reinterpret_cast<const uint32_t*>(&v));
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow + q * 32), "r"(x0) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(pd + nt * 8 * S::kPRow + q * 32 + 16), "r"(x1) : "memory");
+        }
       }
     };
     put();
@@ -693,7 +709,9 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float y = fmaxf(s[nt][e], s[nt][e + 2]) + ev;
+          float y = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < TW; ++q) y = fmaxf(y, fmaxf(s[q][nt][e], s[q][nt][e + 2]) + ev[q]);
           y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
           y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
           y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
@@ -717,11 +735,11 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
       __syncthreads();
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) l[nt][0] += e4[nt][0] + e4[nt][2], l[nt][1] += e4[nt][1] + e4[nt][3];
+    for (int nt = 0; nt < NT; ++nt) l[nt][0] += sum[nt][0], l[nt][1] += sum[nt][1];
 
     // O^T of this warp's dims over the step's tokens, two tiles at a time (tiles behind L are zero)
 #pragma unroll
-    for (int t2 = 0; t2 < W / 2; ++t2) {
+    for (int t2 = 0; t2 < T / 32; ++t2) {
       uint32_t pb[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) ldsm4(pb[nt], psm + (nt * 8 + (lane & 7)) * S::kPRow + t2 * 64 + (lane >> 3) * 16);
