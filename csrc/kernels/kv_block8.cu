@@ -831,21 +831,28 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
   return make_float2(M, warp_sum(sum));
 }
 
-// Joins the parts of the head tiles that several CTAs shared, and zeroes empty rows: the first B * H CTAs, one per
-// (row, head); the others add the softmax weights of 128 tokens of a (row, kv head) to mass, summed over the head group
-// in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows share a block.
-__global__ void __launch_bounds__(128) block8_join_kernel(const DecArgs p, int D, int HB, int mass_tiles) {
+// Joins the parts of the head tiles that several CTAs shared, and zeroes empty rows: the first ceil(B * H / 2) CTAs, half a
+// CTA per (row, head); the others add the softmax weights of kMassTokens tokens of a (row, kv head) to mass, summed over the
+// head group in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
+// share a block.
+constexpr int kJoinThreads = 256, kMassTokens = 1024;
+
+template <int GV>  // heads per KV head where they are 1, 2, 4 or 8, else 0
+__global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB, int mass_tiles) {
   __shared__ float sm[128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
+  const int joins = (p.B * p.H + 1) >> 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
-  if ((int)blockIdx.x < p.B * p.H) {
-    const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
+  if ((int)blockIdx.x < joins) {
+    const int row = blockIdx.x * 2 + (threadIdx.x >> 7), d0 = threadIdx.x & 127;
+    if (row >= p.B * p.H) return;
+    const int b = row / p.H, h = row - b * p.H;
     const int kh = h / p.G, hx = h - kh * p.G, x = kh * p.NG + hx / HB, hh = hx % HB;
     const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + x];
     const int L = min(p.lens[b], p.mb << p.bs_log2);
-    __nv_bfloat16* out = p.out + (int64_t)blockIdx.x * D;
+    __nv_bfloat16* out = p.out + (int64_t)row * D;
     if (L <= 0) {
-      for (int i = threadIdx.x; i < D; i += 128) out[i] = __float2bfloat16(0.f);
+      for (int i = d0; i < D; i += 128) out[i] = __float2bfloat16(0.f);
       return;
     }
     const int n = span.y;
@@ -859,50 +866,51 @@ __global__ void __launch_bounds__(128) block8_join_kernel(const DecArgs p, int D
       const float m = p.part_ml[k * 2], f = m == -INFINITY ? 0.f : ex2(m - all.x);
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        if ((int)threadIdx.x + 128 * e < D) acc[e] += f * p.part_o[k * D + threadIdx.x + 128 * e];
+        if (d0 + 128 * e < D) acc[e] += f * p.part_o[k * D + d0 + 128 * e];
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      if ((int)threadIdx.x + 128 * e < D) out[threadIdx.x + 128 * e] = __float2bfloat16(acc[e] * inv);
+      if (d0 + 128 * e < D) out[d0 + 128 * e] = __float2bfloat16(acc[e] * inv);
     return;
   }
-  const int i = blockIdx.x - p.B * p.H;
+  const int i = blockIdx.x - joins;
   const int bk = i / mass_tiles, b = bk / p.Hk, kh = bk - b * p.Hk;
   const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2), lo = p.window > 0 ? max(0, L - p.window) : 0;
-  const int first = (i - bk * mass_tiles) * 128, t = first + threadIdx.x;
-  if (first >= L || first + 128 <= lo) return;
-  const bool mine = t >= lo && t < L;
-  // the token's scores and block are on their way while the heads' sums are joined
-  const float* sc = p.scores + ((int64_t)bk * (p.mb << p.bs_log2) + t) * p.G;
-  float v[8];
-  int id = 0;
-  if (mine) id = checked_index(p.tables[(int64_t)b * p.bt_stride + (t >> p.bs_log2)], p.num_blocks, p.bounds);
-  if (p.G % 4 == 0) {
-#pragma unroll
-    for (int h = 0; h < 8; h += 4)
-      if (mine && h < p.G) {
-        const float4 y = *reinterpret_cast<const float4*>(sc + h);
-        v[h] = y.x, v[h + 1] = y.y, v[h + 2] = y.z, v[h + 3] = y.w;
-      }
-  } else {
-#pragma unroll
-    for (int h = 0; h < 8; ++h)
-      if (mine && h < p.G) v[h] = sc[h];
-  }
-  for (int h = warp; h < p.G; h += 4) {
+  const int first = (i - bk * mass_tiles) * kMassTokens;
+  if (first >= L || first + kMassTokens <= lo) return;
+  for (int h = warp; h < p.G; h += kJoinThreads / 32) {
     const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
     const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
                                   : join_ml(p, span.x, span.y, HB, h % HB);
     if (lane == 0) sm[h] = ml.x + log2f(ml.y);
   }
   __syncthreads();
-  if (!mine) return;
-  float w = 0.f;
+  const float* sc = p.scores + (int64_t)bk * (p.mb << p.bs_log2) * p.G;
+  const int* bt = p.tables + (int64_t)b * p.bt_stride;
+  float* mass = p.mass + (kh << p.bs_log2);
+  const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
+  constexpr int GN = GV > 0 ? GV : 1;
+  float lse[GN];
 #pragma unroll
-  for (int h = 0; h < 8; ++h)
-    if (h < p.G) w += ex2(v[h] - sm[h]);
-  for (int h = 8; h < p.G; ++h) w += ex2(sc[h] - sm[h]);
-  atomicAdd(p.mass + (((int64_t)id * p.Hk + kh) << p.bs_log2) + (t & ((1 << p.bs_log2) - 1)), w);
+  for (int h = 0; h < GN; ++h) lse[h] = sm[h];
+#pragma unroll 4
+  for (int t = max(first, lo) + threadIdx.x; t < min(first + kMassTokens, L); t += kJoinThreads) {
+    float w = 0.f;
+    if constexpr (GV > 0) {
+      float v[GN];
+      if constexpr (GV == 1) v[0] = sc[t];
+      if constexpr (GV == 2) *reinterpret_cast<float2*>(v) = reinterpret_cast<const float2*>(sc)[t];
+      if constexpr (GV >= 4)
+#pragma unroll
+        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v + h) = reinterpret_cast<const float4*>(sc)[(t * GV + h) / 4];
+#pragma unroll
+      for (int h = 0; h < GN; ++h) w += ex2(v[h] - lse[h]);
+    } else {
+      for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
+    }
+    const int id = checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
+    atomicAdd(mass + (int64_t)id * row + (t & mask), w);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1252,8 +1260,8 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.cap = softcap > 0.f ? 2.f / softcap : 0.f;  // scores are in log2 units: e^(2 x / cap) = 2^(2 x log2(e) / cap)
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
-  const int mass_tiles = mass ? ((mb << p.bs_log2) + 127) / 128 : 0;
-  const int64_t join = (int64_t)B * H + (int64_t)B * Hk * mass_tiles;
+  const int mass_tiles = mass ? ((mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
+  const int64_t join = ((int64_t)B * H + 1) / 2 + (int64_t)B * Hk * mass_tiles;
   throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
   auto go = [&](auto kern, int threads, int smem) {
     GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -1284,14 +1292,19 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   check_launch("block8_decode");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)join);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its CTAs start as the decode kernel's leave
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, block8_join_kernel, p, D, 8 * plan.nt, mass_tiles));
+  auto join_kernel = block8_join_kernel<0>;
+  if (mass && p.G == 1) join_kernel = block8_join_kernel<1>;
+  if (mass && p.G == 2) join_kernel = block8_join_kernel<2>;
+  if (mass && p.G == 4) join_kernel = block8_join_kernel<4>;
+  if (mass && p.G == 8) join_kernel = block8_join_kernel<8>;
+  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel, p, D, 8 * plan.nt, mass_tiles));
 }
 
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
