@@ -982,6 +982,7 @@ GOLLEK_DEVICE uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t& tot
 __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const EvictArgs p) {
   extern __shared__ uint32_t keys[];
   __shared__ uint32_t hist[2048], warp_sums[kSelThreads / 32], found[2];
+  __shared__ uint2 counts[kSelThreads / 32];
   const int h = blockIdx.x, b = blockIdx.y, ly = blockIdx.z;
   const EvictRow r = evict_row(p, b);
   int* kept = p.kept + (((int64_t)ly * p.B + b) * p.Hk + h) * p.max_keep;
@@ -1036,115 +1037,254 @@ __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const Evic
     bits_done += width;
     __syncthreads();
   }
-  // prefix is the smallest key that stays, `want` how many tokens with it do (the first ones)
-  uint32_t gt0 = 0, eq0 = 0;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + threadIdx.x;
-    const uint32_t k = i < n ? (held ? keys[i] : load(i)) : 0u;
-    const uint32_t gt = i < n && k > prefix, eq = i < n && k == prefix;
-    uint32_t total;
-    const uint32_t before = block_scan((gt << 16) | eq, warp_sums, total);
-    const uint32_t gb = gt0 + (before >> 16), eb = eq0 + (before & 0xffffu);
-    if (gt || (eq && eb < want)) kept[a + gb + min(eb, want)] = c0 + i;
-    gt0 += total >> 16;
-    eq0 += total & 0xffffu;
+  // prefix is the smallest key that stays, `want` how many tokens with it do (the first ones). Every warp counts
+  // a stretch of the candidates, then lists it behind the stretches before.
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kSelThreads / 32;
+  const int per = ((n + warps - 1) / warps + 31) & ~31, i0 = min(n, warp * per), i1 = min(n, i0 + per);
+  uint32_t gt = 0, eq = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t k = i < i1 ? (held ? keys[i] : load(i)) : 0u;
+    gt += __popc(__ballot_sync(0xffffffffu, i < i1 && k > prefix));
+    eq += __popc(__ballot_sync(0xffffffffu, i < i1 && k == prefix));
+  }
+  if (lane == 0) counts[warp] = make_uint2(gt, eq);
+  __syncthreads();
+  gt = eq = 0;
+  for (int w = 0; w < warp; ++w) gt += counts[w].x, eq += counts[w].y;
+  const uint32_t before = (1u << lane) - 1;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const uint32_t k = i < i1 ? (held ? keys[i] : load(i)) : 0u;
+    const uint32_t bg = __ballot_sync(0xffffffffu, i < i1 && k > prefix), be = __ballot_sync(0xffffffffu, i < i1 && k == prefix);
+    const uint32_t g = gt + __popc(bg & before), e = eq + __popc(be & before);
+    if (((bg >> lane) & 1) || (((be >> lane) & 1) && e < want)) kept[a + g + min(e, want)] = c0 + i;
+    gt += __popc(bg);
+    eq += __popc(be);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Eviction, step 2: the kept tokens move to the front, in order. One CTA per (layer, sequence, kv head, K/V).
+// Eviction, step 2: the kept tokens move to the front, in order. One CTA per (layer, sequence, kv head, K / V / mass).
 //
-// In place: kept[j] >= j, so a chunk's sources lie at or behind its own places and every chunk that is
-// overwritten by it has been read (chunks go up, a chunk's loads end before its stores). Each destination block
-// gets the smallest power-of-two scale for what it then holds.
+// In place: kept[j] >= j, so a chunk's sources lie at or behind its own places. A chunk may be read as early as one likes
+// (what goes before it is written in front of it), and must be read before it or any later one is written: chunks go
+// up, and a chunk's loads end before a barrier that its stores follow. So codes are read two chunks ahead (cp.async
+// into a ring; a thread only touches the pieces that it loaded itself), the indices and block ids they hang on earlier
+// still. Each destination block gets the smallest power-of-two scale for what it then holds: one barrier a chunk, for its
+// largest magnitude.
 // ---------------------------------------------------------------------------------------------
+// A magnitude costs one instruction a value (packed 16-bit maxima), a change of scale by a power of two two, all exact.
 constexpr int kMoveThreads = 256;
+constexpr int kMovePieces = 4;  // 16-byte pieces per thread and chunk
+constexpr int kMoveStages = 3;
+constexpr int kMoveStage = kMoveThreads * (kMovePieces * 16 + 8);  // codes, then their scales
+constexpr int kMoveSmem = kMoveStages * kMoveStage;
 
+// Running maximum magnitude of four codes each in two 16-bit lanes: hi and lo of int8, magnitude bits of e4m3.
 template <bool E4M3>
-__global__ void __launch_bounds__(kMoveThreads) kv_evict_move_kernel(const EvictArgs p) {
-  constexpr int kItems = 4;       // 16-byte pieces per thread and chunk
-  __shared__ uint32_t top[64];    // largest magnitude of each destination block of the chunk (float bits)
-  const int h = blockIdx.x >> 1, w = blockIdx.x & 1, b = blockIdx.y, ly = blockIdx.z;
-  const EvictRow r = evict_row(p, b);
-  if (!r.cut || r.K == 0) return;
-  const int bs = 1 << p.bs_log2, vec = p.D >> 4;
-  const int chunk = kMoveThreads * kItems / vec / 64 * 64;  // tokens, a multiple of every block size
+struct Top4 {
+  uint32_t hi = 0, lo = 0;
+  GOLLEK_DEVICE void add(uint32_t w) {
+    if constexpr (E4M3) {  // the bits below the sign order like the magnitudes
+      hi = __vimax3_u16x2(hi, w & 0x007f007fu, (w >> 8) & 0x007f007fu);
+    } else {  // bytes sign-extended to 16 bits
+      uint32_t e, o;
+      asm("prmt.b32 %0, %1, 0, 0xa280;" : "=r"(e) : "r"(w));
+      asm("prmt.b32 %0, %1, 0, 0xb391;" : "=r"(o) : "r"(w));
+      hi = __vimax3_s16x2(hi, e, o);
+      lo = __vimin3_s16x2(lo, e, o);
+    }
+  }
+  GOLLEK_DEVICE float value() const {
+    if constexpr (E4M3) {
+      float f[4];
+      decode4<true>(max(hi & 0xffffu, hi >> 16), f);
+      return f[0];
+    } else {
+      const int a = max((int)(int16_t)hi, (int)(int16_t)(hi >> 16)), b = min((int)(int16_t)lo, (int)(int16_t)(lo >> 16));
+      return (float)max(a, -b);
+    }
+  }
+};
+
+// Codes times a ratio of scales. A power of two within f16's reach goes through f16 exactly: e4m3 by a product, int8 by
+// one fma on 1152 + code whose sum with 1536 rounds to the integer (ties to even); others go through fp32.
+template <bool E4M3, int N>
+GOLLEK_DEVICE void rescale(uint32_t* w, float ratio) {
+  if (ratio == 1.f) return;
+  const uint32_t b = __float_as_uint(ratio);
+  const int e = (int)(b >> 23) - 127;
+  const __half2 m = __float2half2_rn(ratio);
+  if ((b & 0x7fffffu) == 0 && (E4M3 ? e >= -14 && e <= 6 : e >= -7 && e <= 5)) {
+    const __half2 c = __float2half2_rn(1536.f - 1152.f * ratio);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (E4M3) {
+        uint32_t lo, hi;
+        expand4<true, false>(w[i], lo, hi);
+        const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&lo), m), y = __hmul2(*reinterpret_cast<const __half2*>(&hi), m);
+        const uint32_t p = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&x), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t q = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&y), __NV_SATFINITE, __NV_E4M3);
+        w[i] = p | (q << 16);
+      } else {
+        const uint32_t ev = (w[i] & 0x00ff00ffu) ^ 0x64806480u, od = ((w[i] >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+        const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&ev), m, c), y = __hfma2(*reinterpret_cast<const __half2*>(&od), m, c);
+        w[i] = __byte_perm(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y), 0x6240);
+      }
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < N; ++i) {
+      float f[4];
+      decode4<E4M3>(w[i], f);
+      w[i] = encode4<E4M3>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+    }
+  }
+}
+
+// The masses of the kept tokens, the same way: a chunk's loads end before its stores.
+GOLLEK_DEVICE void move_masses(const EvictArgs& p, const EvictRow& r, int h, int b, int ly) {
+  constexpr int N = 8;
   const int* kept = p.kept + (((int64_t)ly * p.B + b) * p.Hk + h) * p.max_keep;
   const int* bt = p.tables + (int64_t)b * p.bt_stride;
-  const int64_t pool = (int64_t)ly * p.num_blocks;
-  auto row_of = [&](int t) {  // (block, K/V, head) row of token t's block
-    const int64_t id = pool + checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
-    return (id * 2 + w) * p.Hk + h;
+  float* mass = p.mass + (((int64_t)ly * p.num_blocks * p.Hk + h) << p.bs_log2);
+  const int mask = (1 << p.bs_log2) - 1;
+  auto at = [&](int t) {
+    const int id = checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
+    return mass + (uint64_t)(uint32_t)id * (p.Hk << p.bs_log2) + (t & mask);
   };
-  auto mass_at = [&](int t) {
-    const int64_t id = pool + checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
-    return p.mass + ((id * p.Hk + h) << p.bs_log2) + (t & (bs - 1));
-  };
-  for (int base = 0; base < r.K; base += chunk) {
-    const int n = min(chunk, r.K - base);
-    if (threadIdx.x < 64) top[threadIdx.x] = 0u;
-    __syncthreads();
-    uint4 code[kItems];
-    float sc[kItems];
+  for (int base = threadIdx.x; base - (int)threadIdx.x < r.K; base += N * kMoveThreads) {
+    float v[N];
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int e = k * kMoveThreads + threadIdx.x, j = e / vec;
-      sc[k] = 0.f;
-      if (j < n) {
-        const int t = kept[base + j];
-        const int64_t row = row_of(t);
-        code[k] = *reinterpret_cast<const uint4*>(p.cache + ((row << p.bs_log2) + (t & (bs - 1))) * p.D + (e % vec) * 16);
-        sc[k] = p.scales[row];
-      }
-    }
-    float mv[2];  // masses travel with the K pass (chunk <= 2 * kMoveThreads)
-    if (w == 0)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (k * kMoveThreads + (int)threadIdx.x < n) mv[k] = *mass_at(kept[base + k * kMoveThreads + threadIdx.x]);
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int j = (k * kMoveThreads + threadIdx.x) / vec;
-      if (j < n) {
-        float f[16], amax = 0.f;
-        decode4<E4M3>(code[k].x, f);
-        decode4<E4M3>(code[k].y, f + 4);
-        decode4<E4M3>(code[k].z, f + 8);
-        decode4<E4M3>(code[k].w, f + 12);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(f[i]));
-        atomicMax(&top[j >> p.bs_log2], __float_as_uint(amax * sc[k]));
-      }
-    }
+    for (int k = 0; k < N; ++k)
+      if (base + k * kMoveThreads < r.K) v[k] = *at(kept[base + k * kMoveThreads]);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int e = k * kMoveThreads + threadIdx.x, j = e / vec;
-      if (j < n) {
-        const int to = base + j;
-        const float s = pow2_scale<E4M3>(__uint_as_float(top[j >> p.bs_log2]));
-        const float ratio = sc[k] / s;
-        const int64_t row = row_of(to);
-        float f[16];
-        decode4<E4M3>(code[k].x, f);
-        decode4<E4M3>(code[k].y, f + 4);
-        decode4<E4M3>(code[k].z, f + 8);
-        decode4<E4M3>(code[k].w, f + 12);
-        uint4 o;
-        o.x = encode4<E4M3>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
-        o.y = encode4<E4M3>(f[4] * ratio, f[5] * ratio, f[6] * ratio, f[7] * ratio);
-        o.z = encode4<E4M3>(f[8] * ratio, f[9] * ratio, f[10] * ratio, f[11] * ratio);
-        o.w = encode4<E4M3>(f[12] * ratio, f[13] * ratio, f[14] * ratio, f[15] * ratio);
-        *reinterpret_cast<uint4*>(p.cache + ((row << p.bs_log2) + (to & (bs - 1))) * p.D + (e % vec) * 16) = o;
-        if ((to & (bs - 1)) == 0 && e % vec == 0) p.scales[row] = s;
-      }
-    }
-    if (w == 0)
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (k * kMoveThreads + (int)threadIdx.x < n) *mass_at(base + k * kMoveThreads + threadIdx.x) = mv[k];
-    __syncthreads();
+    for (int k = 0; k < N; ++k)
+      if (base + k * kMoveThreads < r.K) *at(base + k * kMoveThreads) = v[k];
   }
+}
+
+// NP: pieces of one token that a thread takes (4, or 2 where the head size is no multiple of 64: then two tokens).
+template <bool E4M3, int NP>
+__global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const EvictArgs p) {
+  constexpr int NI = kMovePieces / NP;  // tokens per thread and chunk
+  extern __shared__ __align__(16) uint8_t ring[];
+  // largest magnitude of each destination block of a chunk (float bits): one being filled, one read, one cleared
+  __shared__ uint32_t top[3][64];
+  const int h = blockIdx.x / 3, w = blockIdx.x % 3, b = blockIdx.y, ly = blockIdx.z;  // w: K, V, masses
+  const EvictRow r = evict_row(p, b);
+  if (!r.cut || r.K == 0) return;
+  if (w == 2) {
+    move_masses(p, r, h, b, ly);
+    return;
+  }
+  const int bs = 1 << p.bs_log2, share = p.D / (16 * NP);       // threads of a token
+  const int chunk = kMoveThreads * NI / share / 64 * 64;        // tokens, a multiple of every block size
+  const int chunks = (r.K + chunk - 1) / chunk;
+  // a warp's threads of one destination block: all, half of it, or (a head size that leaves a rest) unknown
+  const int lanes = 32 % share != 0 ? 1 : min(32, bs * share);
+  const uint32_t group = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
+  const int* kept = p.kept + (((int64_t)ly * p.B + b) * p.Hk + h) * p.max_keep;
+  const int* bt = p.tables + (int64_t)b * p.bt_stride;
+  // a block's K (or V) of this head and its scale: base + block id * stride
+  const uint32_t row_stride = (uint32_t)(2 * p.Hk << p.bs_log2) * p.D;
+  uint8_t* codes = p.cache + ((int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h) * ((int64_t)p.D << p.bs_log2);
+  float* scales = p.scales + (int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h;
+  int tok[NI];  // this thread's tokens in a chunk; its pieces are piece + 16 share i
+#pragma unroll
+  for (int k = 0; k < NI; ++k) {
+    tok[k] = (k * kMoveThreads + (int)threadIdx.x) / share;
+    if (tok[k] >= chunk) tok[k] = 1 << 30;  // beyond the chunk (a head size that leaves a rest): never below its length
+  }
+  auto piece = [&](int k) { return (k * kMoveThreads + (int)threadIdx.x) % share * 16; };
+  auto block_of = [&](int t) { return checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds); };
+  auto code_at = [&](int id, int t, int k) { return codes + (uint64_t)(uint32_t)id * row_stride + (t & (bs - 1)) * p.D + piece(k); };
+  auto scale_at = [&](int id) { return scales + (uint64_t)(uint32_t)id * (2 * p.Hk); };
+
+  // indices of a chunk, block ids of a chunk, codes and scales of a chunk: each one step behind the one before
+  int src2[NI], src1[NI], id1[NI];
+  auto load_src = [&](int c, int* src) {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) src[k] = tok[k] < r.K - c * chunk ? kept[c * chunk + tok[k]] : -1;
+  };
+  auto load_ids = [&](const int* src, int* id) {
+#pragma unroll
+    for (int k = 0; k < NI; ++k) id[k] = src[k] >= 0 ? block_of(src[k]) : 0;
+  };
+  auto load_codes = [&](int c, const int* src, const int* id) {
+    const uint32_t st = smem_u32(ring) + (c % kMoveStages) * kMoveStage + threadIdx.x * 16;
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      if (src[k] < 0) continue;
+      const uint8_t* g = code_at(id[k], src[k], k);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) cp_async16<0, 0>(st + (NP * k + i) * kMoveThreads * 16, g + i * share * 16);
+      cp_async4(st + kMovePieces * kMoveThreads * 16 - threadIdx.x * 12 + k * kMoveThreads * 4, scale_at(id[k]));
+    }
+    cp_async_commit();
+  };
+  if (threadIdx.x < 64) top[0][threadIdx.x] = 0u;
+  // chunk 0 and 1's codes on their way, chunk 2's ids and chunk 3's indices too
+  load_src(0, src2);
+  load_src(1, src1);
+  load_ids(src2, id1);
+  load_codes(0, src2, id1);
+  load_ids(src1, id1);
+  load_codes(1, src1, id1);
+  load_src(2, src1);
+  load_src(3, src2);
+  load_ids(src1, id1);
+  __syncthreads();
+  for (int c = 0; c < chunks; ++c) {
+    const int base = c * chunk, n = min(chunk, r.K - base);
+    load_codes(c + 2, src1, id1);
+    int to_id[NI];  // destination blocks
+#pragma unroll
+    for (int k = 0; k < NI; ++k) to_id[k] = tok[k] < n ? block_of(base + tok[k]) : 0;
+#pragma unroll
+    for (int k = 0; k < NI; ++k) src1[k] = src2[k];
+    load_ids(src1, id1);
+    load_src(c + 4, src2);
+    cp_async_wait<2>();
+    uint32_t code[NI][4 * NP];
+    float sc[NI];
+    const uint8_t* st = ring + (c % kMoveStages) * kMoveStage;
+    uint32_t* tp = top[c % 3];
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      uint32_t amax = 0u;
+      if (tok[k] < n) {
+        Top4<E4M3> t;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          const uint4 x = reinterpret_cast<const uint4*>(st)[(NP * k + i) * kMoveThreads + threadIdx.x];
+          code[k][4 * i] = x.x, code[k][4 * i + 1] = x.y, code[k][4 * i + 2] = x.z, code[k][4 * i + 3] = x.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * NP; ++i) t.add(code[k][i]);
+        sc[k] = reinterpret_cast<const float*>(st + kMovePieces * kMoveThreads * 16)[k * kMoveThreads + threadIdx.x];
+        amax = __float_as_uint(t.value() * sc[k]);
+      }
+      amax = __reduce_max_sync(group, amax);
+      if ((threadIdx.x & (lanes - 1)) == 0 && tok[k] < n) atomicMax(&tp[tok[k] >> p.bs_log2], amax);
+    }
+    if (threadIdx.x < 64) top[(c + 1) % 3][threadIdx.x] = 0u;  // its readers are behind the last barrier, its writers the next
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NI; ++k) {
+      if (tok[k] >= n) continue;
+      const int to = base + tok[k];
+      const float s = pow2_scale<E4M3>(__uint_as_float(tp[tok[k] >> p.bs_log2]));
+      rescale<E4M3, 4 * NP>(code[k], sc[k] * __uint_as_float((254u << 23) - __float_as_uint(s)));  // sc / s, s = 2^e
+      uint8_t* d = code_at(to_id[k], to, k);
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        *reinterpret_cast<uint4*>(d + i * share * 16) =
+            make_uint4(code[k][4 * i], code[k][4 * i + 1], code[k][4 * i + 2], code[k][4 * i + 3]);
+      if ((to & (bs - 1)) == 0 && piece(k) == 0) *scale_at(to_id[k]) = s;
+    }
+  }
+  cp_async_wait<0>();
 }
 
 int log2_block(int bs) {
@@ -1310,7 +1450,7 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
                      const int* lens, const int* keep, int* kept, int layers, int B, int Hk, int D, int bs,
                      int num_blocks, int sink, int recent, int max_keep, bool e4m3, cudaStream_t s) {
-  throw_if(D % 16 != 0 || D < 32 || D > 256, "kv_evict: head_dim must be a multiple of 16, 32 to 256");
+  throw_if(D % 32 != 0 || D > 256, "kv_evict: head_dim must be a multiple of 32, <= 256");
   throw_if(B > 65535 || layers > 65535, "kv_evict: at most 65535 sequences and layers");
   EvictArgs p;
   p.bs_log2 = log2_block(bs);
@@ -1331,8 +1471,10 @@ void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables,
   kv_evict_select_kernel<<<dim3(Hk, B, layers), kSelThreads, smem, s>>>(p);
   check_launch("kv_evict_select");
   if (max_keep == 0) return;
-  auto k = e4m3 ? kv_evict_move_kernel<true> : kv_evict_move_kernel<false>;
-  k<<<dim3(2 * Hk, B, layers), kMoveThreads, 0, s>>>(p);
+  auto k = D % 64 == 0 ? (e4m3 ? kv_evict_move_kernel<true, 4> : kv_evict_move_kernel<false, 4>)
+                       : (e4m3 ? kv_evict_move_kernel<true, 2> : kv_evict_move_kernel<false, 2>);
+  GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveSmem));
+  k<<<dim3(3 * Hk, B, layers), kMoveThreads, kMoveSmem, s>>>(p);
   check_launch("kv_evict_move");
 }
 
