@@ -747,9 +747,9 @@ void kv_quant_blocks_py(torch::Tensor kv, torch::Tensor slots, torch::Tensor cac
   check_same_device(slots, cache);
   TORCH_CHECK(kv.dim() == 4 && kv.size(1) == 2 && kv.size(2) == cache.size(2) && kv.size(3) == cache.size(4),
               "kv must be [T, 2, Hk, D] like the cache");
-  TORCH_CHECK(kv.stride(3) == 1 && kv.stride(0) % 4 == 0 && kv.stride(1) % 4 == 0 && kv.stride(2) % 4 == 0 &&
-                  reinterpret_cast<uintptr_t>(kv.data_ptr()) % 8 == 0,
-              "kv: unit stride over D, rows at multiples of 8 bytes");
+  TORCH_CHECK(kv.stride(3) == 1 && kv.stride(0) % 8 == 0 && kv.stride(1) % 8 == 0 && kv.stride(2) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(kv.data_ptr()) % 16 == 0,
+              "kv: unit stride over D, rows at multiples of 16 bytes");
   TORCH_CHECK(slots.dim() == 1 && slots.is_contiguous() && slots.numel() >= kv.size(0), "one slot per token");
   float* mp = check_mass(mass, cache, 0);
   c10::cuda::CUDAGuard guard(cache.device());

@@ -21,7 +21,6 @@ namespace gollek {
 
 namespace {
 
-constexpr float kBf16Max = 3.3895313892515355e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------------------------------------
@@ -71,116 +70,210 @@ GOLLEK_DEVICE void decode4(uint32_t w, float* f) {
 // A run is found by its first token: the token whose nearest earlier token with a slot lies in another block.
 // The warp takes the run's largest magnitude, fixes the block's scale (a run that writes the block's
 // first slot starts the block anew, any other can only raise the scale), rounds the codes already
-// there to a raised scale, and stores the run's codes. Memory-bound: 3 bytes a value.
+// there to a raised scale, and stores the run's codes. Memory-bound: 3 bytes a value. A run of at most 16 tokens stays
+// in registers between its magnitude and its codes (16-byte loads, all of them in flight at once); a longer one is read twice.
 // ---------------------------------------------------------------------------------------------
-GOLLEK_DEVICE float clean(float x) {  // NaN -> 0, infinities -> the largest bf16
-  return x == x ? fminf(fmaxf(x, -kBf16Max), kBf16Max) : 0.f;
+GOLLEK_DEVICE uint32_t clean2(uint32_t w) {  // two bf16: NaN -> 0, infinities -> the largest bf16
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 16) {
+    const uint32_t x = (w >> i) & 0xffffu, a = x & 0x7fffu;
+    r |= (a > 0x7f80u ? 0u : a == 0x7f80u ? (x & 0x8000u) | 0x7f7fu : x) << i;
+  }
+  return r;
+}
+GOLLEK_DEVICE uint4 clean8(const uint4& u) { return make_uint4(clean2(u.x), clean2(u.y), clean2(u.z), clean2(u.w)); }
+// Running maximum of magnitudes in two bf16 lanes (NaN stays visible).
+GOLLEK_DEVICE void top8(uint32_t& m, const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = w[i] & 0x7fff7fffu;
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(a));
+  }
+}
+GOLLEK_DEVICE bool not_finite(uint32_t m) { return (m & 0x7fffu) >= 0x7f80u || (m >> 16) >= 0x7f80u; }
+GOLLEK_DEVICE float top_value(uint32_t m) { return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)); }
+// Eight bf16 times inv -> codes; |value * inv| <= qmax and the product is exact, so adding 1.5 * 2^23 rounds it to the
+// integer (ties to even) that the sum's low byte is.
+template <bool E4M3>
+GOLLEK_DEVICE uint2 encode8(const uint4& u, float inv) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float a = __uint_as_float(w[2 * i] << 16), b = __uint_as_float(w[2 * i] & 0xffff0000u);
+    const float d = __uint_as_float(w[2 * i + 1] << 16), e = __uint_as_float(w[2 * i + 1] & 0xffff0000u);
+    if constexpr (E4M3) {
+      c[i] = encode4<true>(a * inv, b * inv, d * inv, e * inv);
+    } else {
+      constexpr float kRound = 12582912.f;
+      const uint32_t x = __byte_perm(__float_as_uint(fmaf(a, inv, kRound)), __float_as_uint(fmaf(b, inv, kRound)), 0x0040);
+      const uint32_t y = __byte_perm(__float_as_uint(fmaf(d, inv, kRound)), __float_as_uint(fmaf(e, inv, kRound)), 0x0040);
+      c[i] = __byte_perm(x, y, 0x5410);
+    }
+  }
+  return make_uint2(c[0], c[1]);
 }
 
-template <bool E4M3, int NCH>  // NCH: 4-value pieces per lane (D <= 128 * NCH)
-__global__ void __launch_bounds__(256)
-    kv_quant_blocks_kernel(const __nv_bfloat16* __restrict__ kv, int64_t st, int64_t sw, int64_t sh,
-                           const int* __restrict__ slots, uint8_t* __restrict__ cache, float* __restrict__ scales,
-                           float* __restrict__ mass, int T, int Hk, int D, int bs_log2, int num_blocks, int g,
-                           uint32_t* bounds) {
+struct QuantArgs {
+  const __nv_bfloat16* kv;
+  int64_t st, sw, sh;  // element strides of kv [T, 2, Hk, D]
+  const int* slots;
+  uint8_t* cache;
+  float* scales;
+  float* mass;
+  int T, Hk, bs_log2, num_blocks, g;  // g: tokens a warp looks at
+  uint32_t* bounds;
+};
+
+template <bool E4M3, int D>
+__global__ void __launch_bounds__(256) kv_quant_blocks_kernel(const QuantArgs p) {
+  constexpr int LPR = D / 8, TPI = 32 / LPR;      // lanes of a row (8 values each), rows a warp takes at once
+  constexpr int R = (16 + TPI - 1) / TPI;         // rounds for 16 rows
   const int64_t gw = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int pair = (int)(gw % (2 * Hk));
-  const int64_t grp = gw / (2 * Hk);
-  const int t0 = (int)(grp * g);
-  if (t0 >= T) return;
-  const int w = pair / Hk, h = pair % Hk;
-  const int bs = 1 << bs_log2;
-  const int pieces = D >> 2;
-  // lane i: slot of token t0 - 1 + i; lanes 1 .. g are this warp's tokens
+  const int lane = threadIdx.x & 31, sub = lane / LPR, pos = lane % LPR;
+  const int64_t grp = gw / (2 * p.Hk);
+  const int pair = (int)(gw - grp * (2 * p.Hk));
+  const int t0 = (int)(grp * p.g);
+  if (t0 >= p.T) return;
+  const int w = pair / p.Hk, h = pair - w * p.Hk;
+  const int bs = 1 << p.bs_log2;
+  const __nv_bfloat16* kv = p.kv + w * p.sw + h * p.sh + pos * 8;
+  // lane i: slot of token t0 - 1 + i; lanes 1 .. g are this warp's tokens, the others show where a run ends
   const int tl = t0 - 1 + lane;
-  const int sl = (tl >= 0 && tl < T && lane <= g) ? slots[tl] : -1;
-  const int bl = sl >= 0 ? sl >> bs_log2 : -1;
+  const int sl = tl >= 0 && tl < p.T ? p.slots[tl] : -1;
+  const int bl = sl >= 0 ? sl >> p.bs_log2 : -1;
   const int bp = __shfl_up_sync(0xffffffffu, bl, 1);
-  uint32_t leaders = __ballot_sync(0xffffffffu, lane >= 1 && bl >= 0 && bl != bp);
+  uint32_t leaders = __ballot_sync(0xffffffffu, lane >= 1 && lane <= p.g && bl >= 0 && bl != bp);
   while (leaders) {
     const int li = __ffs(leaders) - 1;
     leaders &= leaders - 1;
     const int tlead = t0 - 1 + li;
     const int blk = __shfl_sync(0xffffffffu, bl, li);
-    // a skipped token before it: look further back for the nearest token with a slot
-    int back = tlead - 1;
-    while (back >= 0 && slots[back] < 0) --back;
-    if (back >= 0 && (slots[back] >> bs_log2) == blk) continue;
-    if (checked_index(blk, num_blocks, bounds, -1) < 0) continue;  // beyond the pool: skipped
-    // pass 1: largest magnitude, offsets written
-    float amax = 0.f;
-    uint64_t written = 0;
-    int tend = tlead;
-    for (bool more = true; more && tend < T;) {
-      const int s = tend + lane < T ? slots[tend + lane] : -1;
-      const bool other = s >= 0 && (s >> bs_log2) != blk;
-      const uint32_t om = __ballot_sync(0xffffffffu, other);
-      const int n = min(T - tend, om ? __ffs(om) - 1 : 32);
-      more = om == 0;
-      const uint32_t valid = __ballot_sync(0xffffffffu, s >= 0 && lane < n);
-      for (int i0 = 0; i0 < n; i0 += 8) {
-        uint2 raw[8][NCH];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int c = 0; c < NCH; ++c) {
-            raw[i][c] = make_uint2(0u, 0u);
-            if (i0 + i < n && ((valid >> (i0 + i)) & 1) && lane + 32 * c < pieces)
-              raw[i][c] = reinterpret_cast<const uint2*>(kv + (int64_t)(tend + i0 + i) * st + w * sw + h * sh)[lane + 32 * c];
-          }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int c = 0; c < NCH; ++c) {
-            const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i][c].x));
-            const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i][c].y));
-            amax = fmaxf(amax, fmaxf(fmaxf(fabsf(clean(a.x)), fabsf(clean(a.y))), fmaxf(fabsf(clean(b.x)), fabsf(clean(b.y)))));
-          }
-      }
-      uint32_t lo = 0, hi = 0;
-      if ((valid >> lane) & 1) {
-        const int off = s & (bs - 1);
-        if (off < 32) lo = 1u << off; else hi = 1u << (off - 32);
-      }
-      written |= (uint64_t)__reduce_or_sync(0xffffffffu, lo) | ((uint64_t)__reduce_or_sync(0xffffffffu, hi) << 32);
-      tend += n;
+    if (__shfl_sync(0xffffffffu, bp, li) < 0) {  // a skipped token (or none) before it: look for the nearest one with a slot
+      int back = tlead - 1;
+      while (back >= 0 && p.slots[back] < 0) --back;
+      if (back >= 0 && (p.slots[back] >> p.bs_log2) == blk) continue;
     }
-    amax = warp_max(amax);
-    const int64_t row = ((int64_t)blk * 2 + w) * Hk + h;
-    const float old = scales[row];
-    const float need = pow2_scale<E4M3>(amax);
+    if (checked_index(blk, p.num_blocks, p.bounds, -1) < 0) continue;  // beyond the pool: skipped
+    const int64_t row = ((int64_t)blk * 2 + w) * p.Hk + h;
+    uint8_t* codes = p.cache + (row << p.bs_log2) * D;
+    // the run's tokens among the lanes, and whether they are all of it
+    const uint32_t other = __ballot_sync(0xffffffffu, lane > li && bl >= 0 && bl != blk);
+    const uint32_t run = __ballot_sync(0xffffffffu, lane >= li && bl >= 0 && (other == 0 || lane < __ffs(other) - 1));
+    const int span = 32 - __clz(run) - li;  // tokens from the first to the last one
+    const int off = bl == blk && ((run >> lane) & 1) ? sl & (bs - 1) : 64;
+    uint64_t written = (uint64_t)__reduce_or_sync(0xffffffffu, off < 32 ? 1u << off : 0u) |
+                       ((uint64_t)__reduce_or_sync(0xffffffffu, off >= 32 && off < 64 ? 1u << (off - 32) : 0u) << 32);
+    const bool held = (other != 0 || tlead - li + 32 >= p.T) && span <= 16 && __popc(run) == __popcll(written);
+    uint4 raw[R];
+    uint32_t m = 0;
+    bool special = false;
+    int tend = tlead;
+    if (held) {  // at most 16 tokens, every slot once: they stay in registers
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int i = r * TPI + sub;
+        raw[r] = make_uint4(0u, 0u, 0u, 0u);
+        if (sub < TPI && i < span && ((run >> (li + i)) & 1)) raw[r] = *reinterpret_cast<const uint4*>(kv + (int64_t)(tlead + i) * p.st);
+      }
+    } else {
+      written = 0;
+      for (bool more = true; more && tend < p.T;) {
+        const int s = tend + lane < p.T ? p.slots[tend + lane] : -1;
+        const uint32_t om = __ballot_sync(0xffffffffu, s >= 0 && (s >> p.bs_log2) != blk);
+        const int n = min(p.T - tend, om ? __ffs(om) - 1 : 32);
+        more = om == 0;
+        for (int i0 = 0; i0 < n; i0 += 16) {
+          bool bad = false;
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const int i = i0 + r * TPI + sub;
+            const int si = __shfl_sync(0xffffffffu, s, i & 31);
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (sub < TPI && i < min(n, i0 + 16) && si >= 0) u = *reinterpret_cast<const uint4*>(kv + (int64_t)(tend + i) * p.st);
+            uint32_t x = 0;
+            top8(x, u);
+            if (not_finite(x)) {
+              bad = true;
+              x = 0;
+              top8(x, clean8(u));
+            }
+            asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(x));
+          }
+          special |= bad;
+        }
+        const int o = s >= 0 && lane < n ? s & (bs - 1) : 64;
+        written |= (uint64_t)__reduce_or_sync(0xffffffffu, o < 32 ? 1u << o : 0u) |
+                   ((uint64_t)__reduce_or_sync(0xffffffffu, o >= 32 && o < 64 ? 1u << (o - 32) : 0u) << 32);
+        tend += n;
+      }
+    }
+    const float old = p.scales[row];
+    if (held) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) top8(m, raw[r]);
+      if (not_finite(m)) {
+        m = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          raw[r] = clean8(raw[r]);
+          top8(m, raw[r]);
+        }
+      }
+    }
+    const float need = pow2_scale<E4M3>(warp_max(top_value(m)));
     const bool fresh = written & 1;
     const float s = fresh ? need : fmaxf(old, need);
-    uint32_t* codes = reinterpret_cast<uint32_t*>(cache + (row << bs_log2) * D);
     if (!fresh && s > old) {  // the block's scale grows: round what it holds to the new one
       const float ratio = old / s;
-      for (int off = 0; off < bs; ++off) {
-        if ((written >> off) & 1) continue;
-        for (int c = lane; c < pieces; c += 32) {
-          float f[4];
-          decode4<E4M3>(codes[off * pieces + c], f);
-          codes[off * pieces + c] = encode4<E4M3>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+#pragma unroll 1
+      for (int o0 = 0; o0 < bs; o0 += R * TPI) {
+        uint2 c[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int o = o0 + r * TPI + sub;
+          if (sub < TPI && o < bs) c[r] = *reinterpret_cast<const uint2*>(codes + o * D + pos * 8);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const int o = o0 + r * TPI + sub;
+          if (sub >= TPI || o >= bs || ((written >> o) & 1)) continue;
+          float f[8];
+          decode4<E4M3>(c[r].x, f);
+          decode4<E4M3>(c[r].y, f + 4);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] *= ratio;
+          *reinterpret_cast<uint2*>(codes + o * D + pos * 8) =
+              make_uint2(encode4<E4M3>(f[0], f[1], f[2], f[3]), encode4<E4M3>(f[4], f[5], f[6], f[7]));
         }
       }
     }
     __syncwarp();
-    if (lane == 0) scales[row] = s;
+    if (lane == 0) p.scales[row] = s;
     const float inv = 1.f / s;
-    for (int t = tlead; t < tend; ++t) {  // pass 2: the run's rows are in L1 / L2 now
-      const int slot = slots[t];
-      if (slot < 0) continue;
-      const int off = slot & (bs - 1);
+    const bool mass = p.mass != nullptr && w == 0 && pos == 0;
+    float* ms = p.mass + (((int64_t)blk * p.Hk + h) << p.bs_log2);
+    if (held) {
 #pragma unroll
-      for (int c = 0; c < NCH; ++c)
-        if (lane + 32 * c < pieces) {
-          const uint2 raw = reinterpret_cast<const uint2*>(kv + (int64_t)t * st + w * sw + h * sh)[lane + 32 * c];
-          const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.x));
-          const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw.y));
-          codes[off * pieces + lane + 32 * c] =
-              encode4<E4M3>(clean(a.x) * inv, clean(a.y) * inv, clean(b.x) * inv, clean(b.y) * inv);
-        }
-      if (mass != nullptr && w == 0 && lane == 0) mass[(((int64_t)blk * Hk + h) << bs_log2) + off] = 0.f;
+      for (int r = 0; r < R; ++r) {
+        const int i = r * TPI + sub, o = __shfl_sync(0xffffffffu, off, (li + i) & 31);
+        if (sub >= TPI || i >= span || !((run >> (li + i)) & 1)) continue;
+        *reinterpret_cast<uint2*>(codes + o * D + pos * 8) = encode8<E4M3>(raw[r], inv);
+        if (mass) ms[o] = 0.f;
+      }
+    } else {  // tokens in order: of two with the same slot the later one stays
+      special = __any_sync(0xffffffffu, special);
+      for (int t = tlead; t < tend; ++t) {
+        const int slot = p.slots[t];
+        if (slot < 0 || sub != 0) continue;
+        const int o = slot & (bs - 1);
+        uint4 u = *reinterpret_cast<const uint4*>(kv + (int64_t)t * p.st);
+        if (special) u = clean8(u);
+        *reinterpret_cast<uint2*>(codes + o * D + pos * 8) = encode8<E4M3>(u, inv);
+        if (mass) ms[o] = 0.f;
+      }
     }
   }
 }
@@ -1297,25 +1390,26 @@ int log2_block(int bs) {
 void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, const int* slots, void* cache,
                             float* scales, float* mass, int T, int Hk, int D, int bs, int num_blocks, bool e4m3,
                             cudaStream_t s) {
-  throw_if(D % 4 != 0 || D > 256, "block-scaled KV cache: head_dim must be a multiple of 4, <= 256");
-  const int lb = log2_block(bs);
+  QuantArgs p{reinterpret_cast<const __nv_bfloat16*>(kv), st, sw, sh, slots, reinterpret_cast<uint8_t*>(cache), scales, mass,
+              T, Hk, log2_block(bs), num_blocks, 1, bounds_status()};
   if (T == 0) return;
-  const int g = T >= 1024 ? 16 : 1;  // tokens a warp looks at: about one run of a prompt, one row of a decode step
-  const int64_t warps = (int64_t)((T + g - 1) / g) * 2 * Hk;
+  p.g = T >= 1024 ? 16 : 1;  // about one run of a prompt, one row of a decode step
+  const int64_t warps = (int64_t)((T + p.g - 1) / p.g) * 2 * Hk;
   const unsigned grid = (unsigned)((warps + 7) / 8);
-#define GOLLEK_QB(E, N)                                                                                              \
-  kv_quant_blocks_kernel<E, N><<<grid, 256, 0, s>>>(reinterpret_cast<const __nv_bfloat16*>(kv), st, sw, sh, slots,    \
-                                                    reinterpret_cast<uint8_t*>(cache), scales, mass, T, Hk, D, lb,    \
-                                                    num_blocks, g, bounds_status())
-  if (D <= 128) {
-    if (e4m3) GOLLEK_QB(true, 1);
-    else GOLLEK_QB(false, 1);
-  } else {
-    if (e4m3) GOLLEK_QB(true, 2);
-    else GOLLEK_QB(false, 2);
+#define GOLLEK_QB(DD)                                                        \
+  if (D == DD) {                                                             \
+    if (e4m3) kv_quant_blocks_kernel<true, DD><<<grid, 256, 0, s>>>(p);      \
+    else kv_quant_blocks_kernel<false, DD><<<grid, 256, 0, s>>>(p);          \
+    check_launch("kv_quant_blocks");                                         \
+    return;                                                                  \
   }
+  GOLLEK_QB(32)
+  GOLLEK_QB(64)
+  GOLLEK_QB(96)
+  GOLLEK_QB(128)
+  GOLLEK_QB(256)
 #undef GOLLEK_QB
-  check_launch("kv_quant_blocks");
+  throw_if(true, "block-scaled KV cache: unsupported head_dim " + std::to_string(D));
 }
 
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,

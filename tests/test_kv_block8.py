@@ -219,6 +219,20 @@ def test_write_long_runs_gpu(kind, T):
     assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 5, 40])
+def test_write_same_slot_twice_gpu(n):
+    """Of rows with the same slot the last one stays (and all of them count for the scale)."""
+    g = torch.Generator().manual_seed(n)
+    kv = torch.randn(n, 2, 2, 64, generator=g).bfloat16()
+    slots = torch.tensor([16 + (i // 2) % 16 for i in range(n)], dtype=torch.int32)
+    want = [torch.zeros(3, 2, 2, 16, 64, dtype=torch.int8), torch.zeros(3, 2, 2)]
+    got = [x.cuda() for x in want]
+    ops.kv_quant_blocks(kv, slots, *want)
+    ops.kv_quant_blocks(kv.cuda(), slots.cuda(), *got)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 # ------------------------------------------------------------------------------------------- decode
 LENS = [0, 1, 15, 16, 17, 31, 300, 700]
 
