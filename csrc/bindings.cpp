@@ -817,6 +817,60 @@ torch::Tensor block8_decode_py(torch::Tensor q, torch::Tensor cache, torch::Tens
   return out;
 }
 
+// Prompt attention over a block-scaled cache (head_dim 64 or 128): bf16 copy of the sequences' blocks, then the tcgen05 kernel.
+torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Tensor scales, torch::Tensor tables,
+                                torch::Tensor lens, torch::Tensor query_start, double scale,
+                                c10::optional<torch::Tensor> tiles, int64_t emu, c10::optional<torch::Tensor> out_opt,
+                                int64_t window, double softcap) {
+  const bool e4m3 = check_block8(cache, scales, false);
+  check_bf16(q, "q");
+  check_i32(query_start, "query_start");
+  check_same_device(q, cache);
+  check_same_device(query_start, cache);
+  const int64_t T = q.size(0), H = q.dim() == 3 ? q.size(1) : 0, D = cache.size(4), Hk = cache.size(2);
+  TORCH_CHECK(q.dim() == 3 && q.stride(2) == 1 && q.stride(1) == D && q.size(2) == D,
+              "q must be [T, H, D] with packed heads of the cache's D");
+  TORCH_CHECK(q.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
+              "q: rows at multiples of 16 bytes");
+  TORCH_CHECK(Hk > 0 && H % Hk == 0, "H must be a multiple of Hk");
+  TORCH_CHECK(query_start.dim() == 1 && query_start.is_contiguous() && query_start.numel() >= 1, "query_start [B + 1]");
+  const int64_t B = query_start.numel() - 1;
+  check_rows(tables, lens, cache, B);
+  c10::cuda::CUDAGuard guard(cache.device());
+  torch::Tensor out = out_opt.has_value() ? *out_opt : torch::empty({T, H, D}, q.options());
+  check_bf16(out, "out");
+  check_same_device(out, cache);
+  TORCH_CHECK(out.dim() == 3 && out.stride(2) == 1 && out.stride(1) == D && out.sizes() == q.sizes() &&
+                  out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
+              "out must be [T, H, D] like q");
+  const int64_t mb16 = tables.size(1) * cache.size(3) / 16;
+  TORCH_CHECK(B * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: the step's blocks exceed one copy's addresses");
+  auto copy = torch::empty({B * mb16, 2, Hk, 16, D}, q.options());
+  auto ids = torch::empty({B, mb16}, tables.options());
+  // Many items (4096 prompt tokens of 32 heads: 512): the work list's whole items balance by themselves, 155 us against
+  // 197 us in stretches, whose CTAs leave a quarter more parts. Few (eight chunks of 100 over 6000 cached tokens: 128): stretches
+  // fill the GPU and the tiles, 80 us against 104 us.
+  const bool list = tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 && tiles->size(0) >= 2 * device_num_sms();
+  launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>(), tables.stride(0),
+                           lens.data_ptr<int>(), B, tables.size(1), (int)cache.size(0), Hk, D, cache.size(3), e4m3,
+                           copy.data_ptr(), cur_stream(), ids.data_ptr<int>());
+  if (list) {
+    check_i32(*tiles, "tiles");
+    check_same_device(*tiles, cache);
+    TORCH_CHECK(tiles->is_contiguous(), "tiles: contiguous work list");
+    launch_paged_prefill_fa(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
+                            ids.data_ptr<int>(), (int)mb16, lens.data_ptr<int>(), query_start.data_ptr<int>(),
+                            tiles->data_ptr<int>(), tiles->size(0), (int)H, (int)Hk, (float)scale, (int)window,
+                            (float)softcap, (int)emu, cur_stream(), (int)D);
+    return out;
+  }
+  auto ws = torch::empty({prefill_stretch_bytes((int)B, (int)D)}, q.options().dtype(at::kByte));
+  launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
+                         ids.data_ptr<int>(), (int)mb16, lens.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H,
+                         (int)Hk, (float)scale, (int)window, (float)softcap, (int)D, ws.data_ptr(), cur_stream());
+  return out;
+}
+
 void kv_evict_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor mass, torch::Tensor tables,
                  torch::Tensor lens, torch::Tensor keep, torch::Tensor kept, int64_t sink, int64_t recent) {
   const bool e4m3 = check_block8(cache, scales, true);
@@ -1111,6 +1165,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block8_workspace", [](int64_t B, int64_t H, int64_t Hk, int64_t D, int64_t width, int64_t splits, bool mass) {
     return block8_plan((int)B, (int)H, (int)Hk, (int)D, width, (int)splits, mass).floats();
   });
+  m.def("block8_prefill", &block8_prefill_py);
   m.def("kv_evict", &kv_evict_py);
   m.def("num_sms", &device_num_sms);
   m.def("moe_forward", &moe_forward_out, "MoE layer: route, permute, grouped tcgen05 expert GEMMs, combine (K12)",

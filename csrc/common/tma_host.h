@@ -56,6 +56,25 @@ inline CUtensorMap make_tmap_2d(const void* base, CUtensorMapDataType dtype, int
   return m;
 }
 
+// 3-D tensor [d2, d1, d0] of `elem_bytes` elements, d0 contiguous, pitches ld1 and ld2 in elements. Box [b2, b1, b0].
+inline CUtensorMap make_tmap_3d(const void* base, CUtensorMapDataType dtype, int elem_bytes, uint64_t d0, uint64_t d1,
+                                uint64_t d2, uint64_t ld1, uint64_t ld2, uint32_t b0, uint32_t b1, uint32_t b2,
+                                CUtensorMapSwizzle swizzle) {
+  if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) throw std::runtime_error("TMA base address must be 16-byte aligned");
+  if ((ld1 * elem_bytes) % 16 != 0 || (ld2 * elem_bytes) % 16 != 0)
+    throw std::runtime_error("TMA pitches must be multiples of 16 bytes");
+  CUtensorMap m;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {ld1 * (uint64_t)elem_bytes, ld2 * (uint64_t)elem_bytes};
+  cuuint32_t box[3] = {b0, b1, b2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = get_encode_tiled()(&m, dtype, 3, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+  return m;
+}
+
 inline int num_sms() {
   static int n = 0;
   static std::once_flag once;

@@ -414,7 +414,32 @@ struct FaItem {
   int b, qs, ctx0, kh, jlo, jhi, kv_end;
   const int* bt;
   FaSlot sl[2];
+  int whole, part;  // stretch form: the item's every KV tile is in this CTA's stretch; else where its sums go
 };
+
+// Stretch form (ST): no work list. Rows of a query tile are (token, head) pairs of Gp = 2^lg heads of one KV
+// head's group (the largest power of two in the group), so short chunks fill tiles: a slot holds 128 / Gp tokens, an item two
+// slots of consecutive tokens. All (sequence, KV head, head pack, item, KV tile) in this order form one list; every CTA takes
+// an equal stretch of it, whatever the lengths. An item counts kFaLead more places than it has KV tiles, in front of them, for
+// what its Q load, first scores and epilogue cost. An item that crosses a border leaves unnormalised sums per CTA, joined by
+// prefill_join_kernel. plan: int64 [B + 1], list position of each sequence's first KV tile, then the list's length.
+constexpr int kFaLead = 3;
+struct FaStretch {
+  const long long* plan;
+  float* part_o;   // [grid, 2 (an item before, behind the first border), 2 slots, 128, HD]
+  float* part_ml;  // [grid, 2, 2, 128, 2]
+  int* splits;     // [grid, 8]: the item that leaves CTA c's stretch at its end
+  int B, lg;
+};
+
+// KV tiles of item pr of a sequence.
+GOLLEK_DEVICE void fa_range(int pr, int tok2, int qlen, int L, int window, int& lo, int& hi) {
+  const int ctx0 = L - qlen;
+  hi = (max(0, min(L, ctx0 + min(qlen, (pr + 1) * tok2))) + kTK - 1) / kTK;
+  lo = min(hi, window > 0 ? max(0, ctx0 + pr * tok2 - window + 1) / kTK : 0);
+}
+// CTAs that take part: none has an empty stretch.
+GOLLEK_DEVICE int fa_grid(long long total) { return (int)min((long long)gridDim.x, total); }
 
 // Item of round r0 / gridDim.x for this CTA: rounds alternate direction over the heaviest-first list
 // (CTA c takes the c-th item of even rounds and the c-th from the end of odd ones), which evens out
@@ -458,19 +483,129 @@ GOLLEK_DEVICE FaItem fa_item(const int4* __restrict__ work, int w, const int* __
   return it;
 }
 
+// A CTA's way through its items: the work list in rounds, or (ST) its stretch.
+struct FaStart {
+  int b, x, pr, at;  // at: places of the item that lie before the stretch
+  long long count, first;
+};
+template <bool ST>
+struct FaWalk {
+  int r0 = 0;                 // work list
+  FaStart at;                 // stretch: next item's place, its first KV tile here, KV tiles left
+  bool fresh = true;          // the stretch has not left its first item
+  GOLLEK_DEVICE bool next(FaItem& it, const int4* work, int nwork, const FaStretch& sp, const int* seq_lens,
+                          const int* query_start, const int* block_tables, int bt_stride, int H, int Hk, int window) {
+    if constexpr (!ST) {
+      for (; r0 < nwork; r0 += gridDim.x) {
+        const int w = fa_snake(r0, nwork);
+        if (w < 0) continue;
+        it = fa_item(work, w, seq_lens, query_start, block_tables, bt_stride, H, Hk, window);
+        r0 += gridDim.x;
+        return true;
+      }
+      return false;
+    } else {
+      const int tok2 = 2 * (kTQ >> sp.lg), G = H / Hk, packs = G >> sp.lg;
+      int qlen, L, lo, hi, j0, j1;
+      for (;;) {
+        if (at.count <= 0) return false;
+        while (query_start[at.b + 1] <= query_start[at.b]) ++at.b;  // sequences without new tokens
+        it.b = at.b;
+        it.qs = query_start[at.b];
+        qlen = query_start[at.b + 1] - it.qs, L = seq_lens[at.b];
+        fa_range(at.pr, tok2, qlen, L, window, lo, hi);
+        if (hi > lo && at.at + at.count > kFaLead) break;
+        if (hi > lo) {  // only places in front of the item's first KV tile are left: it is the next CTA's
+          at.count = 0;
+          return false;
+        }
+        next_place(tok2, qlen, Hk * packs);
+      }
+      it.ctx0 = L - qlen;
+      it.kh = at.x / packs;
+      j0 = lo + max(0, at.at - kFaLead);
+      j1 = (int)min((long long)hi, lo + at.at + at.count - kFaLead);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        FaSlot& t = it.sl[i];
+        t.h = it.kh * G + (at.x - it.kh * packs << sp.lg);
+        t.q_off = at.pr * tok2 + i * (tok2 >> 1);
+        t.rows = min(tok2 >> 1, max(0, qlen - t.q_off));  // tokens
+        t.kv_end = t.rows > 0 ? min(L, it.ctx0 + t.q_off + t.rows) : 0;
+        t.a = t.rows > 0 && window > 0 ? max(0, it.ctx0 + t.q_off - window + 1) / kTK : 0;
+        t.b = t.rows > 0 ? (t.kv_end + kTK - 1) / kTK : 0;
+        t.a = max(t.a, j0);
+        t.b = min(t.b, j1);
+        if (t.b <= t.a) t.a = t.b = 0;
+      }
+      it.jlo = j0;
+      it.jhi = j1;
+      it.kv_end = max(it.sl[0].kv_end, it.sl[1].kv_end);
+      it.bt = block_tables + (int64_t)at.b * bt_stride;
+      it.whole = j0 == lo && j1 == hi;
+      it.part = blockIdx.x * 2 + (fresh ? 0 : 1);
+      at.count -= (j1 - lo + kFaLead) - at.at;
+      at.at = 0;
+      fresh = false;
+      if (j1 == hi) next_place(tok2, qlen, Hk * packs);
+      return true;
+    }
+  }
+  GOLLEK_DEVICE void next_place(int tok2, int qlen, int X) {
+    if (++at.pr * tok2 < qlen) return;
+    at.pr = 0;
+    if (++at.x == X) at.x = 0, ++at.b;
+  }
+};
+
+// Where CTA blockIdx.x's stretch begins (one thread).
+GOLLEK_DEVICE FaStart fa_start(const FaStretch& sp, const int* seq_lens, const int* query_start, int H, int Hk, int window) {
+  const int tok2 = 2 * (kTQ >> sp.lg), X = Hk * (H / Hk >> sp.lg);
+  const long long total = sp.plan[sp.B];
+  FaStart s;
+  const int grid = fa_grid(total);
+  s.b = s.x = s.pr = s.at = 0;
+  s.first = s.count = 0;
+  if ((int)blockIdx.x >= grid) return s;
+  s.first = total * blockIdx.x / grid;
+  s.count = total * (blockIdx.x + 1) / grid - s.first;
+  int lo = 0, hi = sp.B;  // the last sequence that begins at or before it
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sp.plan[mid] <= s.first) lo = mid; else hi = mid;
+  }
+  s.b = lo;
+  const long long mine = (sp.plan[lo + 1] - sp.plan[lo]) / X;
+  s.x = (int)((s.first - sp.plan[lo]) / mine);
+  long long left = (s.first - sp.plan[lo]) - s.x * mine;
+  const int qlen = query_start[lo + 1] - query_start[lo], L = seq_lens[lo];
+  for (; s.pr * tok2 < qlen; ++s.pr) {
+    int a, b;
+    fa_range(s.pr, tok2, qlen, L, window, a, b);
+    const int n = b > a ? b - a + kFaLead : 0;
+    if (left < n) {
+      s.at = (int)left;
+      return s;
+    }
+    left -= n;
+  }
+  s.count = 0;  // not reached: the plan counts the same tiles
+  return s;
+}
+
 // Persistent: each CTA runs one item per round of gridDim.x items (fa_snake order; the list is sorted
 // heaviest first). Across
 // items the KV ring, the S / P barriers and the Q buffer keep running counters, so the next item's Q
 // and first KV tiles load, and its first S MMAs run, while the softmax warps still normalise and store
 // the previous item's O: q_empty (committed after an item's last S MMA) frees the Q buffer, o_free[i]
 // (the slot's four softmax warps, after reading O_i) lets the next item's first PV overwrite O_i.
-template <int EMU, int HD>
+template <int EMU, int HD, bool ST>
 __global__ void __launch_bounds__(kFaThreads, 1)
     prefill_fa_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
                       __nv_bfloat16* __restrict__ out, int64_t out_stride, const int* __restrict__ block_tables,
                       int bt_stride, const int* __restrict__ seq_lens, const int* __restrict__ query_start,
                       const int4* __restrict__ work, int nwork, int H, int Hk, float scale_log2,
-                      uint32_t* status, int window, float softcap_log2, int num_blocks) {
+                      uint32_t* status, int window, float softcap_log2, int num_blocks, const FaStretch sp) {
   // head size HD (64 or 128): Q / K / V tiles are HD / 64 boxes of 64 dims (128-byte swizzle), each
   // box 128 rows x 128 bytes
   constexpr int QB = kTQ * HD * 2, KVT = kTK * HD * 2, NBOX = HD / 64;
@@ -492,9 +627,11 @@ __global__ void __launch_bounds__(kFaThreads, 1)
   uint64_t* o_free = bars + 15;                // [slot]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ FaStart start;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (ST && threadIdx.x == 32) start = fa_start(sp, seq_lens, query_start, H, Hk, window);
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
@@ -519,6 +656,12 @@ __global__ void __launch_bounds__(kFaThreads, 1)
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  FaWalk<ST> walk;
+  if constexpr (ST) walk.at = start;
+  FaItem it;
+  auto next_item = [&]() {
+    return walk.next(it, work, nwork, sp, seq_lens, query_start, block_tables, bt_stride, H, Hk, window);
+  };
 
   if (warp == 8) {
     if (elect_one()) {
@@ -526,10 +669,7 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       prefetch_tmap(&tmKV);
       int g = 0, nq = 0;  // KV tiles and Q loads issued so far
       bool ok = true;
-      for (int r0 = 0; r0 < nwork && ok; r0 += gridDim.x) {
-        const int w = fa_snake(r0, nwork);
-        if (w < 0) continue;
-        const FaItem it = fa_item(work, w, seq_lens, query_start, block_tables, bt_stride, H, Hk, window);
+      while (ok && next_item()) {
         if (it.jhi <= it.jlo) continue;
         // the previous item's S MMAs have read its Q tiles
         if (nq > 0 && !waitq(q_empty, (nq - 1) & 1, status, abort_flag)) {
@@ -544,7 +684,10 @@ __global__ void __launch_bounds__(kFaThreads, 1)
             const int qrow = it.qs + it.sl[i].q_off;
 #pragma unroll
             for (int bx = 0; bx < NBOX; ++bx)
-              tma_load_2d(sQ + i * QB + bx * BOXQ, &tmQ, it.sl[i].h * HD + 64 * bx, qrow, q_full);
+              if constexpr (ST)
+                tma_load_3d(sQ + i * QB + bx * BOXQ, &tmQ, 64 * bx, it.sl[i].h, qrow, q_full);
+              else
+                tma_load_2d(sQ + i * QB + bx * BOXQ, &tmQ, it.sl[i].h * HD + 64 * bx, qrow, q_full);
           }
         }
         ++nq;
@@ -590,10 +733,7 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       int np[2] = {0, 0};  // P tiles consumed per slot
       int no[2] = {0, 0};  // items finished per slot (O handed to the epilogue)
       bool ok = true;
-      for (int r0 = 0; r0 < nwork && ok; r0 += gridDim.x) {
-        const int w = fa_snake(r0, nwork);
-        if (w < 0) continue;
-        const FaItem it = fa_item(work, w, seq_lens, query_start, block_tables, bt_stride, H, Hk, window);
+      while (ok && next_item()) {
         if (it.jhi <= it.jlo) continue;
         if (!waitq(q_full, nq & 1, status, abort_flag)) {
           ok = false;
@@ -677,15 +817,21 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     const float inv_cap = capped ? 1.f / softcap_log2 : 0.f;
     bool ok = true;
     int ns = 0, no = 0;  // S tiles and items of this slot so far
-    for (int r0 = 0; r0 < nwork && ok; r0 += gridDim.x) {
-        const int w = fa_snake(r0, nwork);
-        if (w < 0) continue;
-      const FaItem it = fa_item(work, w, seq_lens, query_start, block_tables, bt_stride, H, Hk, window);
+    while (ok && next_item()) {
       const FaSlot t = i == 0 ? it.sl[0] : it.sl[1];
+      if constexpr (ST) {
+        const int64_t slot = ((int64_t)it.part * 2 + i) * kTQ + r;
+        if (!it.whole && t.b <= t.a) *reinterpret_cast<float2*>(sp.part_ml + slot * 2) = make_float2(-INFINITY, 0.f);
+        if (threadIdx.x == 0 && !it.whole && walk.at.count <= 0) {  // this item goes on behind the stretch
+          int* d = sp.splits + blockIdx.x * 8;
+          d[0] = it.b, d[1] = it.sl[0].h, d[2] = it.sl[0].q_off, d[3] = it.part, d[4] = it.jhi, d[5] = it.jlo;
+        }
+      }
       if (it.jhi <= it.jlo || t.b <= t.a) continue;
       const int ctx0 = it.ctx0;
-      const int qpos = ctx0 + t.q_off + r;
-      const int qmin = ctx0 + t.q_off + lg * 32, qmax = qmin + 31;
+      const int tlg = ST ? sp.lg : 0;  // rows are (token, head) pairs
+      const int qpos = ctx0 + t.q_off + (r >> tlg);
+      const int qmin = ctx0 + t.q_off + (lg * 32 >> tlg), qmax = ctx0 + t.q_off + (lg * 32 + 31 >> tlg);
       float m = -INFINITY, l = 0.f;
       int n = 0;
       for (int j = t.a; j < t.b; ++j, ++n) {
@@ -694,6 +840,10 @@ __global__ void __launch_bounds__(kFaThreads, 1)
           break;
         }
         ++ns;
+        if (ST && (lg * 32 >> tlg) >= t.rows) {  // no query in these 32 rows: whatever S holds is taken as P, and never stored
+          if (lane == 0) mbar_arrive(&p_full[i]);
+          continue;
+        }
         tcgen05_fence_after();
         const int k0 = j * kTK;
         // visible keys of row qpos: [qpos - window + 1, min(qpos, kv_end - 1)] - k0
@@ -811,7 +961,8 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       ++no;
       tcgen05_fence_after();
       const float inv = l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* dst = out + (int64_t)(it.qs + t.q_off + r) * out_stride + t.h * HD;
+      __nv_bfloat16* dst = out + (int64_t)(it.qs + t.q_off + (r >> tlg)) * out_stride +
+                           (t.h + (ST ? r & ((1 << tlg) - 1) : 0)) * HD;
       uint32_t u[HD];
 #pragma unroll
       for (int c = 0; c < HD; c += 32) tmem_ld_32x32b_x32(tO + c, u + c);
@@ -820,7 +971,17 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[i]);
-      if (r < t.rows) {
+      if constexpr (ST) {
+        if (!it.whole) {
+          const int64_t slot = ((int64_t)it.part * 2 + i) * kTQ + r;
+          *reinterpret_cast<float2*>(sp.part_ml + slot * 2) = make_float2(m, l);
+#pragma unroll
+          for (int e = 0; e < HD; e += 4)
+            *reinterpret_cast<uint4*>(sp.part_o + slot * HD + e) = make_uint4(u[e], u[e + 1], u[e + 2], u[e + 3]);
+          continue;
+        }
+      }
+      if ((r >> tlg) < t.rows) {
 #pragma unroll
         for (int e = 0; e < HD; e += 8) {
           float f[8];
@@ -838,6 +999,110 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     tcgen05_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Joins the items that cross borders of the stretches: CTA (c, i, z): rows [32 z, 32 z + 32) of slot i, four a warp, of the item that
+// begins in CTA c's stretch and goes on behind it. Its first part is c's, the others are the first parts of the CTAs that follow.
+template <int HD>
+__global__ void __launch_bounds__(256)
+    prefill_join_kernel(const FaStretch sp, __nv_bfloat16* __restrict__ out, int64_t out_stride, const int* __restrict__ seq_lens,
+                        const int* __restrict__ query_start, int Hk, int H, int window) {
+  const long long total = sp.plan[sp.B];
+  const int c = blockIdx.x, i = blockIdx.y, grid = fa_grid(total);
+  if (c >= grid - 1) return;  // nothing goes on behind the last stretch
+  const long long end = total * (c + 1) / grid;
+  const int* d = sp.splits + c * 8;
+  const int b = d[0], h0 = d[1], q_off0 = d[2], part0 = d[3], jend = d[4], jfirst = d[5];
+  if (b < 0) return;  // the stretch ends between items
+  const int tok = kTQ >> sp.lg;
+  const int qs = query_start[b], qlen = query_start[b + 1] - qs, L = seq_lens[b];
+  int lo, hi;
+  fa_range(q_off0 / (2 * tok), 2 * tok, qlen, L, window, lo, hi);
+  if (jfirst != lo) return;  // it began in an earlier stretch: joined there
+  // CTAs that share the item: until its last KV tile
+  const long long last = end + (hi - jend) - 1;
+  int n = 2;
+  while (c + n <= grid - 1 && total * (c + n) / grid <= last) ++n;
+  auto slot_of = [&](int k) {
+    const int part = k == 0 ? part0 : (c + k) * 2;
+    return ((int64_t)part * 2 + i) * kTQ;
+  };
+  const int q_off = q_off0 + i * tok;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int N = 4;  // rows of a warp: their loads are in flight together
+  const int r0 = blockIdx.z * 32 + warp * N;
+  if (q_off + (r0 >> sp.lg) >= qlen) return;
+  const float2* ml = reinterpret_cast<const float2*>(sp.part_ml);
+  float M[N], sum[N], acc[N][HD / 32];
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    M[x] = -INFINITY, sum[x] = 0.f;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) acc[x][e] = 0.f;
+  }
+  for (int k = 0; k < n; ++k)
+#pragma unroll
+    for (int x = 0; x < N; ++x) M[x] = fmaxf(M[x], ml[slot_of(k) + r0 + x].x);
+  for (int k = 0; k < n; ++k)
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      const int64_t slot = slot_of(k) + r0 + x;
+      const float2 y = ml[slot];
+      // a row that sees no key of a part has no sums there: its output is not read
+      const float f = y.x == -INFINITY ? 0.f : exp2f(y.x - M[x]);
+      sum[x] += f * y.y;
+#pragma unroll
+      for (int e = 0; e < HD / 32; ++e) {
+        const float o = sp.part_o[slot * HD + lane + 32 * e];
+        acc[x][e] += y.x == -INFINITY ? 0.f : f * o;
+      }
+    }
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+    const int r = r0 + x;
+    if (q_off + (r >> sp.lg) >= qlen) break;
+    const float inv = sum[x] > 0.f ? 1.f / sum[x] : 0.f;
+    __nv_bfloat16* dst = out + (int64_t)(qs + q_off + (r >> sp.lg)) * out_stride + (h0 + (r & ((1 << sp.lg) - 1))) * HD;
+#pragma unroll
+    for (int e = 0; e < HD / 32; ++e) dst[lane + 32 * e] = __float2bfloat16(acc[x][e] * inv);
+  }
+}
+
+// List positions of the sequences (one CTA): KV tiles of all their items, heads included, summed in order.
+__global__ void __launch_bounds__(256)
+    prefill_plan_kernel(long long* __restrict__ plan, int* __restrict__ splits, int grid, const int* __restrict__ seq_lens,
+                        const int* __restrict__ query_start, int B, int lg, int X, int window) {
+  __shared__ long long sums[8];
+  for (int i = threadIdx.x; i < grid; i += 256) splits[i * 8] = -1;
+  const int tok2 = 2 * (kTQ >> lg), per = (B + 255) / 256;
+  const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
+  long long mine = 0;
+  auto tiles = [&](int b) {
+    const int qlen = query_start[b + 1] - query_start[b], L = seq_lens[b];
+    long long n = 0;
+    for (int pr = 0; pr * tok2 < qlen; ++pr) {
+      int lo, hi;
+      fa_range(pr, tok2, qlen, L, window, lo, hi);
+      n += hi > lo ? hi - lo + kFaLead : 0;
+    }
+    return n * X;
+  };
+  for (int b = b0; b < b1; ++b) mine += tiles(b);
+  long long at = mine;  // inclusive sum over the warp, then over the warps before
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, at, o);
+    if ((int)(threadIdx.x & 31) >= o) at += y;
+  }
+  if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = at;
+  __syncthreads();
+  at -= mine;
+  for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) at += sums[w];
+  for (int b = b0; b < b1; ++b) {
+    plan[b] = at;
+    at += tiles(b);
+  }
+  if (threadIdx.x == 255) plan[B] = at;
 }
 
 }  // namespace
@@ -887,12 +1152,12 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
   auto* w4 = reinterpret_cast<const int4*>(work);
 #define GOLLEK_FA_LAUNCH(E, HDV)                                                                                   \
   do {                                                                                                             \
-    GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(prefill_fa_kernel<E, HDV>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
-                                           fa_smem(HDV)));                                                         \
-    prefill_fa_kernel<E, HDV><<<grid, kFaThreads, fa_smem(HDV), s>>>(tq, tkv, o, out_stride, block_tables,         \
+    GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(prefill_fa_kernel<E, HDV, false>,                                      \
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, fa_smem(HDV)));            \
+    prefill_fa_kernel<E, HDV, false><<<grid, kFaThreads, fa_smem(HDV), s>>>(tq, tkv, o, out_stride, block_tables,  \
                                                                      bt_stride, seq_lens, query_start, w4, nwork,  \
                                                                      H, Hk, sl2, bounds_status(), window, cap,     \
-                                                                     num_blocks);                                  \
+                                                                     num_blocks, FaStretch{});                     \
   } while (0)
   if (head_dim == 64) {
     if (emu == 2)
@@ -911,6 +1176,59 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
   }
 #undef GOLLEK_FA_LAUNCH
   check_launch("paged_prefill_attention (tcgen05, two-tile)");
+}
+
+// The stretch form over a bf16 cache of 16-token blocks. Workspace (bytes): plan, splits, parts.
+static int pack_log2(int G) {  // heads of a group in one query tile: the largest power of two in the group, at most 8
+  int lg = 0;
+  while (lg < 3 && G % (2 << lg) == 0) ++lg;
+  return lg;
+}
+int64_t prefill_stretch_bytes(int B, int head_dim) {
+  const int64_t grid = num_sms();
+  return (((int64_t)B + 1) * 8 + grid * 32 + 255) / 256 * 256 + grid * 4 * kTQ * ((int64_t)head_dim + 2) * 4;
+}
+
+void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
+                            int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
+                            int B, int H, int Hk, float scale, int window, float softcap, int head_dim, void* workspace,
+                            cudaStream_t s) {
+  throw_if(H % Hk != 0, "H must be a multiple of Hk");
+  throw_if(q_stride % 8 != 0, "prefill: q row pitch must keep 16-byte alignment");
+  throw_if(head_dim != 64 && head_dim != 128, "tcgen05 prefill: head_dim 64 or 128");
+  if (q_rows == 0 || B == 0) return;
+  const int grid = num_sms(), G = H / Hk;
+  FaStretch sp;
+  sp.B = B;
+  sp.lg = pack_log2(G);
+  auto* w8 = reinterpret_cast<uint8_t*>(workspace);
+  auto* plan = reinterpret_cast<long long*>(w8);
+  sp.plan = plan;
+  sp.splits = reinterpret_cast<int*>(w8 + ((int64_t)B + 1) * 8);
+  sp.part_o = reinterpret_cast<float*>(w8 + (((int64_t)B + 1) * 8 + (int64_t)grid * 32 + 255) / 256 * 256);
+  sp.part_ml = sp.part_o + (int64_t)grid * 4 * kTQ * head_dim;
+  prefill_plan_kernel<<<1, 256, 0, s>>>(plan, sp.splits, grid, seq_lens, query_start, B, sp.lg, Hk * (G >> sp.lg), window);
+  check_launch("prefill_plan");
+  const uint64_t kv_rows = (uint64_t)num_blocks * 2 * Hk * kBS;
+  CUtensorMap tq = make_tmap_3d(q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, head_dim, H, q_rows, head_dim, q_stride, 64, 1 << sp.lg,
+                                kTQ >> sp.lg, CU_TENSOR_MAP_SWIZZLE_128B);
+  CUtensorMap tkv = make_tmap_2d(cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kv_rows, head_dim, head_dim, kBS, 64,
+                                 CU_TENSOR_MAP_SWIZZLE_128B);
+  const float sl2 = scale * 1.4426950408889634f, cap = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
+  auto* o = reinterpret_cast<__nv_bfloat16*>(out);
+  auto go = [&](auto kern) {
+    GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fa_smem(head_dim)));
+    kern<<<grid, kFaThreads, fa_smem(head_dim), s>>>(tq, tkv, o, out_stride, block_tables, bt_stride, seq_lens, query_start,
+                                                     nullptr, 0, H, Hk, sl2, bounds_status(), window, cap, num_blocks, sp);
+  };
+  if (head_dim == 64) go(prefill_fa_kernel<1, 64, true>);
+  else go(prefill_fa_kernel<1, 128, true>);
+  check_launch("paged_prefill_attention (tcgen05, stretches)");
+  if (head_dim == 64)
+    prefill_join_kernel<64><<<dim3(grid, 2, kTQ / 32), 256, 0, s>>>(sp, o, out_stride, seq_lens, query_start, Hk, H, window);
+  else
+    prefill_join_kernel<128><<<dim3(grid, 2, kTQ / 32), 256, 0, s>>>(sp, o, out_stride, seq_lens, query_start, Hk, H, window);
+  check_launch("prefill_join");
 }
 
 }  // namespace gollek

@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(256)
     kv_dequant_scaled_kernel(const uint8_t* __restrict__ cache, const float* __restrict__ scales,
                              const int* __restrict__ tables, int64_t bt_stride, const int* __restrict__ lens, int mb16,
                              int num_blocks, int Hk, int D, int bs_log2, __nv_bfloat16* __restrict__ dst,
-                             uint32_t* bounds) {
+                             int* __restrict__ ids, uint32_t* bounds) {
   const int r = blockIdx.y, i = blockIdx.x;             // table row, 16-token block of the row
+  if (ids != nullptr && threadIdx.x == 0) ids[(int64_t)r * mb16 + i] = r * mb16 + i;
   const int L = lens ? min(max(lens[r], 0), mb16 << 4) : mb16 << 4;
   const int tok0 = i << 4;
   if (tok0 >= ((L + 127) & ~127)) return;
@@ -1414,7 +1415,7 @@ void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, 
 
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
                               const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
-                              void* dst, cudaStream_t s) {
+                              void* dst, cudaStream_t s, int* ids) {
   throw_if(D % 16 != 0, "block-scaled KV cache: head_dim must be a multiple of 16");
   const int lb = log2_block(bs);
   throw_if(rows > 65535, "kv_dequant_blocks: at most 65535 sequences");
@@ -1422,7 +1423,7 @@ void launch_kv_dequant_scaled(const void* cache, const float* scales, const int*
   auto k = e4m3 ? kv_dequant_scaled_kernel<true> : kv_dequant_scaled_kernel<false>;
   const int mb16 = mb << (lb - 4);
   k<<<dim3(mb16, rows), 256, 0, s>>>(reinterpret_cast<const uint8_t*>(cache), scales, tables, bt_stride, lens, mb16,
-                                     num_blocks, Hk, D, lb, reinterpret_cast<__nv_bfloat16*>(dst), bounds_status());
+                                     num_blocks, Hk, D, lb, reinterpret_cast<__nv_bfloat16*>(dst), ids, bounds_status());
   check_launch("kv_dequant_blocks");
 }
 

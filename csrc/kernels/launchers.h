@@ -59,6 +59,13 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
                              const void* cache, int num_blocks, const int* block_tables, int bt_stride,
                              const int* seq_lens, const int* query_start, const int* work, int nwork, int H, int Hk,
                              float scale, int window, float softcap, int emu, cudaStream_t s, int head_dim = 128);
+// Without a work list: heads of a group packed into the rows of a query tile, KV tiles of all queries shared evenly by
+// the CTAs (bf16 cache of 16-token blocks, head_dim 64 or 128). workspace: prefill_stretch_bytes, 256-byte aligned.
+int64_t prefill_stretch_bytes(int B, int head_dim);
+void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
+                            int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
+                            int B, int H, int Hk, float scale, int window, float softcap, int head_dim, void* workspace,
+                            cudaStream_t s);
 void launch_paged_prefill(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* cache,
                           const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
                           const int* tiles, int ntiles, int H, int Hk, int D, int block_size, float scale,
@@ -252,7 +259,7 @@ void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, 
                             cudaStream_t s);
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
                               const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
-                              void* dst, cudaStream_t s);
+                              void* dst, cudaStream_t s, int* ids = nullptr);  // ids: the copy's block table, if wanted
 // Decode attention over it: a grid of CTAs that share the batch's steps evenly, and the fp32 workspace (counts of
 // floats, in this order) for what they share.
 struct Block8Plan {

@@ -414,6 +414,53 @@ def test_prefill_gpu(kind, D, G, bs, window):
         assert bool((err <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all()), (b, float((err / absv).max()))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D,G,bs,window,softcap", [(64, 4, 16, 0, 0.0), (128, 8, 16, 0, 0.0), (128, 7, 32, 300, 0.0),
+                                                   (64, 12, 16, 129, 20.0), (64, 1, 64, 1, 0.0), (128, 2, 16, 0, 5.0)])
+def test_prefill_long_prefixes_gpu(kind, D, G, bs, window, softcap):
+    """Items that several CTAs share, sequences without new tokens, more CTAs than tiles; sampled rows."""
+    for lens, new in (([2000, 5, 3100, 64, 700], [50, 0, 1, 0, 700]), ([40, 129], [3, 129]), ([6000], [90])):
+        cache, scales, _, bt, sl = filled(kind, lens, 1, D, bs, 61)
+        cache, scales = cache[0], scales[0]
+        qs = torch.tensor([0] + new).cumsum(0).int()
+        g = torch.Generator().manual_seed(7)
+        wide = (torch.randn(int(qs[-1]), G * D + 64, generator=g) * 0.5).bfloat16().cuda()
+        q = wide[:, :G * D].view(-1, G, D)                                        # rows of a wider projection
+        scale = 1 / math.sqrt(D)
+        got = ops.paged_prefill_attention(q, cache.cuda(), bt.cuda(), sl.cuda(), qs.cuda(), scale, window=window,
+                                          softcap=softcap, kv_scales=scales.cuda()).double().cpu()
+        for b, n in enumerate(new):
+            rows = sorted({0, n - 1, n // 2, *torch.randint(0, max(n, 1), (6,), generator=g).tolist()}) if n else []
+            for r in rows:
+                at = lens[b] - n + r + 1
+                out, _, absv, _ = attend(q[qs[b] + r: qs[b] + r + 1].cpu(), cache, scales, bt[b:b + 1],
+                                         torch.tensor([at]), scale, window, softcap)
+                err = (got[qs[b] + r] - out[0]).abs()
+                # p in bf16 (half a step 2^-8), and the cap's tanh in hardware (2^-11 relative, on a score of at most the cap)
+                tol = 2.0 ** -8 * out[0].abs() + (2.0 ** -7 + 2 * softcap * 2.0 ** -11) * absv[0]
+                assert bool((err <= tol).all()), (lens, b, r, float((err / tol).max()))
+
+
+@pytest.mark.gpu
+def test_prefill_captured_gpu():
+    """A captured step replayed with other lengths and chunk borders."""
+    lens, new = [300, 50, 210], [100, 50, 3]
+    cache, scales, _, bt, sl = filled("int8", lens, 2, 64, 16, 67)
+    c, s, t = cache[0].cuda(), scales[0].cuda(), bt.cuda()
+    qs = torch.tensor([0] + new).cumsum(0).int().cuda()
+    q = torch.randn(int(qs[-1]), 8, 64, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    lg, qg = torch.tensor([160, 40, 200], dtype=torch.int32).cuda(), torch.tensor([0, 40, 80, 153], dtype=torch.int32).cuda()
+    ops.paged_prefill_attention(q, c, t, lg, qg, 0.1, kv_scales=s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.paged_prefill_attention(q, c, t, lg, qg, 0.1, kv_scales=s)
+    lg.copy_(sl.cuda())
+    qg.copy_(qs)
+    g.replay()
+    assert torch.equal(out, ops.paged_prefill_attention(q, c, t, sl.cuda(), qs, 0.1, kv_scales=s))
+
+
 def test_gather_cpu_behind_the_end():
     cache, scales, _, bt, lens = filled("e4m3", [5, 70], 2, 32, 32, 23)
     tmp, table = ops.kv_dequant_blocks(cache[0], scales[0], bt, lens)
