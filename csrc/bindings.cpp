@@ -871,26 +871,28 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
   return out;
 }
 
-void kv_evict_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor mass, torch::Tensor tables,
-                 torch::Tensor lens, torch::Tensor keep, torch::Tensor kept, int64_t sink, int64_t recent) {
-  const bool e4m3 = check_block8(cache, scales, true);
-  float* mp = check_mass(mass, cache, 1);
+// cache [(layers,) NB, 2, Hk, bs, D]; returns kept int32 [(layers,) B, Hk, max_keep]
+torch::Tensor kv_evict_py(torch::Tensor cache, torch::Tensor scales, torch::Tensor mass, torch::Tensor tables,
+                          torch::Tensor lens, torch::Tensor keep, int64_t sink, int64_t recent, int64_t max_keep) {
+  const int o = cache.dim() == 6 ? 1 : 0;
+  const bool e4m3 = check_block8(cache, scales, o == 1);
+  float* mp = check_mass(mass, cache, o);
   check_i32(keep, "keep_lens");
-  check_i32(kept, "kept");
   check_same_device(keep, cache);
-  check_same_device(kept, cache);
-  const int64_t B = tables.size(0);
+  const int64_t B = tables.size(0), Hk = cache.size(2 + o), layers = o ? cache.size(0) : 1;
   check_rows(tables, lens, cache, B);
   TORCH_CHECK(keep.dim() == 1 && keep.is_contiguous() && keep.numel() >= B, "keep_lens [B]");
   TORCH_CHECK(sink >= 0 && recent >= 0 && sink <= INT32_MAX && recent <= INT32_MAX, "kv_evict: sink and recent are token counts >= 0");
-  TORCH_CHECK(kept.is_contiguous() && kept.dim() == 4 && kept.size(0) == cache.size(0) && kept.size(1) == B &&
-                  kept.size(2) == cache.size(3),
-              "kept int32 [layers, B, Hk, max_keep]");
+  TORCH_CHECK(max_keep >= 0 && max_keep <= INT32_MAX - 65536, "kv_evict: max_keep must be >= 0");
   c10::cuda::CUDAGuard guard(cache.device());
+  std::vector<int64_t> shape = {B, Hk, max_keep};
+  if (o) shape.insert(shape.begin(), layers);
+  auto kept = torch::empty(shape, keep.options());
   launch_kv_evict(cache.data_ptr(), scales.data_ptr<float>(), mp, tables.data_ptr<int>(), tables.stride(0),
-                  tables.size(1), lens.data_ptr<int>(), keep.data_ptr<int>(), kept.data_ptr<int>(), cache.size(0), B,
-                  cache.size(3), cache.size(5), cache.size(4), (int)cache.size(1), (int)sink, (int)recent,
-                  (int)kept.size(3), e4m3, cur_stream());
+                  tables.size(1), lens.data_ptr<int>(), keep.data_ptr<int>(), kept.data_ptr<int>(), layers, B, Hk,
+                  cache.size(4 + o), cache.size(3 + o), (int)cache.size(o), (int)sink, (int)recent, (int)max_keep, e4m3,
+                  cur_stream());
+  return kept;
 }
 
 // Grouped (per-expert) GEMM: out = a · b_g^T per M tile (tile_group names g); epi 0 none, 2 SwiGLU,

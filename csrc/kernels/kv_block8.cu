@@ -12,6 +12,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../common/common.cuh"
 #include "../common/tma_host.h"
@@ -1077,6 +1078,7 @@ __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const Evic
   extern __shared__ uint32_t keys[];
   __shared__ uint32_t hist[2048], warp_sums[kSelThreads / 32], found[2];
   __shared__ uint2 counts[kSelThreads / 32];
+  asm volatile("griddepcontrol.launch_dependents;");
   const int h = blockIdx.x, b = blockIdx.y, ly = blockIdx.z;
   const EvictRow r = evict_row(p, b);
   int* kept = p.kept + (((int64_t)ly * p.B + b) * p.Hk + h) * p.max_keep;
@@ -1266,6 +1268,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
   // largest magnitude of each destination block of a chunk (float bits): one being filled, one read, one cleared
   __shared__ uint32_t top[3][64];
   const int h = blockIdx.x / 3, w = blockIdx.x % 3, b = blockIdx.y, ly = blockIdx.z;  // w: K, V, masses
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the choice is still being made
   const EvictRow r = evict_row(p, b);
   if (!r.cut || r.K == 0) return;
   if (w == 2) {
@@ -1379,6 +1382,33 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
     }
   }
   cp_async_wait<0>();
+}
+
+// Raises a kernel's shared-memory limit once per device (the attribute lasts as long as the context).
+template <auto Kernel>
+void max_smem_once(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  GOLLEK_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && ((done.load(std::memory_order_relaxed) >> dev) & 1)) return;
+  GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+}
+
+// Launch whose CTAs start as the kernel before it leaves (it waits for that one's results itself).
+template <class... P, class... A>
+void launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 int log2_block(int bs) {
@@ -1498,12 +1528,12 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   const int mass_tiles = mass ? ((mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
   const int64_t join = ((int64_t)B * H + 1) / 2 + (int64_t)B * Hk * mass_tiles;
   throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
-  auto go = [&](auto kern, int threads, int smem) {
-    GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    kern<<<(unsigned)plan.grid, threads, smem, s>>>(p);
-  };
-#define GOLLEK_B8_M(DD, NN, E, M) \
-  go(block8_decode_kernel<DD, NN, E, M>, DecShape<DD, NN>::kThreads, DecShape<DD, NN>::kSmem)
+#define GOLLEK_B8_M(DD, NN, E, M)                                                                          \
+  do {                                                                                                     \
+    using S = DecShape<DD, NN>;                                                                            \
+    max_smem_once<block8_decode_kernel<DD, NN, E, M>>(S::kSmem);                                           \
+    block8_decode_kernel<DD, NN, E, M><<<(unsigned)plan.grid, S::kThreads, S::kSmem, s>>>(p);              \
+  } while (0)
 #define GOLLEK_B8_N(DD, NN)                             \
   if (e4m3) {                                           \
     if (mass) GOLLEK_B8_M(DD, NN, true, true);          \
@@ -1525,21 +1555,12 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
 #undef GOLLEK_B8_N
 #undef GOLLEK_B8_M
   check_launch("block8_decode");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)join);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;  // its CTAs start as the decode kernel's leave
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   auto join_kernel = block8_join_kernel<0>;
   if (mass && p.G == 1) join_kernel = block8_join_kernel<1>;
   if (mass && p.G == 2) join_kernel = block8_join_kernel<2>;
   if (mass && p.G == 4) join_kernel = block8_join_kernel<4>;
   if (mass && p.G == 8) join_kernel = block8_join_kernel<8>;
-  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, join_kernel, p, D, 8 * plan.nt, mass_tiles));
+  launch_after(join_kernel, dim3((unsigned)join), kJoinThreads, 0, s, p, D, 8 * plan.nt, mass_tiles);
 }
 
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
@@ -1562,15 +1583,24 @@ void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables,
   p.sink = sink, p.recent = recent, p.max_keep = max_keep;
   p.bounds = bounds_status();
   const int smem = (int)std::min<int64_t>((int64_t)mb << p.bs_log2, kSelKeys) * 4;
-  GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kv_evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4));
+  max_smem_once<kv_evict_select_kernel>(kSelKeys * 4);
   kv_evict_select_kernel<<<dim3(Hk, B, layers), kSelThreads, smem, s>>>(p);
   check_launch("kv_evict_select");
   if (max_keep == 0) return;
-  auto k = D % 64 == 0 ? (e4m3 ? kv_evict_move_kernel<true, 4> : kv_evict_move_kernel<false, 4>)
-                       : (e4m3 ? kv_evict_move_kernel<true, 2> : kv_evict_move_kernel<false, 2>);
-  GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMoveSmem));
-  k<<<dim3(3 * Hk, B, layers), kMoveThreads, kMoveSmem, s>>>(p);
-  check_launch("kv_evict_move");
+  const dim3 grid(3 * Hk, B, layers);
+#define GOLLEK_MOVE(E, NP)                                                                      \
+  do {                                                                                          \
+    max_smem_once<kv_evict_move_kernel<E, NP>>(kMoveSmem);                                      \
+    launch_after(kv_evict_move_kernel<E, NP>, grid, kMoveThreads, kMoveSmem, s, p);             \
+  } while (0)
+  if (D % 64 == 0) {
+    if (e4m3) GOLLEK_MOVE(true, 4);
+    else GOLLEK_MOVE(false, 4);
+  } else {
+    if (e4m3) GOLLEK_MOVE(true, 2);
+    else GOLLEK_MOVE(false, 2);
+  }
+#undef GOLLEK_MOVE
 }
 
 }  // namespace gollek

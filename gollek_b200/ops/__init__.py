@@ -315,20 +315,16 @@ def kv_evict(cache: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor, bloc
     bs]. Returns the kept tokens' former places, int32 [(layers,) B, Hk, max_keep], padded with -1;
     ``max_keep`` (default: the table's width in tokens) must be at least the largest K below its L: a larger
     one is cut to it."""
-    bs = cache.shape[-2]
-    one = cache.dim() == 5
     if max_keep is None:
-        max_keep = block_tables.shape[1] * bs
+        max_keep = block_tables.shape[1] * cache.shape[-2]
+    if cache.is_cuda:
+        return _C(2).kv_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, sink, recent, max_keep)
     if max_keep < 0:
         raise ValueError("kv_evict: max_keep must be >= 0")
+    one = cache.dim() == 5
     if one:
         cache, scales, mass = cache.unsqueeze(0), scales.unsqueeze(0), mass.unsqueeze(0)
-    if not cache.is_cuda:
-        kept = ref.block8_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, sink, recent, max_keep)
-    else:
-        kept = torch.empty(cache.shape[0], block_tables.shape[0], cache.shape[3], max_keep, dtype=torch.int32,
-                           device=cache.device)
-        _C(2 if max_keep else 1).kv_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, kept, int(sink), int(recent))
+    kept = ref.block8_evict(cache, scales, mass, block_tables, seq_lens, keep_lens, sink, recent, max_keep)
     return kept[0] if one else kept
 
 
