@@ -973,6 +973,26 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
   const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2), lo = p.window > 0 ? max(0, L - p.window) : 0;
   const int first = (i - bk * mass_tiles) * kMassTokens;
   if (first >= L || first + kMassTokens <= lo) return;
+  const float* sc = p.scores + (int64_t)bk * (p.mb << p.bs_log2) * p.G;
+  const int* bt = p.tables + (int64_t)b * p.bt_stride;
+  float* mass = p.mass + (kh << p.bs_log2);
+  const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
+  constexpr int GN = GV > 0 ? GV : 1, N = kMassTokens / kJoinThreads;
+  // the tokens' scores and blocks are on their way while the heads' sums are joined
+  float v[N][GN];
+  int id[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int t = first + threadIdx.x + k * kJoinThreads;
+    id[k] = t >= lo && t < L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
+    if (GV > 0 && id[k] >= 0) {
+      if constexpr (GV == 1) v[k][0] = sc[t];
+      if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
+      if constexpr (GV >= 4)
+#pragma unroll
+        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[(t * GV + h) / 4];
+    }
+  }
   for (int h = warp; h < p.G; h += kJoinThreads / 32) {
     const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
     const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
@@ -980,31 +1000,21 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
     if (lane == 0) sm[h] = ml.x + log2f(ml.y);
   }
   __syncthreads();
-  const float* sc = p.scores + (int64_t)bk * (p.mb << p.bs_log2) * p.G;
-  const int* bt = p.tables + (int64_t)b * p.bt_stride;
-  float* mass = p.mass + (kh << p.bs_log2);
-  const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
-  constexpr int GN = GV > 0 ? GV : 1;
   float lse[GN];
 #pragma unroll
   for (int h = 0; h < GN; ++h) lse[h] = sm[h];
-#pragma unroll 4
-  for (int t = max(first, lo) + threadIdx.x; t < min(first + kMassTokens, L); t += kJoinThreads) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (id[k] < 0) continue;
+    const int t = first + threadIdx.x + k * kJoinThreads;
     float w = 0.f;
     if constexpr (GV > 0) {
-      float v[GN];
-      if constexpr (GV == 1) v[0] = sc[t];
-      if constexpr (GV == 2) *reinterpret_cast<float2*>(v) = reinterpret_cast<const float2*>(sc)[t];
-      if constexpr (GV >= 4)
 #pragma unroll
-        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v + h) = reinterpret_cast<const float4*>(sc)[(t * GV + h) / 4];
-#pragma unroll
-      for (int h = 0; h < GN; ++h) w += ex2(v[h] - lse[h]);
+      for (int h = 0; h < GN; ++h) w += ex2(v[k][h] - lse[h]);
     } else {
       for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
     }
-    const int id = checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
-    atomicAdd(mass + (int64_t)id * row + (t & mask), w);
+    atomicAdd(mass + (int64_t)id[k] * row + (t & mask), w);
   }
 }
 
@@ -1264,6 +1274,7 @@ GOLLEK_DEVICE void move_masses(const EvictArgs& p, const EvictRow& r, int h, int
 template <bool E4M3, int NP>
 __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const EvictArgs p) {
   constexpr int NI = kMovePieces / NP;  // tokens per thread and chunk
+  static_assert(NI <= 2, "a stage has room for two scales a thread");
   extern __shared__ __align__(16) uint8_t ring[];
   // largest magnitude of each destination block of a chunk (float bits): one being filled, one read, one cleared
   __shared__ uint32_t top[3][64];
