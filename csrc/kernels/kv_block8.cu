@@ -384,7 +384,8 @@ struct DecArgs {
   float* part_o;       // [grid, 2, HB, D]: sums of a stretch's first and last sequence, where it is shared
   float* part_ml;      // [grid, 2, HB, 2]: their reference (log2) and sum of probabilities
   float* row_ml;       // [B * H, 2]: reference and sum of the sequences that one CTA finished (mass)
-  int* spans;          // [B * Hk * NG, 2]: first part and number of parts of each head tile (1: finished)
+  int* splits;         // [grid, 4]: the head tile that leaves a CTA's stretch at its end: row (-1: none), tile, first part, parts
+  int* spans;          // [B * Hk * NG, 2]: first part and number of parts of each head tile (1: finished) (mass)
   float* scores;       // [B * Hk, mb * bs, G] log2 scores (mass)
   float* mass;
   int64_t q_stride, bt_stride;
@@ -513,19 +514,34 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
   const uint32_t ring = smem_u32(dsm), psm = ring + S::kStages * S::kStage;
 
   asm volatile("griddepcontrol.launch_dependents;");
-  // this CTA's stretch of the list: every warp sums the rows' steps, then finds the row it starts in
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) total += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? dec_row(p, b0 + lane, T).n : 0);
-  total *= X;
+  if (threadIdx.x == 0) p.splits[blockIdx.x * 4] = -1;
+  // rows without tokens are shared out too
+  for (int b = blockIdx.x; b < p.B; b += p.grid)
+    if (p.lens[b] <= 0 || p.mb == 0)
+      for (int i = threadIdx.x; i < p.H * D / 2; i += S::kThreads) reinterpret_cast<uint32_t*>(p.out + (int64_t)b * p.H * D)[i] = 0u;
+  // this CTA's stretch of the list: every lane sums the steps of an equal range of rows; then the range, and in it the row,
+  // that the stretch begins in
+  const int per = (p.B + 31) / 32, r0 = min(p.B, lane * per), r1 = min(p.B, r0 + per);
+  int64_t mine = 0;
+#pragma unroll 8
+  for (int i = r0; i < r1; ++i) mine += dec_row(p, i, T).n;
+  int64_t upto = mine * X;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
   const int grid = stretch_grid(p, total);
   if ((int)blockIdx.x >= grid) return;
   const int64_t first = stretch_begin(blockIdx.x, total, grid);
   const int count = (int)(stretch_begin(blockIdx.x + 1, total, grid) - first);
   DecPlace at;  // of the next step to issue
   {
-    int64_t before = 0;
+    const int range = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
+    int64_t before = __shfl_sync(0xffffffffu, upto - mine * X, range);
     at.b = 0;
-    for (int b0 = 0;; b0 += 32) {
+    for (int b0 = range * per;; b0 += 32) {
       const int n = b0 + lane < p.B ? dec_row(p, b0 + lane, T).n : 0;
       int sum = n;
 #pragma unroll
@@ -898,8 +914,11 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
       }
     if (begun && threadIdx.x == 0) {  // the CTA that holds the first step says how many parts there are
       int parts = 1;
-      if (!last) parts = (int)(stretch_of(first + j - step + cur.r.n - 1, total, grid) - blockIdx.x) + 1;
-      *reinterpret_cast<int2*>(p.spans + ((int64_t)b * X + kh * p.NG + cur.hg) * 2) = make_int2((int)part, parts);
+      if (!last) {
+        parts = (int)(stretch_of(first + j - step + cur.r.n - 1, total, grid) - blockIdx.x) + 1;
+        *reinterpret_cast<int4*>(p.splits + blockIdx.x * 4) = make_int4(b, kh * p.NG + cur.hg, (int)part, parts);
+      }
+      if (MASS) *reinterpret_cast<int2*>(p.spans + ((int64_t)b * X + kh * p.NG + cur.hg) * 2) = make_int2((int)part, parts);
     }
     if (last) next_head(cur, p, T);
   }
@@ -926,8 +945,8 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
   return make_float2(M, warp_sum(sum));
 }
 
-// Joins the parts of the head tiles that several CTAs shared, and zeroes empty rows: the first ceil(B * H / 2) CTAs, half a
-// CTA per (row, head); the others add the softmax weights of kMassTokens tokens of a (row, kv head) to mass, summed over the
+// Joins the parts of the head tiles that several CTAs shared: CTA c < grid the one that leaves the decode kernel's
+// CTA c; the others add the softmax weights of kMassTokens tokens of a (row, kv head) to mass, summed over the
 // head group in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
 // share a block.
 constexpr int kJoinThreads = 256, kMassTokens = 1024;
@@ -935,40 +954,62 @@ constexpr int kJoinThreads = 256, kMassTokens = 1024;
 template <int GV>  // heads per KV head where they are 1, 2, 4 or 8, else 0
 __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB, int mass_tiles) {
   __shared__ float sm[128];
+  __shared__ float4 others[kJoinThreads];
+  __shared__ float2 others_ml[kJoinThreads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
-  const int joins = (p.B * p.H + 1) >> 1;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
-  if ((int)blockIdx.x < joins) {
-    const int row = blockIdx.x * 2 + (threadIdx.x >> 7), d0 = threadIdx.x & 127;
-    if (row >= p.B * p.H) return;
-    const int b = row / p.H, h = row - b * p.H;
-    const int kh = h / p.G, hx = h - kh * p.G, x = kh * p.NG + hx / HB, hh = hx % HB;
-    const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + x];
-    const int L = min(p.lens[b], p.mb << p.bs_log2);
-    __nv_bfloat16* out = p.out + (int64_t)row * D;
-    if (L <= 0) {
-      for (int i = d0; i < D; i += 128) out[i] = __float2bfloat16(0.f);
-      return;
-    }
-    const int n = span.y;
-    if (n == 1) return;
-    const float2 all = join_ml(p, span.x, n, HB, hh);  // every warp for itself
-    const float inv = all.y > 0.f ? 1.f / all.y : 0.f;
-    float acc[2] = {0.f, 0.f};  // D <= 256
+  if ((int)blockIdx.x < p.grid) {
+    const int4 sp = *reinterpret_cast<const int4*>(p.splits + blockIdx.x * 4);  // row, head tile, first part, parts
+    if (sp.x < 0) return;
+    const int kh = sp.y / p.NG, h0 = (sp.y - kh * p.NG) * HB, nh = min(p.G - h0, HB);
+    // a thread takes four dims of a head; where they leave threads over, those share the parts
+    const int quads = nh * D / 4, groups = max(1, kJoinThreads / quads);
+    __nv_bfloat16* out = p.out + ((int64_t)sp.x * p.H + kh * p.G + h0) * D;
+    for (int q0 = 0; q0 < quads; q0 += kJoinThreads) {
+      const int gr = threadIdx.x / quads, q = q0 + (groups > 1 ? threadIdx.x % quads : threadIdx.x);
+      float M = -INFINITY, sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (q < quads && (groups == 1 || gr < groups)) {
+        const int hh = q * 4 / D;
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const int64_t k = part_slot(span.x, i) * HB + hh;
-      const float m = p.part_ml[k * 2], f = m == -INFINITY ? 0.f : ex2(m - all.x);
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (d0 + 128 * e < D) acc[e] += f * p.part_o[k * D + d0 + 128 * e];
+        for (int i = groups > 1 ? gr : 0; i < sp.w; i += groups) {
+          const int64_t k = part_slot(sp.z, i) * HB + hh;
+          const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[k];
+          const float4 o = *reinterpret_cast<const float4*>(p.part_o + k * D + (q * 4 - hh * D));
+          const float m = fmaxf(M, ml.x), d0 = m == -INFINITY ? 0.f : M - m, d1 = m == -INFINITY ? 0.f : ml.x - m;
+          const float f0 = ex2(d0), f1 = ex2(d1);
+          M = m;
+          sum = shift_sum(sum, d0) + shift_sum(ml.y, d1);
+          acc.x = f0 * acc.x + f1 * o.x;
+          acc.y = f0 * acc.y + f1 * o.y;
+          acc.z = f0 * acc.z + f1 * o.z;
+          acc.w = f0 * acc.w + f1 * o.w;
+        }
+      }
+      if (groups > 1) {
+        if (gr > 0 && gr < groups) others[threadIdx.x] = acc, others_ml[threadIdx.x] = make_float2(M, sum);
+        __syncthreads();
+        if (gr > 0) return;
+        for (int g = 1; g < groups; ++g) {
+          const float4 o = others[threadIdx.x + g * quads];
+          const float2 ml = others_ml[threadIdx.x + g * quads];
+          const float m = fmaxf(M, ml.x), d0 = m == -INFINITY ? 0.f : M - m, d1 = m == -INFINITY ? 0.f : ml.x - m;
+          const float f0 = ex2(d0), f1 = ex2(d1);
+          M = m;
+          sum = shift_sum(sum, d0) + shift_sum(ml.y, d1);
+          acc.x = f0 * acc.x + f1 * o.x;
+          acc.y = f0 * acc.y + f1 * o.y;
+          acc.z = f0 * acc.z + f1 * o.z;
+          acc.w = f0 * acc.w + f1 * o.w;
+        }
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      if (q < quads)
+        *reinterpret_cast<uint2*>(out + q * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (d0 + 128 * e < D) out[d0 + 128 * e] = __float2bfloat16(acc[e] * inv);
     return;
   }
-  const int i = blockIdx.x - joins;
+  const int i = blockIdx.x - p.grid;
   const int bk = i / mass_tiles, b = bk / p.Hk, kh = bk - b * p.Hk;
   const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2), lo = p.window > 0 ? max(0, L - p.window) : 0;
   const int first = (i - bk * mass_tiles) * kMassTokens;
@@ -990,7 +1031,7 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
       if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
       if constexpr (GV >= 4)
 #pragma unroll
-        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[(t * GV + h) / 4];
+        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[((int64_t)t * GV + h) / 4];
     }
   }
   for (int h = warp; h < p.G; h += kJoinThreads / 32) {
@@ -1485,7 +1526,7 @@ Block8Plan plan_for(int B, int H, int Hk, int64_t width, int splits, bool mass) 
   p.n_o = (int64_t)p.grid * 2 * HB * D;
   p.n_ml = (int64_t)p.grid * 2 * HB * 2;
   p.n_row = mass ? (int64_t)B * H * 2 : 0;
-  p.n_span = tiles * 2;
+  p.n_span = (int64_t)p.grid * 4 + (mass ? tiles * 2 : 0);
   p.n_scores = mass ? (int64_t)B * H * width : 0;  // a multiple of 16, like n_o and n_ml
   return p;
 }
@@ -1524,8 +1565,9 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
   p.part_o = workspace;
   p.part_ml = p.part_o + plan.n_o;
-  p.scores = p.part_ml + plan.n_ml;
+  p.scores = p.part_ml + plan.n_ml + (int64_t)plan.grid * 4;  // behind the splits: every section a multiple of 16 bytes
   p.row_ml = p.scores + plan.n_scores;
+  p.splits = reinterpret_cast<int*>(p.part_ml + plan.n_ml);
   p.spans = reinterpret_cast<int*>(p.row_ml + plan.n_row);
   p.mass = mass;
   p.q_stride = q_stride;
@@ -1537,7 +1579,7 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
   const int mass_tiles = mass ? ((mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
-  const int64_t join = ((int64_t)B * H + 1) / 2 + (int64_t)B * Hk * mass_tiles;
+  const int64_t join = plan.grid + (int64_t)B * Hk * mass_tiles;
   throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
 #define GOLLEK_B8_M(DD, NN, E, M)                                                                          \
   do {                                                                                                     \

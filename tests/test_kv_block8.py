@@ -287,6 +287,41 @@ def test_decode_window_and_cap_gpu(kind, window, softcap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [33, 100, 1100])
+def test_decode_many_rows_gpu(B):
+    """More rows than lanes (and than lanes of lanes), a third of them empty, tables wider than any row."""
+    g = torch.Generator().manual_seed(B)
+    lens = (torch.randint(-20, 60, (B,), generator=g).clamp(min=0)).tolist()
+    cache, scales, mass, bt, sl = filled("int8", lens, 1, 32, 16, B)
+    bt = torch.nn.functional.pad(bt, (0, 70))
+    q = torch.randn(B, 4, 32, generator=g).bfloat16()
+    m = mass[0].cuda()
+    got = ops.paged_decode_attention(q.cuda(), cache[0].cuda(), bt.cuda(), sl.cuda(), 0.2, num_splits=0,
+                                     kv_scales=scales[0].cuda(), mass=m)
+    out, w, absv, big = attend(q, cache[0], scales[0], bt, sl, 0.2)
+    check_out(got, out, absv)
+    check_mass(m, mass[0], w, bt, sl, 16, 32, big)
+    assert not bool(got[sl.cuda() == 0].any())
+
+
+@pytest.mark.gpu
+def test_no_rows_and_no_blocks_gpu():
+    cache, scales = torch.zeros(3, 2, 2, 16, 64, dtype=torch.int8, device="cuda"), torch.ones(3, 2, 2, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    out = ops.paged_decode_attention(q[:0], cache, torch.zeros(0, 4, **i32), torch.zeros(0, **i32), 1.0, num_splits=0, kv_scales=scales)
+    assert out.shape == (0, 4, 64)
+    out = ops.paged_decode_attention(q, cache, torch.zeros(2, 0, **i32), torch.ones(2, **i32), 1.0, num_splits=0, kv_scales=scales)
+    assert not bool(out.any())
+    kept = ops.kv_evict(cache, scales, torch.zeros(3, 2, 16, device="cuda"), torch.zeros(0, 4, **i32), torch.zeros(0, **i32),
+                        torch.zeros(0, **i32), 1, 1, max_keep=3)
+    assert kept.shape == (0, 2, 3)
+    out = ops.paged_prefill_attention(q[:0], cache, torch.zeros(1, 2, **i32), torch.zeros(1, **i32), torch.zeros(2, **i32), 1.0,
+                                      kv_scales=scales)
+    assert out.shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
 def test_decode_uneven_scales_gpu(kind):
     """Value scales 2^-100 .. 2^90 apart from block to block, a dominant token in a block of tiny values, all-zero
