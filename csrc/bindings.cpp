@@ -791,6 +791,7 @@ torch::Tensor block8_decode_py(torch::Tensor q, torch::Tensor cache, torch::Tens
   const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = cache.size(2);
   TORCH_CHECK(splits >= 0 && splits <= 64, "block-scaled decode attention: 0 (automatic) to 64 splits");
   TORCH_CHECK(B <= INT32_MAX / 1024, "block-scaled decode attention: too many rows");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX && softcap >= 0, "window and softcap must be >= 0");
   check_rows(tables, lens, cache, B);
   float* mp = check_mass(mass, cache, 0);
   c10::cuda::CUDAGuard guard(cache.device());
@@ -833,6 +834,7 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
   TORCH_CHECK(q.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               "q: rows at multiples of 16 bytes");
   TORCH_CHECK(Hk > 0 && H % Hk == 0, "H must be a multiple of Hk");
+  TORCH_CHECK(window >= 0 && window <= INT32_MAX && softcap >= 0, "window and softcap must be >= 0");
   TORCH_CHECK(query_start.dim() == 1 && query_start.is_contiguous() && query_start.numel() >= 1, "query_start [B + 1]");
   const int64_t B = query_start.numel() - 1;
   check_rows(tables, lens, cache, B);
@@ -867,7 +869,7 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
   auto ws = torch::empty({prefill_stretch_bytes((int)B, (int)D)}, q.options().dtype(at::kByte));
   launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
                          ids.data_ptr<int>(), (int)mb16, lens.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H,
-                         (int)Hk, (float)scale, (int)window, (float)softcap, (int)D, ws.data_ptr(), cur_stream());
+                         (int)Hk, (float)scale, (int)window, (float)softcap, (int)emu, (int)D, ws.data_ptr(), cur_stream());
   return out;
 }
 

@@ -1191,8 +1191,8 @@ int64_t prefill_stretch_bytes(int B, int head_dim) {
 
 void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
                             int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
-                            int B, int H, int Hk, float scale, int window, float softcap, int head_dim, void* workspace,
-                            cudaStream_t s) {
+                            int B, int H, int Hk, float scale, int window, float softcap, int emu, int head_dim,
+                            void* workspace, cudaStream_t s) {
   throw_if(H % Hk != 0, "H must be a multiple of Hk");
   throw_if(q_stride % 8 != 0, "prefill: q row pitch must keep 16-byte alignment");
   throw_if(head_dim != 64 && head_dim != 128, "tcgen05 prefill: head_dim 64 or 128");
@@ -1221,8 +1221,15 @@ void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_
     kern<<<grid, kFaThreads, fa_smem(head_dim), s>>>(tq, tkv, o, out_stride, block_tables, bt_stride, seq_lens, query_start,
                                                      nullptr, 0, H, Hk, sl2, bounds_status(), window, cap, num_blocks, sp);
   };
-  if (head_dim == 64) go(prefill_fa_kernel<1, 64, true>);
-  else go(prefill_fa_kernel<1, 128, true>);
+  if (head_dim == 64) {
+    if (emu == 2) go(prefill_fa_kernel<2, 64, true>);
+    else if (emu == 1) go(prefill_fa_kernel<1, 64, true>);
+    else go(prefill_fa_kernel<0, 64, true>);
+  } else {
+    if (emu == 2) go(prefill_fa_kernel<2, 128, true>);
+    else if (emu == 1) go(prefill_fa_kernel<1, 128, true>);
+    else go(prefill_fa_kernel<0, 128, true>);
+  }
   check_launch("paged_prefill_attention (tcgen05, stretches)");
   if (head_dim == 64)
     prefill_join_kernel<64><<<dim3(grid, 2, kTQ / 32), 256, 0, s>>>(sp, o, out_stride, seq_lens, query_start, Hk, H, window);

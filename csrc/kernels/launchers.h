@@ -64,8 +64,8 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
 int64_t prefill_stretch_bytes(int B, int head_dim);
 void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
                             int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
-                            int B, int H, int Hk, float scale, int window, float softcap, int head_dim, void* workspace,
-                            cudaStream_t s);
+                            int B, int H, int Hk, float scale, int window, float softcap, int emu, int head_dim,
+                            void* workspace, cudaStream_t s);
 void launch_paged_prefill(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* cache,
                           const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
                           const int* tiles, int ntiles, int H, int Hk, int D, int block_size, float scale,

@@ -219,6 +219,8 @@ def block8_decode(q: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor, bl
     Hk, bs = cache.shape[2], cache.shape[3]
     if H % Hk or D != cache.shape[4]:
         raise ValueError("q must be [B, H, D] with H a multiple of Hk and the cache's D")
+    if window < 0 or softcap < 0:
+        raise ValueError("window and softcap must be >= 0")
     out = torch.zeros_like(q)
     for b in range(B):
         L = min(max(int(seq_lens[b]), 0), block_tables.shape[1] * bs)

@@ -667,6 +667,8 @@ def refusals(dev):
     no(dec, q, cache, bt, lens, 1.0, kv_scales=scales, mass=mass.half())
     no(dec, q, torch.zeros(8, 2, 2, 16, 64, dtype=dt, device=dev), bt, lens, 1.0, mass=mass)   # weights of a bf16 cache
     no(dec, q, cache[:, :, :, :8].contiguous(), bt, lens, 1.0, kv_scales=scales)    # blocks of 8 tokens
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales, window=-1)
+    no(dec, q, cache, bt, lens, 1.0, kv_scales=scales, softcap=-1.0)
     no(wr, kv[..., :32].contiguous(), slots, cache, scales)
     no(wr, kv, slots[:1], cache, scales)
     no(wr, kv, slots, cache.float(), scales)
