@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "../common/common.cuh"
 #include "../common/tma_host.h"
@@ -338,10 +339,14 @@ __global__ void __launch_bounds__(256)
 // A step: warp w (of W) takes the scores of its 16 tokens, S^T = K Q^T, then all warps exchange the
 // probabilities in shared memory and warp w takes dims [w D / W, (w + 1) D / W) of O^T = V^T P^T over all T
 // tokens, so O is never reduced across warps. Heads are the N = 8 columns of mma.m16n8k16, tokens and
-// dims its 16 rows: a group of up to 8 heads wastes no row. Codes turn into f16 inside the fragments, exactly:
-//   K: a lane's four consecutive bytes of a 16-byte chunk are two k-pairs of a k16 step. Any order of dims will
-//      do as long as Q follows it, so Q is gathered in that order once per sequence.
-//   V: ldmatrix.trans moves byte pairs; a byte permute splits them into the fragments of the even and the odd dims.
+// dims its 16 rows: a group of up to 8 heads wastes no row.
+//   K, int8: the codes are the operand as they lie (m16n8k32 s8). Q is written to 2^-22 of its head's largest value as
+//      three signed digits to the base 256, whose products add up in 32-bit integers. Against codes turned into f16:
+//      16 rows of 32k, 64 heads: 174 us, not 193, where the power cap holds the clock.
+//   K, e4m3: a lane's four consecutive bytes of a 16-byte chunk become two f16 k-pairs, exactly. Any order of dims will
+//      do as long as Q follows it, so Q is gathered in that order once per sequence. (Two e4m3 planes of Q would do for
+//      the codes as they lie, but 64 rows of up to 4k took 65.6 us with them, not 61.4.)
+//   V: ldmatrix.trans moves byte pairs; a byte permute splits them into f16 fragments (exact) of the even and the odd dims.
 // Scores get the key scale, probabilities the value scale. The running reference m of the softmax
 // covers score + exponent of the value scale, so p * scale fits f16 whatever the scales; the sum l
 // uses p alone. m only moves when a score passes it by 2^8: the vote rides on the barrier that the
@@ -433,6 +438,12 @@ GOLLEK_DEVICE void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+GOLLEK_DEVICE void mma_s8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 GOLLEK_DEVICE float ex2(float x) {
@@ -657,7 +668,8 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
 #pragma unroll
   for (int j = 0; j < S::kStages - 1; ++j) issue();
 
-  uint32_t qf[NT][CH][2];
+  constexpr int PL = E4M3 ? 2 : 3;  // registers of Q a chunk of 16 dims: two f16 pairs, or three digits
+  uint32_t qf[NT][CH][PL];
   float qmul[NT][2];
   float o[OWN][NT][4];
   float m[NT][2], l[NT][2];
@@ -673,13 +685,12 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
     const int tok0 = cur.r.t0 + cur.s * T;
     if (cur.s == 0 || j == 0) {
       begun = cur.s == 0;
-      // Q^T as the B operand, columns = heads: chunk i of the lane's head, dims 16 i + 4 c + {0, 1} and
-      // + {2, 3}. Each head is brought to an amax in [2^11, 2^12) by a power of two: f16 then holds every
-      // bf16 within 2^-28 of it exactly.
+      // Q^T as the B operand, columns = heads: dims 16 i + 4 c + {0 .. 3} of the lane's head. A power of two brings the
+      // head's amax to [2^11, 2^12), where f16 holds every bf16 within 2^-28 of it exactly, or to [2^21, 2^22).
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         uint2 raw[CH];
-        float amax = 0.f;
+        float amax = 0.f, poison = 0.f;  // NaN where the head holds a NaN or an infinity
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           if constexpr (S::kStageQ) {
@@ -696,19 +707,34 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
           const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].x));
           const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].y));
           amax = fmaxf(amax, fmaxf(fmaxf(fabsf(u.x), fabsf(u.y)), fmaxf(fabsf(v.x), fabsf(v.y))));
+          poison = fmaf(u.x, 0.f, fmaf(u.y, 0.f, fmaf(v.x, 0.f, fmaf(v.y, 0.f, poison))));
         }
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -100), 127) - 11;
+        poison += __shfl_xor_sync(0xffffffffu, poison, 1);
+        poison += __shfl_xor_sync(0xffffffffu, poison, 2);
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -90), 127) - (E4M3 ? 11 : 21);
         const float f = __uint_as_float((uint32_t)(127 - e) << 23);
-        const float back = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+        const float back = fmaf(__uint_as_float((uint32_t)(127 + e) << 23), p.scale_log2, poison);
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
           const float2 u = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].x));
           const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[i].y));
-          const __half2 hu = __floats2half2_rn(u.x * f, u.y * f), hv = __floats2half2_rn(v.x * f, v.y * f);
-          qf[nt][i][0] = *reinterpret_cast<const uint32_t*>(&hu);
-          qf[nt][i][1] = *reinterpret_cast<const uint32_t*>(&hv);
+          const float x[4] = {u.x * f, u.y * f, v.x * f, v.y * f};
+          if constexpr (E4M3) {
+            const __half2 hu = __floats2half2_rn(x[0], x[1]), hv = __floats2half2_rn(x[2], x[3]);
+            qf[nt][i][0] = *reinterpret_cast<const uint32_t*>(&hu);
+            qf[nt][i][1] = *reinterpret_cast<const uint32_t*>(&hv);
+          } else {
+            qf[nt][i][0] = qf[nt][i][1] = qf[nt][i][2] = 0u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int q0 = __float2int_rn(x[k]), q1 = (q0 - (int8_t)q0) >> 8, q2 = (q1 - (int8_t)q1) >> 8;
+              qf[nt][i][0] |= (uint32_t)(q0 & 0xff) << (8 * k);
+              qf[nt][i][1] |= (uint32_t)(q1 & 0xff) << (8 * k);
+              qf[nt][i][2] |= (uint32_t)(q2 & 0xff) << (8 * k);
+            }
+          }
         }
         qmul[nt][0] = __shfl_sync(0xffffffffu, back, 8 * c);  // columns 2 c and 2 c + 1
         qmul[nt][1] = __shfl_sync(0xffffffffu, back, 8 * c + 4);
@@ -727,25 +753,41 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
 #pragma unroll
     for (int q = 0; q < TW; ++q) {
       const int tile = tok0 + (warp * TW + q) * 16, tok = tile + g;
-      float s2[NT][4];
+      using Acc = typename std::conditional<E4M3, float, int>::type;
+      Acc acc[NT][PL][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[q][nt][e] = s2[nt][e] = 0.f;
+        for (int e = 0; e < PL * 4; ++e) acc[nt][e / 4][e % 4] = 0;
       const uint32_t kb = st + ((warp * TW + q) * 16 + frow) * S::kRow;
 #pragma unroll
       for (int j2 = 0; j2 < CH / 2; ++j2) {
-        uint32_t r[4], a[4];
+        uint32_t r[4];  // rows 0-7 and 8-15 of chunk 2 j2, then of the next one
         ldsm4(r, kb + ((S::kSwizzle ? (2 * j2) ^ (fhi ^ (frow & 7)) : 2 * j2 + fhi) << 4));
-        expand4<E4M3, false>(r[0], a[0], a[2]);
-        expand4<E4M3, false>(r[1], a[1], a[3]);
+        if constexpr (E4M3) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(s[q][nt], a, qf[nt][2 * j2][0], qf[nt][2 * j2][1]);
-        expand4<E4M3, false>(r[2], a[0], a[2]);
-        expand4<E4M3, false>(r[3], a[1], a[3]);
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a[4];
+            expand4<E4M3, false>(r[2 * i], a[0], a[2]);
+            expand4<E4M3, false>(r[2 * i + 1], a[1], a[3]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(s2[nt], a, qf[nt][2 * j2 + 1][0], qf[nt][2 * j2 + 1][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(acc[nt][i], a, qf[nt][2 * j2 + i][0], qf[nt][2 * j2 + i][1]);
+          }
+        } else {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) mma_s8(acc[nt][pl], r, qf[nt][2 * j2][pl], qf[nt][2 * j2 + 1][pl]);
+        }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if constexpr (E4M3)
+            s[q][nt][e] = acc[nt][0][e] + acc[nt][1][e];
+          else
+            s[q][nt][e] = fmaf((float)acc[nt][PL - 1][e], 65536.f, fmaf((float)acc[nt][1][e], 256.f, (float)acc[nt][0][e]));
       float ks;
       asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs[q]) : "r"(tail + 8 * (warp * TW + q)) : "memory");
       if (tile >= cur.r.L) vs[q] = 0.f;  // no token here: whatever scale was read, the probabilities are 0
@@ -753,7 +795,7 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[q][nt][e] = (s[q][nt][e] + s2[nt][e]) * (ks * qmul[nt][e & 1]);
+        for (int e = 0; e < 4; ++e) s[q][nt][e] *= ks * qmul[nt][e & 1];
       if (p.cap > 0.f) {  // cap * tanh(x / cap) = cap * (1 - 2 / (1 + e^(2 x / cap)))
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)

@@ -287,6 +287,26 @@ def test_decode_window_and_cap_gpu(kind, window, softcap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("D", [64, 128])
+def test_decode_queries_out_of_the_ordinary_gpu(kind, D):
+    """A NaN or an infinity in a head's query spoils that head alone; queries of any size keep their precision."""
+    cache, scales, _, bt, lens = filled(kind, [50, 300, 129], 2, D, 16, 71)
+    q = torch.randn(3, 8, D, generator=torch.Generator().manual_seed(9))
+    q[0, 1, 3], q[0, 6, 5], q[1, 2, 0] = math.nan, math.inf, -math.inf
+    q[2] *= 2.0 ** torch.tensor([-60, -20, -3, 0, 2, 3, -110, -133]).view(8, 1)     # the last two below the smallest kept size
+    q[2, 4, ::2] *= 2.0 ** -12                                                       # a wide spread within a head
+    q = q.bfloat16()
+    got = ops.paged_decode_attention(q.cuda(), cache[0].cuda(), bt.cuda(), lens.cuda(), 0.1, num_splits=0,
+                                     kv_scales=scales[0].cuda())
+    bad = torch.zeros(3, 8, dtype=torch.bool)
+    bad[0, 1] = bad[0, 6] = bad[1, 2] = True
+    assert bool(got.cpu()[bad].isnan().all())
+    out, _, absv, _ = attend(q.nan_to_num(0.0, 0.0, 0.0), cache[0], scales[0], bt, lens, 0.1)
+    check_out(torch.where(bad[..., None].cuda(), out.cuda().float(), got.float()), out, absv)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B", [33, 100, 1100])
 def test_decode_many_rows_gpu(B):
     """More rows than lanes (and than lanes of lanes), a third of them empty, tables wider than any row."""
