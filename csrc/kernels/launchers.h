@@ -257,9 +257,19 @@ void launch_kv_dequant_blocks(const void* cache, const float* scales, const int*
 void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, const int* slots, void* cache,
                             float* scales, float* mass, int T, int Hk, int D, int bs, int num_blocks, bool e4m3,
                             cudaStream_t s);
+// What prompt attention over the copy needs beside it, where ids is given: the copy's block table, the rows' lengths cut to
+// their tables, and zeros in `out` for queries in front of their sequence's first token (more queries than tokens).
+struct PromptRows {
+  int* ids = nullptr;
+  int* lens = nullptr;
+  const int* query_start = nullptr;
+  void* out = nullptr;
+  int64_t out_stride = 0;
+  int width = 0;  // values of an out row
+};
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
                               const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
-                              void* dst, cudaStream_t s, int* ids = nullptr);  // ids: the copy's block table, if wanted
+                              void* dst, cudaStream_t s, const PromptRows& prompt = {});
 // Decode attention over it: a grid of CTAs that share the batch's steps evenly, and the fp32 workspace (counts of
 // floats, in this order) for what they share.
 struct Block8Plan {
