@@ -845,26 +845,31 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
   TORCH_CHECK(out.dim() == 3 && out.stride(2) == 1 && out.stride(1) == D && out.sizes() == q.sizes() &&
                   out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "out must be [T, H, D] like q");
-  const int64_t mb16 = tables.size(1) * cache.size(3) / 16;
-  TORCH_CHECK(B * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: the step's blocks exceed one copy's addresses");
-  auto copy = torch::empty({B * mb16, 2, Hk, 16, D}, q.options());
-  TORCH_CHECK(T == 0 || B == 0 || mb16 > 0, "block_tables: no columns");
-  auto ids = torch::empty({B, mb16}, tables.options());
-  auto cut = torch::empty({B}, lens.options());
-  PromptRows prompt;
-  prompt.ids = ids.data_ptr<int>(), prompt.lens = cut.data_ptr<int>(), prompt.query_start = query_start.data_ptr<int>();
-  prompt.out = out.data_ptr(), prompt.out_stride = out.stride(0), prompt.width = (int)(H * D);
   // Many items (4096 prompt tokens of 32 heads: 512): the work list's whole items balance by themselves, 155 us against
   // 197 us in stretches, whose CTAs leave a quarter more parts. Few (eight chunks of 100 over 6000 cached tokens: 128): stretches
   // fill the GPU and the tiles, 80 us against 104 us.
   const bool list = tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 && tiles->size(0) >= 2 * device_num_sms();
-  launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>(), tables.stride(0),
-                           lens.data_ptr<int>(), B, tables.size(1), (int)cache.size(0), Hk, D, cache.size(3), e4m3,
-                           copy.data_ptr(), cur_stream(), prompt);
+  const int64_t width = tables.size(1) * cache.size(3);
+  const int64_t mb16 = list ? width / 16 : (width + 127) / 128 * 8;
+  TORCH_CHECK(B * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: the step's blocks exceed one copy's addresses");
+  TORCH_CHECK(T == 0 || B == 0 || mb16 > 0, "block_tables: no columns");
+  auto copy = torch::empty({B * mb16, 2, Hk, 16, D}, q.options());
+  auto cut = torch::empty({B}, lens.options());
+  PromptRows prompt;
+  prompt.together = !list, prompt.lens = cut.data_ptr<int>(), prompt.query_start = query_start.data_ptr<int>();
+  prompt.out = out.data_ptr(), prompt.out_stride = out.stride(0), prompt.width = (int)(H * D);
+  auto make_copy = [&]() {
+    launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>(), tables.stride(0),
+                             lens.data_ptr<int>(), B, tables.size(1), (int)cache.size(0), Hk, D, cache.size(3), e4m3,
+                             copy.data_ptr(), cur_stream(), prompt);
+  };
   if (list) {
     check_i32(*tiles, "tiles");
     check_same_device(*tiles, cache);
     TORCH_CHECK(tiles->is_contiguous(), "tiles: contiguous work list");
+    auto ids = torch::empty({B, mb16}, tables.options());
+    prompt.ids = ids.data_ptr<int>();
+    make_copy();
     launch_paged_prefill_fa(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
                             ids.data_ptr<int>(), (int)mb16, cut.data_ptr<int>(), query_start.data_ptr<int>(),
                             tiles->data_ptr<int>(), tiles->size(0), (int)H, (int)Hk, (float)scale, (int)window,
@@ -872,9 +877,12 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
     return out;
   }
   auto ws = torch::empty({prefill_stretch_bytes((int)B, (int)D)}, q.options().dtype(at::kByte));
-  launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
-                         ids.data_ptr<int>(), (int)mb16, cut.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H,
-                         (int)Hk, (float)scale, (int)window, (float)softcap, (int)emu, (int)D, ws.data_ptr(), cur_stream());
+  launch_prefill_plan(lens.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H, (int)Hk, (int)width, (int)window,
+                      (int)D, ws.data_ptr(), cur_stream());
+  make_copy();
+  launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(mb16 * 16),
+                         cut.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H, (int)Hk, (float)scale, (int)window,
+                         (float)softcap, (int)emu, (int)D, ws.data_ptr(), cur_stream());
   return out;
 }
 

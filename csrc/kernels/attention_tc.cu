@@ -377,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // on the FMA pipe instead of MUFU (EMU 1: every 4th column, 2: every 2nd).
 // ---------------------------------------------------------------------------------------------
 constexpr int kFaThreads = 320;
-constexpr int fa_smem(int hd) { return 1024 + 2 * kTQ * hd * 2 + kStages * 2 * kTK * hd * 2 + 256; }
+constexpr int fa_stages_log2(int hd) { return hd == 64 ? 2 : 1; }  // KV tiles in shared memory
+constexpr int fa_smem(int hd) { return 1024 + 2 * kTQ * hd * 2 + (1 << fa_stages_log2(hd)) * 2 * kTK * hd * 2 + 256; }
 
 GOLLEK_DEVICE float ex2_mufu(float x) {
   float y;
@@ -432,7 +433,7 @@ struct FaStretch {
   float* part_o;   // [grid, 2 (an item before, behind the first border), 2 slots, 128, HD]
   float* part_ml;  // [grid, 2, 2, 128, 2]
   int* splits;     // [grid, 8]: the item that leaves CTA c's stretch at its end
-  int B, lg;
+  int B, lg, tokens;  // tokens: of a (sequence, K/V, head) of the copy
 };
 
 // KV tiles of item pr of a sequence.
@@ -544,7 +545,6 @@ struct FaWalk {
       it.jlo = j0;
       it.jhi = j1;
       it.kv_end = max(it.sl[0].kv_end, it.sl[1].kv_end);
-      it.bt = block_tables + (int64_t)at.b * bt_stride;
       it.whole = j0 == lo && j1 == hi;
       it.part = blockIdx.x * 2 + (fresh ? 0 : 1);
       at.count -= (j1 - lo + kFaLead) - at.at;
@@ -613,22 +613,28 @@ __global__ void __launch_bounds__(kFaThreads, 1)
   // box 128 rows x 128 bytes
   constexpr int QB = kTQ * HD * 2, KVT = kTK * HD * 2, NBOX = HD / 64;
   constexpr int BOXQ = kTQ * 64 * 2, BOXK = kTK * 64 * 2;
+  constexpr int LS = fa_stages_log2(HD), KS = 1 << LS, SM = KS - 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* sQ = smem;                          // slot i at + i * QB
   uint8_t* sKV = sQ + 2 * QB;             // stage s: K at + s*2*tile, V at + s*2*tile + tile
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kStages * 2 * KVT);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + KS * 2 * KVT);
   uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;                 // [2]
-  uint64_t* v_full = bars + 3;                 // [2]
-  uint64_t* kv_empty = bars + 5;               // [2]
-  uint64_t* s_full = bars + 7;                 // [slot]
-  uint64_t* p_full = bars + 9;                 // [slot]
-  uint64_t* o_done = bars + 11;                // [slot]
-  uint64_t* done_bar = bars + 13;
-  uint64_t* q_empty = bars + 14;
-  uint64_t* o_free = bars + 15;                // [slot]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  uint64_t* k_full = bars + 1;                 // [stage]
+  uint64_t* v_full = k_full + KS;              // [stage]
+  uint64_t* kv_empty = v_full + KS;            // [stage]
+  uint64_t* s_full = kv_empty + KS;            // [slot][parity of the slot's tile]
+  uint64_t* p_full = s_full + 4;               // the same
+  uint64_t* o_done = p_full + 4;               // [slot]
+  uint64_t* done_bar = o_done + 2;
+  uint64_t* q_empty = done_bar + 1;
+  uint64_t* o_free = q_empty + 1;              // [slot]
+  uint64_t* pv_done = o_free + 2;              // [slot], kAhead only
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
+  // Head size 64 leaves TMEM for a third S buffer: tiles take them in turn, whatever their slot, and a slot's next scores
+  // are computed while its softmax still works on this tile. O_i is then quiescent only after pv_done.
+  constexpr bool kAhead = HD == 64;
+  constexpr int kTmemO = kAhead ? 3 * kTK : 2 * kTK;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ FaStart start;
 
@@ -639,13 +645,18 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_free[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&kv_empty[i], 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&o_done[i], 1);
-      mbar_init(&o_free[i], 4);
     }
     mbar_init(done_bar, 1);
     *abort_flag = 0;
@@ -695,13 +706,24 @@ __global__ void __launch_bounds__(kFaThreads, 1)
         }
         ++nq;
         for (int j = it.jlo; j < it.jhi; ++j, ++g) {
-          const int st = g & 1;
-          if (!waitq(&kv_empty[st], ((g >> 1) & 1) ^ 1, status, abort_flag)) {
+          const int st = g & SM;
+          if (!waitq(&kv_empty[st], ((g >> LS) & 1) ^ 1, status, abort_flag)) {
             ok = false;
             break;
           }
           uint8_t* dk = sKV + st * 2 * KVT;
           uint8_t* dv = dk + KVT;
+          if constexpr (ST) {  // a sequence's tokens of a head lie together
+            const int64_t rk = ((int64_t)it.b * 2 * Hk + it.kh) * sp.tokens + j * kTK;
+            mbar_arrive_expect_tx(&k_full[st], KVT);
+#pragma unroll
+            for (int bx = 0; bx < NBOX; ++bx) tma_load_2d(dk + bx * BOXK, &tmKV, 64 * bx, (int)rk, &k_full[st]);
+            mbar_arrive_expect_tx(&v_full[st], KVT);
+#pragma unroll
+            for (int bx = 0; bx < NBOX; ++bx)
+              tma_load_2d(dv + bx * BOXK, &tmKV, 64 * bx, (int)(rk + (int64_t)Hk * sp.tokens), &v_full[st]);
+            continue;
+          }
           mbar_arrive_expect_tx(&k_full[st], KVT);
           for (int blk = 0; blk < kTK / kBS; ++blk) {
             const int kb = (j * kTK) / kBS + blk;
@@ -722,9 +744,9 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       }
       if (!ok) {  // copies still in flight land before the CTA leaves
         if (nq > 0) drainq(q_full, (nq - 1) & 1);
-        for (int x = max(0, g - 2); x < g; ++x) {
-          drainq(&k_full[x & 1], (x >> 1) & 1);
-          drainq(&v_full[x & 1], (x >> 1) & 1);
+        for (int x = max(0, g - KS); x < g; ++x) {
+          drainq(&k_full[x & SM], (x >> LS) & 1);
+          drainq(&v_full[x & SM], (x >> LS) & 1);
         }
       }
     }
@@ -734,6 +756,9 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       constexpr uint32_t idesc_o = make_idesc_bf16(kTQ, HD) | (1u << 16);  // P (TMEM) V, V MN-major
       int g = 0, nq = 0;
       int np[2] = {0, 0};  // P tiles consumed per slot
+      int ns[2] = {0, 0};  // S tiles issued per slot
+      uint32_t buf[2] = {tmem, tmem + kTK};  // the slot's latest S (then P)
+      uint32_t turn = 0;                     // kAhead: the next tile's S buffer
       int no[2] = {0, 0};  // items finished per slot (O handed to the epilogue)
       bool ok = true;
       while (ok && next_item()) {
@@ -745,7 +770,7 @@ __global__ void __launch_bounds__(kFaThreads, 1)
         for (int j = it.jlo; j <= it.jhi && ok; ++j) {
           const int gi = g + (j - it.jlo);
           const bool prev = j > it.jlo, cur = j < it.jhi;
-          if (prev && !waitq(&v_full[(gi - 1) & 1], ((gi - 1) >> 1) & 1, status, abort_flag)) {
+          if (prev && !waitq(&v_full[(gi - 1) & SM], ((gi - 1) >> LS) & 1, status, abort_flag)) {
             ok = false;
             break;
           }
@@ -754,9 +779,36 @@ __global__ void __launch_bounds__(kFaThreads, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const FaSlot& t = it.sl[i];
-            const uint32_t tS = tmem + i * kTK, tO = tmem + 256 + i * HD;
+            const uint32_t tP = buf[i], tO = tmem + kTmemO + i * HD;
+            auto scores = [&]() {
+              if (!cur || j < t.a || j >= t.b) return true;
+              if (!k_ready) {
+                if (!waitq(&k_full[gi & SM], (gi >> LS) & 1, status, abort_flag)) return false;
+                tcgen05_fence_after();
+                k_ready = true;
+              }
+              if constexpr (kAhead) {
+                buf[i] = tmem + turn * kTK;
+                turn = turn == 2 ? 0 : turn + 1;
+              }
+              const uint32_t q_addr = smem_u32(sQ + i * QB);
+              const uint32_t k_addr = smem_u32(sKV + (gi & SM) * 2 * KVT);
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks) {
+                const uint64_t a = make_smem_desc_sw128(q_addr + (ks >> 2) * (BOXQ) + (ks & 3) * 32);
+                const uint64_t bd = make_smem_desc_sw128(k_addr + (ks >> 2) * (BOXK) + (ks & 3) * 32);
+                umma_f16_ss(buf[i], a, bd, idesc_s, ks > 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[i * 2 + (ns[i] & 1)]);
+              ++ns[i];
+              return true;
+            };
+            if (kAhead && !scores()) {
+              ok = false;
+              break;
+            }
             if (prev && j - 1 >= t.a && j - 1 < t.b) {
-              if (!waitq(&p_full[i], np[i] & 1, status, abort_flag)) {
+              if (!waitq(&p_full[i * 2 + (np[i] & 1)], (np[i] >> 1) & 1, status, abort_flag)) {
                 ok = false;
                 break;
               }
@@ -767,37 +819,23 @@ __global__ void __launch_bounds__(kFaThreads, 1)
                 break;
               }
               tcgen05_fence_after();
-              const uint32_t v_addr = smem_u32(sKV + ((gi - 1) & 1) * 2 * KVT + KVT);
+              const uint32_t v_addr = smem_u32(sKV + ((gi - 1) & SM) * 2 * KVT + KVT);
 #pragma unroll
               for (int ks = 0; ks < kTK / 16; ++ks)
-                umma_f16_ts(tO, tS + ks * 8, make_desc_mn_sw128(v_addr + ks * 2048, BOXK), idesc_o,
+                umma_f16_ts(tO, tP + ks * 8, make_desc_mn_sw128(v_addr + ks * 2048, BOXK), idesc_o,
                             (j - 1 > t.a || ks > 0) ? 1u : 0u);
+              if constexpr (kAhead) umma_commit(&pv_done[i]);
               if (j == t.b) {
                 umma_commit(&o_done[i]);
                 ++no[i];
               }
             }
-            if (cur && j >= t.a && j < t.b) {
-              if (!k_ready) {
-                if (!waitq(&k_full[gi & 1], (gi >> 1) & 1, status, abort_flag)) {
-                  ok = false;
-                  break;
-                }
-                tcgen05_fence_after();
-                k_ready = true;
-              }
-              const uint32_t q_addr = smem_u32(sQ + i * QB);
-              const uint32_t k_addr = smem_u32(sKV + (gi & 1) * 2 * KVT);
-#pragma unroll
-              for (int ks = 0; ks < HD / 16; ++ks) {
-                const uint64_t a = make_smem_desc_sw128(q_addr + (ks >> 2) * (BOXQ) + (ks & 3) * 32);
-                const uint64_t bd = make_smem_desc_sw128(k_addr + (ks >> 2) * (BOXK) + (ks & 3) * 32);
-                umma_f16_ss(tS, a, bd, idesc_s, ks > 0 ? 1u : 0u);
-              }
-              umma_commit(&s_full[i]);
+            if (!kAhead && !scores()) {
+              ok = false;
+              break;
             }
           }
-          if (prev && ok) umma_commit(&kv_empty[(gi - 1) & 1]);
+          if (prev && ok) umma_commit(&kv_empty[(gi - 1) & SM]);
           if (j == it.jhi - 1 && ok) umma_commit(q_empty);  // the item's last S MMAs read Q
         }
         g += it.jhi - it.jlo;
@@ -815,7 +853,9 @@ __global__ void __launch_bounds__(kFaThreads, 1)
     const int i = warp >> 2, lg = warp & 3;
     const int r = lg * 32 + lane;
     const uint32_t lane_off = (uint32_t)(lg * 32) << 16;
-    const uint32_t tS = tmem + i * kTK + lane_off, tO = tmem + 256 + i * HD + lane_off;
+    const uint32_t tO = tmem + kTmemO + i * HD + lane_off;
+    uint32_t tS = tmem + i * kTK + lane_off;
+    uint32_t turn0 = 0;  // kAhead: tiles of both slots before this item
     const bool capped = softcap_log2 > 0.f;
     const float inv_cap = capped ? 1.f / softcap_log2 : 0.f;
     bool ok = true;
@@ -830,6 +870,8 @@ __global__ void __launch_bounds__(kFaThreads, 1)
           d[0] = it.b, d[1] = it.sl[0].h, d[2] = it.sl[0].q_off, d[3] = it.part, d[4] = it.jhi, d[5] = it.jlo;
         }
       }
+      const uint32_t turns = turn0;
+      if (kAhead) turn0 += (it.sl[0].b - it.sl[0].a) + (it.sl[1].b - it.sl[1].a);
       if (it.jhi <= it.jlo || t.b <= t.a) continue;
       const int ctx0 = it.ctx0;
       const int tlg = ST ? sp.lg : 0;  // rows are (token, head) pairs
@@ -838,13 +880,18 @@ __global__ void __launch_bounds__(kFaThreads, 1)
       float m = -INFINITY, l = 0.f;
       int n = 0;
       for (int j = t.a; j < t.b; ++j, ++n) {
-        if (!waitq(&s_full[i], ns & 1, status, abort_flag)) {
+        if (!waitq(&s_full[i * 2 + (ns & 1)], (ns >> 1) & 1, status, abort_flag)) {
           ok = false;
           break;
         }
+        uint64_t* const p_bar = &p_full[i * 2 + (ns & 1)];
         ++ns;
+        if constexpr (kAhead) {  // tiles go slot 0, slot 1 of a KV tile, then the next KV tile's
+          const int x0 = min(j + i, it.sl[0].b) - it.sl[0].a, x1 = min(j, it.sl[1].b) - it.sl[1].a;
+          tS = tmem + (turns + max(x0, 0) + max(x1, 0)) % 3 * kTK + lane_off;
+        }
         if (ST && (lg * 32 >> tlg) >= t.rows) {  // no query in these 32 rows: whatever S holds is taken as P, and never stored
-          if (lane == 0) mbar_arrive(&p_full[i]);
+          if (lane == 0) mbar_arrive(p_bar);
           continue;
         }
         tcgen05_fence_after();
@@ -941,7 +988,14 @@ __global__ void __launch_bounds__(kFaThreads, 1)
         }
         const float psum = (ps[0] + ps[1]) + (ps[2] + ps[3]);
         l = l * corr + psum;
-        if (__any_sync(0xffffffffu, corr != 1.f)) {  // O_i is quiescent: PV_i(j-1) completed before S_i(j)
+        if (__any_sync(0xffffffffu, corr != 1.f)) {  // O_i is quiescent: PV_i(j-1) completed before S_i(j), or is waited for
+          if constexpr (kAhead) {
+            if (!waitq(&pv_done[i], ns & 1, status, abort_flag)) {
+              ok = false;
+              break;
+            }
+            tcgen05_fence_after();
+          }
 #pragma unroll 1
           for (int c = 0; c < HD; c += 32) {
             uint32_t u[32];
@@ -955,7 +1009,7 @@ __global__ void __launch_bounds__(kFaThreads, 1)
         tmem_st_wait();
         tcgen05_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i]);
+        if (lane == 0) mbar_arrive(p_bar);
       }
       if (!ok || !waitq(&o_done[i], no & 1, status, abort_flag)) {
         ok = false;
@@ -1010,6 +1064,7 @@ template <int HD>
 __global__ void __launch_bounds__(256)
     prefill_join_kernel(const FaStretch sp, __nv_bfloat16* __restrict__ out, int64_t out_stride, const int* __restrict__ seq_lens,
                         const int* __restrict__ query_start, int Hk, int H, int window) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched as the attention's CTAs leave
   const long long total = sp.plan[sp.B];
   const int c = blockIdx.x, i = blockIdx.y, grid = fa_grid(total);
   if (c >= grid - 1) return;  // nothing goes on behind the last stretch
@@ -1074,14 +1129,15 @@ __global__ void __launch_bounds__(256)
 // List positions of the sequences (one CTA): KV tiles of all their items, heads included, summed in order.
 __global__ void __launch_bounds__(256)
     prefill_plan_kernel(long long* __restrict__ plan, int* __restrict__ splits, int grid, const int* __restrict__ seq_lens,
-                        const int* __restrict__ query_start, int B, int lg, int X, int window) {
+                        const int* __restrict__ query_start, int B, int lg, int X, int width, int window) {
   __shared__ long long sums[8];
+  asm volatile("griddepcontrol.launch_dependents;");  // the copy is made beside it
   for (int i = threadIdx.x; i < grid; i += 256) splits[i * 8] = -1;
   const int tok2 = 2 * (kTQ >> lg), per = (B + 255) / 256;
   const int b0 = min(B, (int)threadIdx.x * per), b1 = min(B, b0 + per);
   long long mine = 0;
   auto tiles = [&](int b) {
-    const int qlen = query_start[b + 1] - query_start[b], L = seq_lens[b];
+    const int qlen = query_start[b + 1] - query_start[b], L = min(max(seq_lens[b], 0), width);
     long long n = 0;
     for (int pr = 0; pr * tok2 < qlen; ++pr) {
       int lo, hi;
@@ -1181,7 +1237,7 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
   check_launch("paged_prefill_attention (tcgen05, two-tile)");
 }
 
-// The stretch form over a bf16 cache of 16-token blocks. Workspace (bytes): plan, splits, parts.
+// The stretch form. Workspace (bytes): plan, splits, parts.
 static int pack_log2(int G) {  // heads of a group in one query tile: the largest power of two in the group, at most 8
   int lg = 0;
   while (lg < 3 && G % (2 << lg) == 0) ++lg;
@@ -1192,37 +1248,51 @@ int64_t prefill_stretch_bytes(int B, int head_dim) {
   return (((int64_t)B + 1) * 8 + grid * 32 + 255) / 256 * 256 + grid * 4 * kTQ * ((int64_t)head_dim + 2) * 4;
 }
 
-void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
-                            int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
-                            int B, int H, int Hk, float scale, int window, float softcap, int emu, int head_dim,
-                            void* workspace, cudaStream_t s) {
+static FaStretch stretch_of(void* workspace, int B, int G, int head_dim) {
+  const int64_t grid = num_sms();
+  auto* w8 = reinterpret_cast<uint8_t*>(workspace);
+  FaStretch sp = {};
+  sp.B = B;
+  sp.lg = pack_log2(G);
+  sp.plan = reinterpret_cast<long long*>(w8);
+  sp.splits = reinterpret_cast<int*>(w8 + ((int64_t)B + 1) * 8);
+  sp.part_o = reinterpret_cast<float*>(w8 + (((int64_t)B + 1) * 8 + grid * 32 + 255) / 256 * 256);
+  sp.part_ml = sp.part_o + grid * 4 * kTQ * head_dim;
+  return sp;
+}
+
+void launch_prefill_plan(const int* seq_lens, const int* query_start, int B, int H, int Hk, int width, int window, int head_dim,
+                         void* workspace, cudaStream_t s) {
+  throw_if(H % Hk != 0, "H must be a multiple of Hk");
+  if (B == 0) return;
+  const FaStretch sp = stretch_of(workspace, B, H / Hk, head_dim);
+  prefill_plan_kernel<<<1, 256, 0, s>>>(const_cast<long long*>(sp.plan), sp.splits, num_sms(), seq_lens, query_start, B, sp.lg,
+                                        Hk * (H / Hk >> sp.lg), width, window);
+  check_launch("prefill_plan");
+}
+
+void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* kv,
+                            int tokens, const int* seq_lens, const int* query_start, int B, int H, int Hk, float scale,
+                            int window, float softcap, int emu, int head_dim, void* workspace, cudaStream_t s) {
   throw_if(H % Hk != 0, "H must be a multiple of Hk");
   throw_if(q_stride % 8 != 0, "prefill: q row pitch must keep 16-byte alignment");
   throw_if(head_dim != 64 && head_dim != 128, "tcgen05 prefill: head_dim 64 or 128");
   if (q_rows == 0 || B == 0) return;
-  const int grid = num_sms(), G = H / Hk;
-  FaStretch sp;
-  sp.B = B;
-  sp.lg = pack_log2(G);
-  auto* w8 = reinterpret_cast<uint8_t*>(workspace);
-  auto* plan = reinterpret_cast<long long*>(w8);
-  sp.plan = plan;
-  sp.splits = reinterpret_cast<int*>(w8 + ((int64_t)B + 1) * 8);
-  sp.part_o = reinterpret_cast<float*>(w8 + (((int64_t)B + 1) * 8 + (int64_t)grid * 32 + 255) / 256 * 256);
-  sp.part_ml = sp.part_o + (int64_t)grid * 4 * kTQ * head_dim;
-  prefill_plan_kernel<<<1, 256, 0, s>>>(plan, sp.splits, grid, seq_lens, query_start, B, sp.lg, Hk * (G >> sp.lg), window);
-  check_launch("prefill_plan");
-  const uint64_t kv_rows = (uint64_t)num_blocks * 2 * Hk * kBS;
+  throw_if(tokens % kTK != 0, "prefill copy: tokens must be a multiple of 128");
+  const int grid = num_sms();
+  FaStretch sp = stretch_of(workspace, B, H / Hk, head_dim);
+  sp.tokens = tokens;
+  const uint64_t kv_rows = (uint64_t)B * 2 * Hk * tokens;
   CUtensorMap tq = make_tmap_3d(q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, head_dim, H, q_rows, head_dim, q_stride, 64, 1 << sp.lg,
                                 kTQ >> sp.lg, CU_TENSOR_MAP_SWIZZLE_128B);
-  CUtensorMap tkv = make_tmap_2d(cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kv_rows, head_dim, head_dim, kBS, 64,
+  CUtensorMap tkv = make_tmap_2d(kv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, kv_rows, head_dim, head_dim, kTK, 64,
                                  CU_TENSOR_MAP_SWIZZLE_128B);
   const float sl2 = scale * 1.4426950408889634f, cap = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
   auto* o = reinterpret_cast<__nv_bfloat16*>(out);
   auto go = [&](auto kern) {
     GOLLEK_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, fa_smem(head_dim)));
-    kern<<<grid, kFaThreads, fa_smem(head_dim), s>>>(tq, tkv, o, out_stride, block_tables, bt_stride, seq_lens, query_start,
-                                                     nullptr, 0, H, Hk, sl2, bounds_status(), window, cap, num_blocks, sp);
+    kern<<<grid, kFaThreads, fa_smem(head_dim), s>>>(tq, tkv, o, out_stride, nullptr, 0, seq_lens, query_start, nullptr, 0, H,
+                                                     Hk, sl2, bounds_status(), window, cap, 0, sp);
   };
   if (head_dim == 64) {
     if (emu == 2) go(prefill_fa_kernel<2, 64, true>);
@@ -1235,10 +1305,9 @@ void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_
   }
   check_launch("paged_prefill_attention (tcgen05, stretches)");
   if (head_dim == 64)
-    prefill_join_kernel<64><<<dim3(grid, 2, kTQ / 32), 256, 0, s>>>(sp, o, out_stride, seq_lens, query_start, Hk, H, window);
+    launch_after(prefill_join_kernel<64>, dim3(grid, 2, kTQ / 32), 256, 0, s, sp, o, out_stride, seq_lens, query_start, Hk, H, window);
   else
-    prefill_join_kernel<128><<<dim3(grid, 2, kTQ / 32), 256, 0, s>>>(sp, o, out_stride, seq_lens, query_start, Hk, H, window);
-  check_launch("prefill_join");
+    launch_after(prefill_join_kernel<128>, dim3(grid, 2, kTQ / 32), 256, 0, s, sp, o, out_stride, seq_lens, query_start, Hk, H, window);
 }
 
 }  // namespace gollek

@@ -283,8 +283,9 @@ __global__ void __launch_bounds__(256) kv_quant_blocks_kernel(const QuantArgs p)
 }
 
 // ---------------------------------------------------------------------------------------------
-// bf16 copy of the listed blocks (exact: an 8-bit code times a power of two), for prompt attention,
-// in blocks of 16 tokens whatever the cache's block size: dst [rows * mb16, 2, Hk, 16, D]. Row r of
+// bf16 copy of the listed blocks (exact: an 8-bit code times a power of two), for prompt attention:
+// in blocks of 16 tokens whatever the cache's block size, [rows * mb16, 2, Hk, 16, D], or with a sequence's
+// tokens of a head together, [rows, 2, Hk, mb16 * 16, D] (a KV tile is then one box). Row r of
 // the table holds lens[r] tokens: what lies behind them reads as zero up to the next multiple
 // of 128 tokens (the prompt kernels' KV tile) and is not written beyond it. 16 codes per thread.
 // Memory-bound, 3 bytes a value: 48k tokens of 8 heads of 64 in 30 us, 4.9 TB/s.
@@ -293,12 +294,12 @@ template <bool E4M3>
 __global__ void __launch_bounds__(256)
     kv_dequant_scaled_kernel(const uint8_t* __restrict__ cache, const float* __restrict__ scales,
                              const int* __restrict__ tables, int64_t bt_stride, const int* __restrict__ lens, int mb16,
-                             int num_blocks, int Hk, int D, int bs_log2, __nv_bfloat16* __restrict__ dst,
+                             int width, int num_blocks, int Hk, int D, int bs_log2, __nv_bfloat16* __restrict__ dst,
                              const PromptRows prompt, uint32_t* bounds) {
   const int r = blockIdx.y, i = blockIdx.x;             // table row, 16-token block of the row
-  const int L = lens ? min(max(lens[r], 0), mb16 << 4) : mb16 << 4;
-  if (prompt.ids != nullptr) {
-    if (threadIdx.x == 0) prompt.ids[(int64_t)r * mb16 + i] = r * mb16 + i;
+  const int L = lens ? min(max(lens[r], 0), width) : width;
+  if (prompt.lens != nullptr) {
+    if (prompt.ids != nullptr && threadIdx.x == 0) prompt.ids[(int64_t)r * mb16 + i] = r * mb16 + i;
     if (i == 0) {
       if (threadIdx.x == 0) prompt.lens[r] = L;
       const int q0 = prompt.query_start[r], none = prompt.query_start[r + 1] - q0 - L;
@@ -309,35 +310,47 @@ __global__ void __launch_bounds__(256)
     }
   }
   const int tok0 = i << 4;
-  if (tok0 >= ((L + 127) & ~127)) return;
   const int vec = D >> 4;                               // 16-code vectors per token row
-  const int n = 2 * Hk * vec << 4;                      // of the destination block
+  const int n = tok0 < ((L + 127) & ~127) ? 2 * Hk * vec << 4 : 0;  // of the destination block
   int64_t id = 0;
   if (tok0 < L) id = checked_index(tables[(int64_t)r * bt_stride + (tok0 >> bs_log2)], num_blocks, bounds);
   const int off0 = tok0 & ((1 << bs_log2) - 1);
-  const int64_t out0 = ((int64_t)r * mb16 + i) * n;
-  for (int v = threadIdx.x; v < n; v += 256) {
-    const int rowi = v / vec;                           // (K/V, head, token)
-    const int t = rowi & 15;
-    uint4 o[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-    if (tok0 + t < L) {
-      const int64_t row = id * 2 * Hk + (rowi >> 4);
-      const float s = scales[row];
-      const uint4 c = reinterpret_cast<const uint4*>(cache)[((row << bs_log2) + off0 + t) * vec + v % vec];
-      float f[16];
-      decode4<E4M3>(c.x, f);
-      decode4<E4M3>(c.y, f + 4);
-      decode4<E4M3>(c.z, f + 8);
-      decode4<E4M3>(c.w, f + 12);
+  // first row of (K/V, head) 0, and the distance of the next one
+  const int64_t row0 = prompt.together ? (int64_t)r * 2 * Hk * mb16 * 16 + tok0 : ((int64_t)r * mb16 + i) * 2 * Hk * 16;
+  const int64_t hrow = prompt.together ? (int64_t)mb16 * 16 : 16;
+  constexpr int N = 4;                                  // loads of a thread in flight
+  for (int v0 = threadIdx.x; v0 < n; v0 += N * 256) {
+    uint4 c[N];
+    float s[N];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) f[k] *= s;
-      o[0] = float_to_bf16x8(f);
-      o[1] = float_to_bf16x8(f + 8);
+    for (int k = 0; k < N; ++k) {
+      const int v = v0 + k * 256, rowi = v / vec;       // (K/V, head, token)
+      c[k] = make_uint4(0u, 0u, 0u, 0u);
+      s[k] = 0.f;
+      if (v < n && tok0 + (rowi & 15) < L) {
+        const int64_t row = id * 2 * Hk + (rowi >> 4);
+        s[k] = scales[row];
+        c[k] = reinterpret_cast<const uint4*>(cache)[((row << bs_log2) + off0 + (rowi & 15)) * vec + v % vec];
+      }
     }
-    uint4* d = reinterpret_cast<uint4*>(dst) + (out0 + v) * 2;
-    d[0] = o[0];
-    d[1] = o[1];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int v = v0 + k * 256;
+      if (v >= n) break;
+      float f[16];
+      decode4<E4M3>(c[k].x, f);
+      decode4<E4M3>(c[k].y, f + 4);
+      decode4<E4M3>(c[k].z, f + 8);
+      decode4<E4M3>(c[k].w, f + 12);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) f[e] *= s[k];
+      const int rowi = v / vec;
+      uint4* d = reinterpret_cast<uint4*>(dst) + ((row0 + (rowi >> 4) * hrow + (rowi & 15)) * vec + v % vec) * 2;
+      d[0] = float_to_bf16x8(f);
+      d[1] = float_to_bf16x8(f + 8);
+    }
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched beside the plan: it is done when this kernel is
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1511,22 +1524,6 @@ void max_smem_once(int bytes) {
   if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
 }
 
-// Launch whose CTAs start as the kernel before it leaves (it waits for that one's results itself).
-template <class... P, class... A>
-void launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  GOLLEK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
-}
-
 int log2_block(int bs) {
   throw_if(bs != 16 && bs != 32 && bs != 64, "block-scaled KV cache: block size 16, 32 or 64");
   return bs == 16 ? 4 : bs == 32 ? 5 : 6;
@@ -1567,9 +1564,13 @@ void launch_kv_dequant_scaled(const void* cache, const float* scales, const int*
   throw_if(rows > 65535, "kv_dequant_blocks: at most 65535 sequences");
   if (rows == 0 || mb == 0) return;
   auto k = e4m3 ? kv_dequant_scaled_kernel<true> : kv_dequant_scaled_kernel<false>;
-  const int mb16 = mb << (lb - 4);
-  k<<<dim3(mb16, rows), 256, 0, s>>>(reinterpret_cast<const uint8_t*>(cache), scales, tables, bt_stride, lens, mb16,
-                                     num_blocks, Hk, D, lb, reinterpret_cast<__nv_bfloat16*>(dst), prompt, bounds_status());
+  const int mb16 = prompt.together ? (mb * bs + 127) / 128 * 8 : mb << (lb - 4);
+  auto go = [&](auto... a) {  // a plan goes in front of the `together` form, whose CTAs start as it does
+    if (prompt.together) launch_after(k, dim3(mb16, rows), 256, 0, s, a...);
+    else k<<<dim3(mb16, rows), 256, 0, s>>>(a...);
+  };
+  go(reinterpret_cast<const uint8_t*>(cache), scales, tables, bt_stride, lens, mb16, mb * bs, num_blocks, Hk, D, lb,
+     reinterpret_cast<__nv_bfloat16*>(dst), prompt, bounds_status());
   check_launch("kv_dequant_blocks");
 }
 

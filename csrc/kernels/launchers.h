@@ -23,6 +23,23 @@ inline void check_launch(const char* what) {
   if (e != cudaSuccess) throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+// Launch whose CTAs start as the kernel before it leaves or lets them (it waits for that one's results itself).
+template <class... P, class... A>
+void launch_after(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("kernel launch: ") + cudaGetErrorString(e));
+}
+
 // ---- elementwise (K1, K2, K13)
 void launch_rms_norm(void* out, const void* x, void* residual, const void* w, int T, int d, int64_t x_stride,
                      int64_t out_stride, float eps, cudaStream_t s,
@@ -60,12 +77,15 @@ void launch_paged_prefill_fa(void* out, int64_t out_stride, const void* q, int64
                              const int* seq_lens, const int* query_start, const int* work, int nwork, int H, int Hk,
                              float scale, int window, float softcap, int emu, cudaStream_t s, int head_dim = 128);
 // Without a work list: heads of a group packed into the rows of a query tile, KV tiles of all queries shared evenly by
-// the CTAs (bf16 cache of 16-token blocks, head_dim 64 or 128). workspace: prefill_stretch_bytes, 256-byte aligned.
+// the CTAs. First the plan (lengths are cut to `width`), beside which the copy may be made; then the attention over the copy
+// kv [B, 2, Hk, tokens, head_dim] (head_dim 64 or 128, tokens a multiple of 128) with lengths that fit it. workspace:
+// prefill_stretch_bytes, 256-byte aligned.
 int64_t prefill_stretch_bytes(int B, int head_dim);
-void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* cache,
-                            int num_blocks, const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
-                            int B, int H, int Hk, float scale, int window, float softcap, int emu, int head_dim,
-                            void* workspace, cudaStream_t s);
+void launch_prefill_plan(const int* seq_lens, const int* query_start, int B, int H, int Hk, int width, int window, int head_dim,
+                         void* workspace, cudaStream_t s);
+void launch_prefill_stretch(void* out, int64_t out_stride, const void* q, int64_t q_rows, int64_t q_stride, const void* kv,
+                            int tokens, const int* seq_lens, const int* query_start, int B, int H, int Hk, float scale,
+                            int window, float softcap, int emu, int head_dim, void* workspace, cudaStream_t s);
 void launch_paged_prefill(void* out, int64_t out_stride, const void* q, int64_t q_stride, const void* cache,
                           const int* block_tables, int bt_stride, const int* seq_lens, const int* query_start,
                           const int* tiles, int ntiles, int H, int Hk, int D, int block_size, float scale,
@@ -257,9 +277,11 @@ void launch_kv_dequant_blocks(const void* cache, const float* scales, const int*
 void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, const int* slots, void* cache,
                             float* scales, float* mass, int T, int Hk, int D, int bs, int num_blocks, bool e4m3,
                             cudaStream_t s);
-// What prompt attention over the copy needs beside it, where ids is given: the copy's block table, the rows' lengths cut to
-// their tables, and zeros in `out` for queries in front of their sequence's first token (more queries than tokens).
+// What prompt attention over the copy needs beside it, where lens is given: the rows' lengths cut to their tables, zeros in
+// `out` for queries in front of their sequence's first token (more queries than tokens), and the copy's block table,
+// or (together, no table) the copy as [rows, 2, Hk, table width up to a multiple of 128, D].
 struct PromptRows {
+  bool together = false;
   int* ids = nullptr;
   int* lens = nullptr;
   const int* query_start = nullptr;
