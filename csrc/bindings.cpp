@@ -818,6 +818,22 @@ torch::Tensor block8_decode_py(torch::Tensor q, torch::Tensor cache, torch::Tens
   return out;
 }
 
+// Whether prompt attention over `items` work items is better off in stretches, by the pairs of query tiles and KV tiles that
+// a CTA gets, one after the other. The list: its longest item, or its share of rounds of whole items. Stretches: an even
+// share, with tiles filled by heads as well as tokens, but three more places an item and the time of 8 for plan, parts and
+// joins (20 us). The table's width stands for the lengths, which are on the device. Measured (32 heads, 8 KV heads; list,
+// stretches): a prompt of 2048, heads of 128: 58 us, 79; of 4096: 161, 189; eight chunks of 30 to 100 tokens behind 6000,
+// heads of 64: 122, 108; one chunk of 100 behind 6000, heads of 128: 122, 60.
+static bool stretches_pay(int64_t items, int64_t T, int64_t B, int64_t H, int64_t Hk, int64_t width, int64_t window) {
+  const double sms = device_num_sms(), news = (double)T / std::max<int64_t>(B, 1);
+  double most = width / 128.0, mean = std::max(1.0, most - news / 256.0);
+  if (window > 0) most = std::min(most, window / 128.0 + 2), mean = std::min(mean, most);
+  const double list = std::max(most, std::ceil(items / sms) * mean);
+  const int64_t G = H / Hk, pack = G % 8 == 0 ? 8 : G % 4 == 0 ? 4 : G % 2 == 0 ? 2 : 1;  // heads in a query tile
+  const double shared = T * H / 256.0 + 0.5 * B * H / pack;  // pairs of query tiles, half a pair lost a sequence and pack
+  return shared * (mean + 3) / sms + 8 < list;
+}
+
 // Prompt attention over a block-scaled cache (head_dim 64 or 128): bf16 copy of the sequences' blocks, then the tcgen05 kernel.
 torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Tensor scales, torch::Tensor tables,
                                 torch::Tensor lens, torch::Tensor query_start, double scale,
@@ -845,11 +861,9 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
   TORCH_CHECK(out.dim() == 3 && out.stride(2) == 1 && out.stride(1) == D && out.sizes() == q.sizes() &&
                   out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "out must be [T, H, D] like q");
-  // Many items (4096 prompt tokens of 32 heads: 512): the work list's whole items balance by themselves, 155 us against
-  // 197 us in stretches, whose CTAs leave a quarter more parts. Few (eight chunks of 100 over 6000 cached tokens: 128): stretches
-  // fill the GPU and the tiles, 80 us against 104 us.
-  const bool list = tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 && tiles->size(0) >= 2 * device_num_sms();
   const int64_t width = tables.size(1) * cache.size(3);
+  const bool list = tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 &&
+                    !stretches_pay(tiles->size(0), T, B, H, Hk, width, window);
   const int64_t mb16 = list ? width / 16 : (width + 127) / 128 * 8;
   TORCH_CHECK(B * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: the step's blocks exceed one copy's addresses");
   TORCH_CHECK(T == 0 || B == 0 || mb16 > 0, "block_tables: no columns");

@@ -424,9 +424,9 @@ struct FaItem {
 // an equal stretch of it, whatever the lengths. An item counts kFaLead more places than it has KV tiles, in front of them, for
 // what its Q load, first scores and epilogue cost. An item that crosses a border leaves unnormalised sums per CTA, joined by
 // prefill_join_kernel. plan: int64 [B + 1], list position of each sequence's first KV tile, then the list's length.
-// Measured: eight chunks of 100 tokens behind 6000 cached ones, 32 heads, 8 KV heads of 64: 86 us, and 12 us for the joins; the
-// list form takes 104 us for the same. Neither bytes nor a pipe bound it (tensor memory 23 % busy, 0.32 instructions a cycle
-// and scheduler): a tile's scores, maximum, exponentials and products follow one another, and two query tiles hide half of it.
+// Measured: eight chunks of 30 to 100 tokens behind 6000 cached ones, 32 heads, 8 KV heads of 64: 71 us, and 10 us for the joins;
+// the list form takes 100 us for the same. Exponentials bound it: at 16 a cycle and SM they take 45 us of it (more of them on
+// the FMA pipe are slower, 76 us), the rest is the latency of a softmax warp's other steps.
 constexpr int kFaLead = 3;
 struct FaStretch {
   const long long* plan;

@@ -501,8 +501,8 @@ def test_prefill_long_prefixes_gpu(kind, D, G, bs, window, softcap):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("tiles", [False, True])
 def test_prefill_lengths_beside_the_queries_gpu(D, tiles):
-    """Queries in front of their sequence's first token get zeros; a length beyond the table is cut to it. The work list
-    is taken from 296 items on a GPU of 148 multiprocessors."""
+    """Queries in front of their sequence's first token get zeros; a length beyond the table is cut to it. With its short
+    table the work list is taken where there is one."""
     lens, new, H = [0, 100, 7, 300], [150, 400, 7, 20], 40 if tiles else 4
     cache, scales, _, bt, sl = filled("int8", lens, 2, D, 16, 73)
     bt, sl[3] = bt[:, :16], 1000                                       # 256 tokens fit the table
@@ -510,7 +510,6 @@ def test_prefill_lengths_beside_the_queries_gpu(D, tiles):
     q = torch.randn(int(qs[-1]), H, D, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
     work = torch.tensor([[b, r, -1, h] for b, n in enumerate(new) for r in range(0, n, 128) for h in range(H)],
                         dtype=torch.int32)
-    assert not tiles or len(work) >= 2 * torch.cuda.get_device_properties(0).multi_processor_count
     got = ops.paged_prefill_attention(q, cache[0].cuda(), bt.cuda(), sl.cuda(), qs.cuda(), 0.1, tiles=work.cuda() if tiles else None,
                                       out=torch.full_like(q, math.nan), kv_scales=scales[0].cuda()).double().cpu()
     assert not bool(got[:150].any()) and not bool(got[150:450].any())
