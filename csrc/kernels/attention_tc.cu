@@ -426,7 +426,7 @@ struct FaItem {
 // prefill_join_kernel. plan: int64 [B + 1], list position of each sequence's first KV tile, then the list's length.
 // Measured: eight chunks of 30 to 100 tokens behind 6000 cached ones, 32 heads, 8 KV heads of 64: 71 us, and 10 us for the joins;
 // the list form takes 100 us for the same. Exponentials bound it: at 16 a cycle and SM they take 45 us of it (more of them on
-// the FMA pipe are slower, 76 us), the rest is the latency of a softmax warp's other steps.
+// the FMA pipe: the call takes 8 % longer), the rest is the latency of a softmax warp's other steps.
 constexpr int kFaLead = 3;
 struct FaStretch {
   const long long* plan;

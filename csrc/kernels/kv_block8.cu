@@ -1289,19 +1289,17 @@ __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const Evic
 // In place: kept[j] >= j, so a chunk's sources lie at or behind its own places. A chunk may be read as early as one likes
 // (what goes before it is written in front of it), and must be read before it or any later one is written: chunks go
 // up, and a chunk's loads end before a barrier that its stores follow. So codes are read two chunks ahead (cp.async
-// into a ring; a thread only touches the pieces that it loaded itself), the indices and block ids they hang on earlier
+// into a ring; a thread only touches the codes that it loaded itself), the indices and block ids they hang on earlier
 // still. Each destination block gets the smallest power-of-two scale for what it then holds: one barrier a chunk, for its
 // largest magnitude.
-// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 209 us with step 1. Tokens are
-// rows of 128 bytes each from its own place, and a (layer, sequence, head) is one chain of chunks: four CTAs an SM wait for
-// rows in flight. Copies by the bulk engine, a row each, took 313 us.
+// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 176 us with step 1. A (layer,
+// sequence, head) is one chain of chunks, and 512 chains are three or four an SM: latency. With two threads a token, whose
+// loads and stores touch 32 bytes of 16 rows at a time, the way to L2 was the bound (209 us); copies by the bulk engine, a row
+// each, took 313 us.
 // ---------------------------------------------------------------------------------------------
 // A magnitude costs one instruction a value (packed 16-bit maxima), a change of scale by a power of two two, all exact.
 constexpr int kMoveThreads = 256;
-constexpr int kMovePieces = 4;  // 16-byte pieces per thread and chunk
 constexpr int kMoveStages = 3;
-constexpr int kMoveStage = kMoveThreads * (kMovePieces * 16 + 8);  // codes, then their scales
-constexpr int kMoveSmem = kMoveStages * kMoveStage;
 
 // Running maximum magnitude of four codes each in two 16-bit lanes: hi and lo of int8, magnitude bits of e4m3.
 template <bool E4M3>
@@ -1388,15 +1386,29 @@ GOLLEK_DEVICE void move_masses(const EvictArgs& p, const EvictRow& r, int h, int
   }
 }
 
-// NP: pieces of one token that a thread takes (4, or 2 where the head size is no multiple of 64: then two tokens).
-template <bool E4M3, int NP>
+// A warp moves TW tokens of a chunk. Piece i of its lanes covers whole rows of R tokens, so memory sees full lines; the lanes
+// keep one token's index and block id each and hand them round.
+template <int D>
+struct MoveShape {
+  static constexpr int P = D / 16;                       // 16-byte pieces of a token
+  static constexpr int R = 32 / P;                       // tokens a warp takes at once
+  static constexpr int TW = D <= 64 ? 32 : D <= 128 ? 16 : 8;
+  static constexpr int I = (TW + R - 1) / R;
+  static constexpr int kChunk = kMoveThreads / 32 * TW;  // tokens, a multiple of every block size
+  static constexpr int kStage = kMoveThreads * I * 16 + kChunk * 4;  // codes, then their scales
+  static constexpr int kSmem = kMoveStages * kStage;
+};
+
+template <bool E4M3, int D>
 __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const EvictArgs p) {
-  constexpr int NI = kMovePieces / NP;  // tokens per thread and chunk
-  static_assert(NI <= 2, "a stage has room for two scales a thread");
+  using S = MoveShape<D>;
+  constexpr int P = S::P, R = S::R, TW = S::TW, I = S::I, kChunk = S::kChunk;
+  constexpr int GR = TW > 16 ? 2 : 1;  // 16 tokens at an aligned place share a block: groups of pieces with one scale
   extern __shared__ __align__(16) uint8_t ring[];
   // largest magnitude of each destination block of a chunk (float bits): one being filled, one read, one cleared
-  __shared__ uint32_t top[3][64];
-  const int h = blockIdx.x / 3, w = blockIdx.x % 3, b = blockIdx.y, ly = blockIdx.z;  // w: K, V, masses
+  __shared__ uint32_t top[3][kChunk / 16];
+  // masses come last: the CTAs that move codes spread over the SMs evenly
+  const int h = blockIdx.x, b = blockIdx.y, ly = blockIdx.z % p.layers, w = blockIdx.z / p.layers;  // w: K, V, masses
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the choice is still being made
   const EvictRow r = evict_row(p, b);
   if (!r.cut || r.K == 0) return;
@@ -1404,110 +1416,95 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
     move_masses(p, r, h, b, ly);
     return;
   }
-  const int bs = 1 << p.bs_log2, share = p.D / (16 * NP);       // threads of a token
-  const int chunk = kMoveThreads * NI / share / 64 * 64;        // tokens, a multiple of every block size
-  const int chunks = (r.K + chunk - 1) / chunk;
-  // a warp's threads of one destination block: all, half of it, or (a head size that leaves a rest) unknown
-  const int lanes = 32 % share != 0 ? 1 : min(32, bs * share);
-  const uint32_t group = (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1) << (threadIdx.x & 31 & ~(lanes - 1));
+  const int bs = 1 << p.bs_log2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = (r.K + kChunk - 1) / kChunk;
   const int* kept = p.kept + (((int64_t)ly * p.B + b) * p.Hk + h) * p.max_keep;
   const int* bt = p.tables + (int64_t)b * p.bt_stride;
   // a block's K (or V) of this head and its scale: base + block id * stride
-  const uint32_t row_stride = (uint32_t)(2 * p.Hk << p.bs_log2) * p.D;
-  uint8_t* codes = p.cache + ((int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h) * ((int64_t)p.D << p.bs_log2);
+  const uint32_t row_stride = (uint32_t)(2 * p.Hk << p.bs_log2) * D;
+  uint8_t* codes = p.cache + ((int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h) * ((int64_t)D << p.bs_log2);
   float* scales = p.scales + (int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h;
-  int tok[NI];  // this thread's tokens in a chunk; its pieces are piece + 16 share i
-#pragma unroll
-  for (int k = 0; k < NI; ++k) {
-    tok[k] = (k * kMoveThreads + (int)threadIdx.x) / share;
-    if (tok[k] >= chunk) tok[k] = 1 << 30;  // beyond the chunk (a head size that leaves a rest): never below its length
-  }
-  auto piece = [&](int k) { return (k * kMoveThreads + (int)threadIdx.x) % share * 16; };
   auto block_of = [&](int t) { return checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds); };
-  auto code_at = [&](int id, int t, int k) { return codes + (uint64_t)(uint32_t)id * row_stride + (t & (bs - 1)) * p.D + piece(k); };
   auto scale_at = [&](int id) { return scales + (uint64_t)(uint32_t)id * (2 * p.Hk); };
+  const int own = warp * TW + (lane & (TW - 1));  // the token of a chunk whose index and block ids this lane keeps
+  const int piece = lane % P * 16;
+  auto tok = [&](int i) { return i * R + lane / P; };  // token of the warp's that piece i belongs to
+  auto mine = [&](int i) { return lane < R * P && tok(i) < TW; };
 
   // indices of a chunk, block ids of a chunk, codes and scales of a chunk: each one step behind the one before
-  int src2[NI], src1[NI], id1[NI];
-  auto load_src = [&](int c, int* src) {
+  int src2, src1, id1;
+  auto load_src = [&](int c) { return own < r.K - c * kChunk ? kept[c * kChunk + own] : -1; };
+  auto load_id = [&](int src) { return src >= 0 ? block_of(src) : 0; };
+  auto load_codes = [&](int c, int src, int id) {
+    const uint32_t st = smem_u32(ring) + (c % kMoveStages) * S::kStage;
 #pragma unroll
-    for (int k = 0; k < NI; ++k) src[k] = tok[k] < r.K - c * chunk ? kept[c * chunk + tok[k]] : -1;
-  };
-  auto load_ids = [&](const int* src, int* id) {
-#pragma unroll
-    for (int k = 0; k < NI; ++k) id[k] = src[k] >= 0 ? block_of(src[k]) : 0;
-  };
-  auto load_codes = [&](int c, const int* src, const int* id) {
-    const uint32_t st = smem_u32(ring) + (c % kMoveStages) * kMoveStage + threadIdx.x * 16;
-#pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      if (src[k] < 0) continue;
-      const uint8_t* g = code_at(id[k], src[k], k);
-#pragma unroll
-      for (int i = 0; i < NP; ++i) cp_async16<0, 0>(st + (NP * k + i) * kMoveThreads * 16, g + i * share * 16);
-      cp_async4(st + kMovePieces * kMoveThreads * 16 - threadIdx.x * 12 + k * kMoveThreads * 4, scale_at(id[k]));
+    for (int i = 0; i < I; ++i) {
+      const int t = __shfl_sync(0xffffffffu, src, tok(i) & 31), d = __shfl_sync(0xffffffffu, id, tok(i) & 31);
+      if (mine(i) && t >= 0)
+        cp_async16<0, 0>(st + (i * kMoveThreads + threadIdx.x) * 16,
+                         codes + (uint64_t)(uint32_t)d * row_stride + (t & (bs - 1)) * D + piece);
     }
+    if (src >= 0 && lane < TW) cp_async4(st + kMoveThreads * I * 16 + own * 4, scale_at(id));
     cp_async_commit();
   };
-  if (threadIdx.x < 64) top[0][threadIdx.x] = 0u;
+  if (threadIdx.x < kChunk / 16) top[0][threadIdx.x] = 0u;
   // chunk 0 and 1's codes on their way, chunk 2's ids and chunk 3's indices too
-  load_src(0, src2);
-  load_src(1, src1);
-  load_ids(src2, id1);
+  src2 = load_src(0);
+  src1 = load_src(1);
+  id1 = load_id(src2);
   load_codes(0, src2, id1);
-  load_ids(src1, id1);
+  id1 = load_id(src1);
   load_codes(1, src1, id1);
-  load_src(2, src1);
-  load_src(3, src2);
-  load_ids(src1, id1);
+  src1 = load_src(2);
+  src2 = load_src(3);
+  id1 = load_id(src1);
   __syncthreads();
   for (int c = 0; c < chunks; ++c) {
-    const int base = c * chunk, n = min(chunk, r.K - base);
+    const int base = c * kChunk, n = min(kChunk, r.K - base);
     load_codes(c + 2, src1, id1);
-    int to_id[NI];  // destination blocks
-#pragma unroll
-    for (int k = 0; k < NI; ++k) to_id[k] = tok[k] < n ? block_of(base + tok[k]) : 0;
-#pragma unroll
-    for (int k = 0; k < NI; ++k) src1[k] = src2[k];
-    load_ids(src1, id1);
-    load_src(c + 4, src2);
+    const int to_id = own < n ? block_of(base + own) : 0;  // destination block
+    src1 = src2;
+    id1 = load_id(src1);
+    src2 = load_src(c + 4);
     cp_async_wait<2>();
-    uint32_t code[NI][4 * NP];
-    float sc[NI];
-    const uint8_t* st = ring + (c % kMoveStages) * kMoveStage;
+    __syncwarp();  // a token's scale is another lane's copy
+    uint32_t code[I][4];
+    float sc[I];
+    const uint8_t* st = ring + (c % kMoveStages) * S::kStage;
     uint32_t* tp = top[c % 3];
+    uint32_t amax[GR];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      uint32_t amax = 0u;
-      if (tok[k] < n) {
-        Top4<E4M3> t;
+    for (int q = 0; q < GR; ++q) amax[q] = 0u;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          const uint4 x = reinterpret_cast<const uint4*>(st)[(NP * k + i) * kMoveThreads + threadIdx.x];
-          code[k][4 * i] = x.x, code[k][4 * i + 1] = x.y, code[k][4 * i + 2] = x.z, code[k][4 * i + 3] = x.w;
-        }
+    for (int i = 0; i < I; ++i) {
+      if (!mine(i) || warp * TW + tok(i) >= n) continue;
+      Top4<E4M3> t;
+      const uint4 x = reinterpret_cast<const uint4*>(st)[i * kMoveThreads + threadIdx.x];
+      code[i][0] = x.x, code[i][1] = x.y, code[i][2] = x.z, code[i][3] = x.w;
 #pragma unroll
-        for (int i = 0; i < 4 * NP; ++i) t.add(code[k][i]);
-        sc[k] = reinterpret_cast<const float*>(st + kMovePieces * kMoveThreads * 16)[k * kMoveThreads + threadIdx.x];
-        amax = __float_as_uint(t.value() * sc[k]);
-      }
-      amax = __reduce_max_sync(group, amax);
-      if ((threadIdx.x & (lanes - 1)) == 0 && tok[k] < n) atomicMax(&tp[tok[k] >> p.bs_log2], amax);
+      for (int k = 0; k < 4; ++k) t.add(code[i][k]);
+      sc[i] = reinterpret_cast<const float*>(st + kMoveThreads * I * 16)[warp * TW + tok(i)];
+      amax[i * R / 16 % GR] = max(amax[i * R / 16 % GR], __float_as_uint(t.value() * sc[i]));
     }
-    if (threadIdx.x < 64) top[(c + 1) % 3][threadIdx.x] = 0u;  // its readers are behind the last barrier, its writers the next
+#pragma unroll
+    for (int q = 0; q < GR; ++q) {
+      amax[q] = __reduce_max_sync(0xffffffffu, amax[q]);
+      if (lane == 0) atomicMax(&tp[(warp * TW + 16 * q) >> p.bs_log2], amax[q]);
+    }
+    if (threadIdx.x < kChunk / 16) top[(c + 1) % 3][threadIdx.x] = 0u;  // its readers are behind the last barrier, its writers the next
     __syncthreads();
+    float s[GR];
 #pragma unroll
-    for (int k = 0; k < NI; ++k) {
-      if (tok[k] >= n) continue;
-      const int to = base + tok[k];
-      const float s = pow2_scale<E4M3>(__uint_as_float(tp[tok[k] >> p.bs_log2]));
-      rescale<E4M3, 4 * NP>(code[k], sc[k] * __uint_as_float((254u << 23) - __float_as_uint(s)));  // sc / s, s = 2^e
-      uint8_t* d = code_at(to_id[k], to, k);
+    for (int q = 0; q < GR; ++q) s[q] = pow2_scale<E4M3>(__uint_as_float(tp[(warp * TW + 16 * q) >> p.bs_log2]));
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
-        *reinterpret_cast<uint4*>(d + i * share * 16) =
-            make_uint4(code[k][4 * i], code[k][4 * i + 1], code[k][4 * i + 2], code[k][4 * i + 3]);
-      if ((to & (bs - 1)) == 0 && piece(k) == 0) *scale_at(to_id[k]) = s;
+    for (int i = 0; i < I; ++i) {
+      const int d = __shfl_sync(0xffffffffu, to_id, tok(i) & 31), to = base + warp * TW + tok(i);
+      if (!mine(i) || to - base >= n) continue;
+      const float z = s[i * R / 16 % GR];
+      rescale<E4M3, 4>(code[i], sc[i] * __uint_as_float((254u << 23) - __float_as_uint(z)));  // sc / z, z = 2^e
+      *reinterpret_cast<uint4*>(codes + (uint64_t)(uint32_t)d * row_stride + (to & (bs - 1)) * D + piece) =
+          make_uint4(code[i][0], code[i][1], code[i][2], code[i][3]);
+      if ((to & (bs - 1)) == 0 && piece == 0) *scale_at(d) = z;
     }
   }
   cp_async_wait<0>();
@@ -1684,8 +1681,8 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
                      const int* lens, const int* keep, int* kept, int layers, int B, int Hk, int D, int bs,
                      int num_blocks, int sink, int recent, int max_keep, bool e4m3, cudaStream_t s) {
-  throw_if(D % 32 != 0 || D > 256, "kv_evict: head_dim must be a multiple of 32, <= 256");
-  throw_if(B > 65535 || layers > 65535, "kv_evict: at most 65535 sequences and layers");
+  throw_if(D % 32 != 0 || D < 32 || D > 256, "kv_evict: head_dim must be a multiple of 32, <= 256");
+  throw_if(B > 65535 || layers > 65535 / 3, "kv_evict: at most 65535 sequences and 21845 layers");
   EvictArgs p;
   p.bs_log2 = log2_block(bs);
   if (layers == 0 || B == 0 || Hk == 0) return;
@@ -1705,20 +1702,23 @@ void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables,
   kv_evict_select_kernel<<<dim3(Hk, B, layers), kSelThreads, smem, s>>>(p);
   check_launch("kv_evict_select");
   if (max_keep == 0) return;
-  const dim3 grid(3 * Hk, B, layers);
-#define GOLLEK_MOVE(E, NP)                                                                      \
-  do {                                                                                          \
-    max_smem_once<kv_evict_move_kernel<E, NP>>(kMoveSmem);                                      \
-    launch_after(kv_evict_move_kernel<E, NP>, grid, kMoveThreads, kMoveSmem, s, p);             \
-  } while (0)
-  if (D % 64 == 0) {
-    if (e4m3) GOLLEK_MOVE(true, 4);
-    else GOLLEK_MOVE(false, 4);
-  } else {
-    if (e4m3) GOLLEK_MOVE(true, 2);
-    else GOLLEK_MOVE(false, 2);
+  auto move = [&](auto e, auto d) {
+    constexpr auto k = kv_evict_move_kernel<decltype(e)::value, decltype(d)::value>;
+    constexpr int smem = MoveShape<decltype(d)::value>::kSmem;
+    max_smem_once<k>(smem);
+    launch_after(k, dim3(Hk, B, 3 * layers), kMoveThreads, smem, s, p);
+  };
+  auto kind = [&](auto d) { e4m3 ? move(std::true_type{}, d) : move(std::false_type{}, d); };
+  switch (D) {
+    case 32: kind(std::integral_constant<int, 32>{}); break;
+    case 64: kind(std::integral_constant<int, 64>{}); break;
+    case 96: kind(std::integral_constant<int, 96>{}); break;
+    case 128: kind(std::integral_constant<int, 128>{}); break;
+    case 160: kind(std::integral_constant<int, 160>{}); break;
+    case 192: kind(std::integral_constant<int, 192>{}); break;
+    case 224: kind(std::integral_constant<int, 224>{}); break;
+    default: kind(std::integral_constant<int, 256>{});
   }
-#undef GOLLEK_MOVE
 }
 
 }  // namespace gollek

@@ -613,7 +613,7 @@ def test_evict_cpu(kind, sink, recent, max_keep):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
-@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (96, 16), (256, 64), (32, 16)])
+@pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (64, 16), (96, 16), (256, 64), (32, 16), (160, 16), (192, 32), (224, 16)])
 @pytest.mark.parametrize("sink,recent,max_keep", EVICT)
 def test_evict_gpu(kind, D, bs, sink, recent, max_keep):
     c = evict_case(kind, D, bs, 31)
