@@ -75,7 +75,8 @@ GOLLEK_DEVICE void decode4(uint32_t w, float* f) {
 // there to a raised scale, and stores the run's codes. Memory-bound: 3 bytes a value. A run of at most 16 tokens stays
 // in registers between its magnitude and its codes (16-byte loads, all of them in flight at once); a longer one is read twice.
 // Measured (8 heads of 128): 48 rows of one token 3.2 us, the latency of slot, first code and scale one behind the other;
-// 8190 prompt tokens 16 us, 3.1 TB/s: the 16 warps an SM holds at 126 registers keep too few bytes in flight for more.
+// 8190 prompt tokens 14.7 us, 3.4 TB/s: bytes in flight, with the 20 warps an SM holds at 96 registers (16 at 126: 16.4 us; 24
+// at 80 spill: 18 us).
 // ---------------------------------------------------------------------------------------------
 GOLLEK_DEVICE uint32_t clean2(uint32_t w) {  // two bf16: NaN -> 0, infinities -> the largest bf16
   uint32_t r = 0;
@@ -131,11 +132,13 @@ struct QuantArgs {
   uint32_t* bounds;
 };
 
+constexpr int kQuantThreads = 128;
+
 template <bool E4M3, int D>
-__global__ void __launch_bounds__(256) kv_quant_blocks_kernel(const QuantArgs p) {
+__global__ void __launch_bounds__(kQuantThreads, D <= 64 ? 6 : D <= 128 ? 5 : 3) kv_quant_blocks_kernel(const QuantArgs p) {
   constexpr int LPR = D / 8, TPI = 32 / LPR;      // lanes of a row (8 values each), rows a warp takes at once
   constexpr int R = (16 + TPI - 1) / TPI;         // rounds for 16 rows
-  const int64_t gw = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int64_t gw = (int64_t)blockIdx.x * (kQuantThreads / 32) + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31, sub = lane / LPR, pos = lane % LPR;
   const int64_t grp = gw / (2 * p.Hk);
   const int pair = (int)(gw - grp * (2 * p.Hk));
@@ -1536,11 +1539,11 @@ void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, 
   if (T == 0) return;
   p.g = T >= 1024 ? 16 : 1;  // about one run of a prompt, one row of a decode step
   const int64_t warps = (int64_t)((T + p.g - 1) / p.g) * 2 * Hk;
-  const unsigned grid = (unsigned)((warps + 7) / 8);
+  const unsigned grid = (unsigned)((warps + kQuantThreads / 32 - 1) / (kQuantThreads / 32));
 #define GOLLEK_QB(DD)                                                        \
   if (D == DD) {                                                             \
-    if (e4m3) kv_quant_blocks_kernel<true, DD><<<grid, 256, 0, s>>>(p);      \
-    else kv_quant_blocks_kernel<false, DD><<<grid, 256, 0, s>>>(p);          \
+    if (e4m3) kv_quant_blocks_kernel<true, DD><<<grid, kQuantThreads, 0, s>>>(p);\
+    else kv_quant_blocks_kernel<false, DD><<<grid, kQuantThreads, 0, s>>>(p);\
     check_launch("kv_quant_blocks");                                         \
     return;                                                                  \
   }
