@@ -290,14 +290,15 @@ __global__ void __launch_bounds__(kQuantThreads, D <= 64 ? 6 : D <= 128 ? 5 : 3)
 // in blocks of 16 tokens whatever the cache's block size, [rows * mb16, 2, Hk, 16, D], or with a sequence's
 // tokens of a head together, [rows, 2, Hk, mb16 * 16, D] (a KV tile is then one box). Row r of
 // the table holds lens[r] tokens: what lies behind them reads as zero up to the next multiple
-// of 128 tokens (the prompt kernels' KV tile) and is not written beyond it. 16 codes per thread.
-// Memory-bound, 3 bytes a value: 48k tokens of 8 heads of 64 in 30 us, 4.9 TB/s.
+// of 128 tokens (the prompt kernels' KV tile) and is not written beyond it. 8 codes a lane: a warp stores 512 bytes on end.
+// Memory-bound, 3 bytes a value: 48k tokens of 8 heads of 64 in 26 us, 5.6 TB/s (four CTAs an SM; three, with twice the loads
+// of a thread in flight, 29 us; 16 codes a lane, whose stores fill half a sector each, 31 us).
 // ---------------------------------------------------------------------------------------------
-template <bool E4M3>
-__global__ void __launch_bounds__(256)
+template <bool E4M3, int D>
+__global__ void __launch_bounds__(256, 4)
     kv_dequant_scaled_kernel(const uint8_t* __restrict__ cache, const float* __restrict__ scales,
                              const int* __restrict__ tables, int64_t bt_stride, const int* __restrict__ lens, int mb16,
-                             int width, int num_blocks, int Hk, int D, int bs_log2, __nv_bfloat16* __restrict__ dst,
+                             int width, int num_blocks, int Hk, int bs_log2, __nv_bfloat16* __restrict__ dst,
                              const PromptRows prompt, uint32_t* bounds) {
   const int r = blockIdx.y, i = blockIdx.x;             // table row, 16-token block of the row
   const int L = lens ? min(max(lens[r], 0), width) : width;
@@ -313,7 +314,7 @@ __global__ void __launch_bounds__(256)
     }
   }
   const int tok0 = i << 4;
-  const int vec = D >> 4;                               // 16-code vectors per token row
+  constexpr int vec = D / 8;                            // 8-code vectors per token row
   const int n = tok0 < ((L + 127) & ~127) ? 2 * Hk * vec << 4 : 0;  // of the destination block
   int64_t id = 0;
   if (tok0 < L) id = checked_index(tables[(int64_t)r * bt_stride + (tok0 >> bs_log2)], num_blocks, bounds);
@@ -323,34 +324,30 @@ __global__ void __launch_bounds__(256)
   const int64_t hrow = prompt.together ? (int64_t)mb16 * 16 : 16;
   constexpr int N = 4;                                  // loads of a thread in flight
   for (int v0 = threadIdx.x; v0 < n; v0 += N * 256) {
-    uint4 c[N];
+    uint2 c[N];
     float s[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int v = v0 + k * 256, rowi = v / vec;       // (K/V, head, token)
-      c[k] = make_uint4(0u, 0u, 0u, 0u);
+      c[k] = make_uint2(0u, 0u);
       s[k] = 0.f;
       if (v < n && tok0 + (rowi & 15) < L) {
         const int64_t row = id * 2 * Hk + (rowi >> 4);
         s[k] = scales[row];
-        c[k] = reinterpret_cast<const uint4*>(cache)[((row << bs_log2) + off0 + (rowi & 15)) * vec + v % vec];
+        c[k] = reinterpret_cast<const uint2*>(cache)[((row << bs_log2) + off0 + (rowi & 15)) * vec + v % vec];
       }
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int v = v0 + k * 256;
       if (v >= n) break;
-      float f[16];
+      float f[8];
       decode4<E4M3>(c[k].x, f);
       decode4<E4M3>(c[k].y, f + 4);
-      decode4<E4M3>(c[k].z, f + 8);
-      decode4<E4M3>(c[k].w, f + 12);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) f[e] *= s[k];
+      for (int e = 0; e < 8; ++e) f[e] *= s[k];
       const int rowi = v / vec;
-      uint4* d = reinterpret_cast<uint4*>(dst) + ((row0 + (rowi >> 4) * hrow + (rowi & 15)) * vec + v % vec) * 2;
-      d[0] = float_to_bf16x8(f);
-      d[1] = float_to_bf16x8(f + 8);
+      reinterpret_cast<uint4*>(dst)[(row0 + (rowi >> 4) * hrow + (rowi & 15)) * vec + v % vec] = float_to_bf16x8(f);
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched beside the plan: it is done when this kernel is
@@ -1559,17 +1556,25 @@ void launch_kv_quant_blocks(const void* kv, int64_t st, int64_t sw, int64_t sh, 
 void launch_kv_dequant_scaled(const void* cache, const float* scales, const int* tables, int64_t bt_stride,
                               const int* lens, int rows, int mb, int num_blocks, int Hk, int D, int bs, bool e4m3,
                               void* dst, cudaStream_t s, const PromptRows& prompt) {
-  throw_if(D % 16 != 0, "block-scaled KV cache: head_dim must be a multiple of 16");
   const int lb = log2_block(bs);
   throw_if(rows > 65535, "kv_dequant_blocks: at most 65535 sequences");
   if (rows == 0 || mb == 0) return;
-  auto k = e4m3 ? kv_dequant_scaled_kernel<true> : kv_dequant_scaled_kernel<false>;
+  auto of = [&](auto d) {
+    constexpr int DD = decltype(d)::value;
+    return e4m3 ? kv_dequant_scaled_kernel<true, DD> : kv_dequant_scaled_kernel<false, DD>;
+  };
+  throw_if(D != 32 && D != 64 && D != 96 && D != 128 && D != 256, "block-scaled KV cache: unsupported head_dim " + std::to_string(D));
+  auto k = D == 32    ? of(std::integral_constant<int, 32>{})
+           : D == 64  ? of(std::integral_constant<int, 64>{})
+           : D == 96  ? of(std::integral_constant<int, 96>{})
+           : D == 128 ? of(std::integral_constant<int, 128>{})
+                      : of(std::integral_constant<int, 256>{});
   const int mb16 = prompt.together ? (mb * bs + 127) / 128 * 8 : mb << (lb - 4);
   auto go = [&](auto... a) {  // a plan goes in front of the `together` form, whose CTAs start as it does
     if (prompt.together) launch_after(k, dim3(mb16, rows), 256, 0, s, a...);
     else k<<<dim3(mb16, rows), 256, 0, s>>>(a...);
   };
-  go(reinterpret_cast<const uint8_t*>(cache), scales, tables, bt_stride, lens, mb16, mb * bs, num_blocks, Hk, D, lb,
+  go(reinterpret_cast<const uint8_t*>(cache), scales, tables, bt_stride, lens, mb16, mb * bs, num_blocks, Hk, lb,
      reinterpret_cast<__nv_bfloat16*>(dst), prompt, bounds_status());
   check_launch("kv_dequant_blocks");
 }
