@@ -653,14 +653,14 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
             const uint32_t d2 = st + (tile * 16 + row) * S::kRow + ((ch ^ ((row + 2 * R) & 7)) << 4);
             const uint32_t d3 = st + (tile * 16 + row) * S::kRow + ((ch ^ ((row + 3 * R) & 7)) << 4);
             GOLLEK_TILE(0) GOLLEK_TILE(1) GOLLEK_TILE(4) GOLLEK_TILE(5)
-            cp_async16<2 * RB, 1024>(d2, ck);
-            cp_async16<2 * RB + S::kSide, 1024>(d2, cv);
-            cp_async16<6 * RB, 3072>(d2, ck);
-            cp_async16<6 * RB + S::kSide, 3072>(d2, cv);
-            cp_async16<3 * RB, 1536>(d3, ck);
-            cp_async16<3 * RB + S::kSide, 1536>(d3, cv);
-            cp_async16<7 * RB, 3584>(d3, ck);
-            cp_async16<7 * RB + S::kSide, 3584>(d3, cv);
+            cp_async16<2 * RB, 2 * 512>(d2, ck);
+            cp_async16<2 * RB + S::kSide, 2 * 512>(d2, cv);
+            cp_async16<6 * RB, 6 * 512>(d2, ck);
+            cp_async16<6 * RB + S::kSide, 6 * 512>(d2, cv);
+            cp_async16<3 * RB, 3 * 512>(d3, ck);
+            cp_async16<3 * RB + S::kSide, 3 * 512>(d3, cv);
+            cp_async16<7 * RB, 7 * 512>(d3, ck);
+            cp_async16<7 * RB + S::kSide, 7 * 512>(d3, cv);
           }
 #undef GOLLEK_TILE
         } else {
