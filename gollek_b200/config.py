@@ -615,7 +615,7 @@ class EngineConfig:
     num_gpu_blocks: Optional[int] = None      # None => size from memory fraction
     gpu_memory_utilization: float = 0.85
     # auto (= model dtype) | fp8 (e4m3, a scale per token and head) | int8 or fp8_block (8-bit codes with one
-    # power-of-two scale per block and head)
+    # power-of-two scale per block and head; not with speculative decoding, whose rejected drafts would raise scales)
     kv_cache_dtype: str = "auto"
     enable_prefix_caching: bool = True
     # KV eviction under memory pressure (opt-in; changes outputs): when the block pool is more than

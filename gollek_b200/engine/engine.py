@@ -107,12 +107,14 @@ class LLMEngine:
                 raise ValueError("block-scaled KV cache: block size 16, 32 or 64")
             if cfg.kv_eviction and not weigh:
                 raise ValueError("block-scaled KV cache: eviction is by attention weight (kv_eviction_policy attention)")
+            if cfg.speculative_method != "none":
+                # a draft's row may raise its block's scale, which rounds the accepted tokens' codes for good
+                raise ValueError("block-scaled KV cache: rejected drafts would coarsen accepted tokens; "
+                                 "speculative decoding is not supported")
             self.model.kv_block8 = True
         elif weigh:
             raise ValueError("kv_eviction_policy attention needs a block-scaled KV cache (kv_cache_dtype int8 or fp8_block)")
         if weigh:
-            if cfg.speculative_method != "none":
-                raise ValueError("kv_eviction_policy attention: rejected drafts would weigh the cache; not supported")
             cfg.enable_prefix_caching = False  # tokens move between blocks: none may be shared
         kv_fp8 = cfg.kv_cache_dtype in ("fp8", "fp8_e4m3")
         if kv_fp8:

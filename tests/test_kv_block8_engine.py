@@ -150,6 +150,15 @@ def test_refusals_and_stats(tiny_cfg, tiny_weights):
         ae.shutdown(drain=False)
 
 
+@pytest.mark.parametrize("kind", ["int8", "fp8_block"])
+@pytest.mark.parametrize("method", ["ngram", "draft"])
+def test_speculation_is_refused(tiny_cfg, tiny_weights, kind, method):
+    """A draft's row raises its block's scale and rounds the rows before it; a rejected draft leaves them so."""
+    with pytest.raises(ValueError, match="coarsen"):
+        engine(tiny_cfg, tiny_weights, kv_cache_dtype=kind, speculative_method=method)
+    assert engine(tiny_cfg, tiny_weights, kv_cache_dtype="auto", speculative_method="ngram").spec is not None
+
+
 def test_snapshot_of_another_cache_is_refused(tiny_cfg, tiny_weights, tmp_path):
     src = engine(tiny_cfg, tiny_weights, kv_cache_dtype="auto")
     src.generate([list(range(3, 100))], SamplingParams(temperature=0.0, max_tokens=2, ignore_eos=True))
