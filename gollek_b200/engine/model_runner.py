@@ -178,7 +178,7 @@ class ModelRunner:
         m = AttnMetadata(positions=positions[r0:r1], slot_mapping=slots[r0:r1], num_decode=max(0, min(s1, nd) - s0))
         ndh = m.num_decode
         if ndh > 0:
-            m.decode_block_tables = bt[s0:s0 + ndh]
+            m.decode_block_tables = bt[s0:s0 + ndh, :self._table_width(h.seq_lens[s0:s0 + ndh].max())]
             m.decode_seq_lens = lens[s0:s0 + ndh]
             m.decode_splits = self._decode_splits(ndh, int(h.seq_lens[s0:s0 + ndh].max()))
         p0 = max(s0, nd)
@@ -199,7 +199,7 @@ class ModelRunner:
             for q in q_lens:
                 qs.append(qs[-1] + q)
             m.num_prefill_tokens = qs[-1]
-            m.prefill_block_tables = bt[p0:s1]
+            m.prefill_block_tables = bt[p0:s1, :self._table_width(max(seq_lens))]
             m.prefill_seq_lens = torch.tensor(seq_lens, dtype=torch.int32).to(dev, non_blocking=True)
             m.prefill_query_start = torch.tensor(qs, dtype=torch.int32).to(dev, non_blocking=True)
             if self.is_cuda:
@@ -242,6 +242,11 @@ class ModelRunner:
         if rows:
             meta.mm_rows = torch.tensor(rows, dtype=torch.int64).to(self.device, non_blocking=True)
             meta.mm_embeds = torch.cat(embs).to(self.device)
+
+    def _table_width(self, longest) -> int:
+        """Columns of the block table that rows of at most ``longest`` tokens need. Operators over an 8-bit cache size copies,
+        scores and grids by the table's width, so each call gets its own rows' width, not the step's."""
+        return max(1, (int(longest) + self.block_size - 1) // self.block_size)
 
     def _decode_splits(self, nd: int, max_len: int) -> int:
         return ops.decode_splits(nd, self.model.Hk, max_len, self.num_sms, self.block_size)
@@ -387,7 +392,7 @@ class ModelRunner:
             if not sync:
                 return self._replay_decode(nd, patch=patch, sync=False)
             return [[t] for t in self._replay_decode(nd)]
-        nb = int(max(1, (int(h.seq_lens[:n].max()) + self.block_size - 1) // self.block_size))
+        nb = self._table_width(h.seq_lens[:n].max())
         self.h2d_bytes += 4 * (3 * T + n * self.max_blocks + n + (n - nd + 1)) + 8 * max(1, len(sample_rows))
         self.d2h_bytes += 8 * len(sample_rows)
         input_ids = h.input_ids[:T].to(dev, non_blocking=True)
@@ -400,13 +405,13 @@ class ModelRunner:
         meta = AttnMetadata(positions=positions, slot_mapping=slots, num_decode=nd)
         self._gdn_meta(meta, n)
         if nd > 0:
-            meta.decode_block_tables = bt[:nd]
+            meta.decode_block_tables = bt[:nd, :self._table_width(h.seq_lens[:nd].max())]
             meta.decode_seq_lens = lens[:nd]
             meta.decode_splits = self._decode_splits(nd, int(h.seq_lens[:nd].max()))
         if n > nd:
             qs = h.query_start[nd: n + 1] - h.query_start[nd]
             meta.num_prefill_tokens = T - nd
-            meta.prefill_block_tables = bt[nd:]
+            meta.prefill_block_tables = bt[nd:, :self._table_width(h.seq_lens[nd:n].max())]
             meta.prefill_seq_lens = lens[nd:]
             meta.prefill_query_start = qs.to(dev, non_blocking=True)
             if self.is_cuda:
@@ -471,7 +476,7 @@ class ModelRunner:
         n, T, _, _ = self._fill_host(out)
         h = self.host
         dev = self.device
-        nb = int(max(1, (int(h.seq_lens[:n].max()) + self.block_size - 1) // self.block_size))
+        nb = self._table_width(h.seq_lens[:n].max())
         bt = h.block_tables[:n].to(dev)[:, :nb]
         qs = h.query_start[: n + 1].clone()
         meta = AttnMetadata(positions=h.positions[:T].to(dev), slot_mapping=h.slots[:T].to(dev), num_decode=0,

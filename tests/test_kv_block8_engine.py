@@ -210,3 +210,37 @@ def test_captured_padding_rows_weigh_nothing_gpu():
     total = float(eng.model.kv_mass.double().sum())
     queries = sum(len(s.output_token_ids) for s in eng.seqs.values())
     assert len(eng.seqs) == 3 and abs(total - queries * cfg.num_attention_heads) < 1e-2
+
+
+@pytest.mark.parametrize("halves", [False, True])
+def test_tables_are_as_wide_as_their_own_rows(tiny_cfg, tiny_weights, halves):
+    """Decoding rows of 300 tokens beside prompts of 20 and the other way round: operators over an 8-bit cache size their
+    copies and scores by the table, so neither call may get the step's widest row."""
+    eng = engine(tiny_cfg, tiny_weights)
+    if halves:
+        eng.runner.split_min_tokens = 1
+        eng.model.can_split_batch = lambda: True
+    seen, forward = [], eng.model.forward
+
+    def spy(ids, meta, cache, **kw):
+        for m in meta.halves[1:] if meta.halves else (meta,):
+            for kind in ("decode", "prefill"):
+                bt, lens = getattr(m, kind + "_block_tables"), getattr(m, kind + "_seq_lens")
+                if bt is not None and lens is not None and len(lens):
+                    assert bt.shape[0] == len(lens)
+                    seen.append((kind, bt.shape[1], max(1, -(-int(lens.max()) // 16)), m.num_decode > 0 and m.num_prefill_tokens > 0))
+        meta.halves = None
+        return forward(ids, meta, cache, **kw)
+
+    eng.model.forward = spy
+    g = torch.Generator().manual_seed(6)
+    params = SamplingParams(temperature=0.0, max_tokens=12, ignore_eos=True)
+    for at, n in ((0, 300), (2, 20), (3, 20), (6, 330)):
+        while eng._steps < at:
+            eng.step()
+        eng.add_request(str(at), torch.randint(3, 250, (n,), generator=g).tolist(), params)
+    while eng.has_unfinished():
+        eng.step()
+    assert {k for k, *_, mixed in seen if mixed} == {"decode", "prefill"} or halves
+    assert all(w == need for _, w, need, _ in seen), seen
+    assert any(w < 3 for _, w, *_ in seen) and any(w > 18 for _, w, *_ in seen)
