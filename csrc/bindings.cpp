@@ -834,6 +834,10 @@ static bool stretches_pay(int64_t items, int64_t T, int64_t B, int64_t H, int64_
   return shared * (mean + 3) / sms + 8 < list;
 }
 
+// The most that the bf16 copy of prompt attention takes (unless the queries take half as much themselves): a quarter of what the
+// engine keeps back from the pool. At 8 KV heads of 128 that is 262144 tokens; fewer, longer groups would not be faster.
+constexpr int64_t kPromptCopyBytes = 1ll << 30;
+
 // Prompt attention over a block-scaled cache (head_dim 64 or 128): bf16 copy of the sequences' blocks, then the tcgen05 kernel.
 torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Tensor scales, torch::Tensor tables,
                                 torch::Tensor lens, torch::Tensor query_start, double scale,
@@ -862,20 +866,26 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
                   out.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "out must be [T, H, D] like q");
   const int64_t width = tables.size(1) * cache.size(3);
-  const bool list = tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 &&
+  TORCH_CHECK(T == 0 || B == 0 || width > 0, "block_tables: no columns");
+  // The copy is as wide as the table, for the lengths are on the device. Sequences whose copy would pass the limit go
+  // in groups, one behind the other, through one copy of the limit's size (or of one sequence, if that is more).
+  const int64_t limit = std::max<int64_t>(kPromptCopyBytes, 2 * q.numel() * q.element_size());
+  const int64_t wide16 = (width + 127) / 128 * 8, row_bytes = std::max<int64_t>(1, wide16 * 2 * Hk * 16 * D * 2);
+  const int64_t group = std::max<int64_t>(1, std::min({B, limit / row_bytes, INT32_MAX / std::max<int64_t>(1, wide16 * 2 * Hk * 16)}));
+  const bool list = group >= B && tiles.has_value() && tiles->dim() == 2 && tiles->size(1) == 4 &&
                     !stretches_pay(tiles->size(0), T, B, H, Hk, width, window);
-  const int64_t mb16 = list ? width / 16 : (width + 127) / 128 * 8;
-  TORCH_CHECK(B * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: the step's blocks exceed one copy's addresses");
-  TORCH_CHECK(T == 0 || B == 0 || mb16 > 0, "block_tables: no columns");
-  auto copy = torch::empty({B * mb16, 2, Hk, 16, D}, q.options());
+  const int64_t mb16 = list ? width / 16 : wide16;
+  TORCH_CHECK(group * mb16 * 2 * Hk * 16 <= INT32_MAX, "prompt attention: a sequence's blocks exceed one copy's addresses");
+  auto copy = torch::empty({std::min(B, group) * mb16, 2, Hk, 16, D}, q.options());
   auto cut = torch::empty({B}, lens.options());
   PromptRows prompt;
-  prompt.together = !list, prompt.lens = cut.data_ptr<int>(), prompt.query_start = query_start.data_ptr<int>();
+  prompt.together = !list;
   prompt.out = out.data_ptr(), prompt.out_stride = out.stride(0), prompt.width = (int)(H * D);
-  auto make_copy = [&]() {
-    launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>(), tables.stride(0),
-                             lens.data_ptr<int>(), B, tables.size(1), (int)cache.size(0), Hk, D, cache.size(3), e4m3,
-                             copy.data_ptr(), cur_stream(), prompt);
+  auto make_copy = [&](int64_t b0, int64_t n) {
+    prompt.lens = cut.data_ptr<int>() + b0, prompt.query_start = query_start.data_ptr<int>() + b0;
+    launch_kv_dequant_scaled(cache.data_ptr(), scales.data_ptr<float>(), tables.data_ptr<int>() + b0 * tables.stride(0),
+                             tables.stride(0), lens.data_ptr<int>() + b0, n, tables.size(1), (int)cache.size(0), Hk, D,
+                             cache.size(3), e4m3, copy.data_ptr(), cur_stream(), prompt);
   };
   if (list) {
     check_i32(*tiles, "tiles");
@@ -883,20 +893,24 @@ torch::Tensor block8_prefill_py(torch::Tensor q, torch::Tensor cache, torch::Ten
     TORCH_CHECK(tiles->is_contiguous(), "tiles: contiguous work list");
     auto ids = torch::empty({B, mb16}, tables.options());
     prompt.ids = ids.data_ptr<int>();
-    make_copy();
+    make_copy(0, B);
     launch_paged_prefill_fa(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(B * mb16),
                             ids.data_ptr<int>(), (int)mb16, cut.data_ptr<int>(), query_start.data_ptr<int>(),
                             tiles->data_ptr<int>(), tiles->size(0), (int)H, (int)Hk, (float)scale, (int)window,
                             (float)softcap, (int)emu, cur_stream(), (int)D);
     return out;
   }
-  auto ws = torch::empty({prefill_stretch_bytes((int)B, (int)D)}, q.options().dtype(at::kByte));
-  launch_prefill_plan(lens.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H, (int)Hk, (int)width, (int)window,
-                      (int)D, ws.data_ptr(), cur_stream());
-  make_copy();
-  launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(mb16 * 16),
-                         cut.data_ptr<int>(), query_start.data_ptr<int>(), (int)B, (int)H, (int)Hk, (float)scale, (int)window,
-                         (float)softcap, (int)emu, (int)D, ws.data_ptr(), cur_stream());
+  auto ws = torch::empty({prefill_stretch_bytes((int)group, (int)D)}, q.options().dtype(at::kByte));
+  for (int64_t b0 = 0; b0 < B; b0 += group) {
+    const int n = (int)std::min(group, B - b0);
+    const int* qs = query_start.data_ptr<int>() + b0;
+    launch_prefill_plan(lens.data_ptr<int>() + b0, qs, n, (int)H, (int)Hk, (int)width, (int)window, (int)D, ws.data_ptr(),
+                        cur_stream());
+    make_copy(b0, n);
+    launch_prefill_stretch(out.data_ptr(), out.stride(0), q.data_ptr(), T, q.stride(0), copy.data_ptr(), (int)(mb16 * 16),
+                           cut.data_ptr<int>() + b0, qs, n, (int)H, (int)Hk, (float)scale, (int)window, (float)softcap,
+                           (int)emu, (int)D, ws.data_ptr(), cur_stream());
+  }
   return out;
 }
 

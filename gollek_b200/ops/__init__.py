@@ -401,9 +401,10 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     head_dim 64 / 128 runs on tcgen05/TMEM (the two-tile kernel when ``tiles`` is a ``prefill_schedule``
     work list); other sizes on mma.sync (64-row tiles). ``window`` > 0: sliding-window attention;
     ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (8-bit cache, scales per token or per
-    block) the referenced blocks are dequantized into a bf16 copy first."""
+    block) the referenced blocks are dequantized into a bf16 copy first, as wide as the table; with scales per block and
+    head_dim 64 / 128 the copy stays within 1 GiB (or twice the queries' bytes, or one sequence's): more sequences go in groups."""
     if kv_scales is not None and kv_scales.dim() == 3 and q.is_cuda and tensor_cores and q.shape[2] in (64, 128):
-        # few items, or no work list: the CTAs share the KV tiles evenly by the lengths on the device
+        # by an estimate of both: over the work list, or the CTAs share the KV tiles evenly by the lengths on the device
         return _C(4).block8_prefill(q, kv_cache, kv_scales, block_tables, seq_lens, query_start, scale, tiles,
                                     PREFILL_EMU if emu is None else emu, out, window, softcap)
     if kv_scales is not None:

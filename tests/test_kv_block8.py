@@ -539,6 +539,35 @@ def test_prefill_captured_gpu():
     assert torch.equal(out, ops.paged_prefill_attention(q, c, t, sl.cuda(), qs, 0.1, kv_scales=s))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefill_copy_of_a_wide_table_is_bounded_gpu(D):
+    """Tables far wider than their rows need: the copy stays within 1 GiB and the sequences go in groups; without a work
+    list and with one (which the groups leave unused), a row without queries and one without tokens among them."""
+    lens, new, H = [700, 0, 2100, 40, 333], [60, 0, 130, 40, 1], 8
+    cache, scales, _, bt, sl = filled("int8", lens, 2, D, 16, 83)
+    qs = torch.tensor([0] + new).cumsum(0).int()
+    q = torch.randn(int(qs[-1]), H, D, generator=torch.Generator().manual_seed(9)).bfloat16().cuda()
+    c, s, l = cache[0].cuda(), scales[0].cuda(), sl.cuda()
+    width = 400 * 2 ** 20 // (4 * D * 2) // 16                          # a row's copy takes 400 MiB: two rows a group
+    wide = torch.zeros(len(lens), width, dtype=torch.int32, device="cuda")
+    wide[:, :bt.shape[1]] = bt.cuda()
+    work = ops.prefill_schedule(qs.tolist(), lens, H, 2, D).cuda()
+    want = ops.paged_prefill_attention(q, c, bt.cuda(), l, qs.cuda(), 0.1, kv_scales=s)
+    for tiles in (None, work):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        got = ops.paged_prefill_attention(q, c, wide, l, qs.cuda(), 0.1, tiles=tiles, kv_scales=s)
+        assert torch.cuda.max_memory_allocated() - before < 2 ** 30 + 2 ** 27
+        got = got.double().cpu()
+        for b, n in enumerate(new):
+            rows = torch.arange(lens[b] - n + 1, lens[b] + 1, dtype=torch.int32)
+            out, _, absv, _ = attend(q[qs[b]:qs[b + 1]].cpu(), cache[0], scales[0], bt[b:b + 1].expand(n, -1), rows, 0.1)
+            for x in (got, want.double().cpu()):
+                assert bool(((x[qs[b]:qs[b + 1]] - out).abs() <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all())
+
+
 def test_gather_cpu_behind_the_end():
     cache, scales, _, bt, lens = filled("e4m3", [5, 70], 2, 32, 32, 23)
     tmp, table = ops.kv_dequant_blocks(cache[0], scales[0], bt, lens)
