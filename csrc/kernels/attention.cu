@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(kPfThreads) paged_prefill_kernel(
   const int ctx0 = L - qlen;  // absolute position of query 0
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rows = min(kPfBM, qlen - q_off);
+  if (rows <= 0) return;  // a work list may name tiles that these query_start leave empty
 
   // ---- load Q tile
   for (int i = tid; i < kPfBM * (D / 8); i += kPfThreads) {

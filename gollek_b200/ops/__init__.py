@@ -401,12 +401,15 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     head_dim 64 / 128 runs on tcgen05/TMEM (the two-tile kernel when ``tiles`` is a ``prefill_schedule``
     work list); other sizes on mma.sync (64-row tiles). ``window`` > 0: sliding-window attention;
     ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (8-bit cache, scales per token or per
-    block) the referenced blocks are dequantized into a bf16 copy first, as wide as the table; with scales per block and
-    head_dim 64 / 128 the copy stays within 1 GiB (or twice the queries' bytes, or one sequence's): more sequences go in groups."""
+    block) the referenced blocks are dequantized into a bf16 copy first, as wide as the table; with scales per block the
+    copy stays within 1 GiB (or twice the queries' bytes, or one sequence's): more sequences go in groups."""
     if kv_scales is not None and kv_scales.dim() == 3 and q.is_cuda and tensor_cores and q.shape[2] in (64, 128):
         # by an estimate of both: over the work list, or the CTAs share the KV tiles evenly by the lengths on the device
         return _C(4).block8_prefill(q, kv_cache, kv_scales, block_tables, seq_lens, query_start, scale, tiles,
                                     PREFILL_EMU if emu is None else emu, out, window, softcap)
+    if kv_scales is not None and kv_scales.dim() == 3 and q.is_cuda:
+        return _prefill_block8_mma(q, kv_cache, block_tables, seq_lens, query_start, scale, tiles, out, tensor_cores, window,
+                                   softcap, emu, kv_scales)
     if kv_scales is not None:
         kv_cache, block_tables = kv_dequant_blocks(kv_cache, kv_scales, block_tables,
                                                    seq_lens if kv_scales.dim() == 3 else None)
@@ -420,6 +423,37 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     _C().paged_prefill_attention(out, q, kv_cache, block_tables, seq_lens, query_start, tiles, float(scale),
                                  bool(tensor_cores), int(window), float(softcap),
                                  PREFILL_EMU if emu is None else int(emu))
+    return out
+
+
+PROMPT_COPY_BYTES = 1 << 30  # bf16 copy of prompt attention over a block-scaled cache, as in the binding
+
+
+def _prefill_block8_mma(q, cache, block_tables, seq_lens, query_start, scale, tiles, out, tensor_cores, window, softcap, emu,
+                        scales):
+    """Prompt attention over a block-scaled cache by the kernels that walk a work list over a bf16 cache. Sequences whose
+    copy would pass the limit go in groups: the others have no queries in a group's launch."""
+    n = query_start.shape[0] - 1
+    if block_tables.shape[0] < n or seq_lens.shape[0] < n:
+        raise ValueError("paged_prefill_attention: a block table row and a length for each sequence")
+    out = torch.empty_like(q) if out is None else out
+    if tiles is None:
+        tiles = prefill_schedule(query_start.tolist(), seq_lens.tolist(), q.shape[1], cache.shape[2], q.shape[2],
+                                 tensor_cores).to(q.device)
+    row = block_tables.shape[1] * cache.shape[3] * 2 * cache.shape[2] * cache.shape[4] * 2
+    group = max(1, min(n, max(PROMPT_COPY_BYTES, 4 * q.numel()) // max(1, row)))
+    for b0 in range(0, n, group):
+        b1 = min(n, b0 + group)
+        copy = None  # the last group's goes before this one's comes
+        copy, table = kv_dequant_blocks(cache, scales, block_tables[b0:b1], seq_lens[b0:b1])
+        starts = query_start
+        if group < n:
+            starts = torch.minimum(torch.maximum(query_start, query_start[b0]), query_start[b1])
+            wide = torch.zeros(n, table.shape[1], dtype=torch.int32, device=q.device)
+            wide[b0:b1] = table
+            table = wide
+        _C().paged_prefill_attention(out, q, copy, table, seq_lens, starts, tiles, float(scale), bool(tensor_cores), int(window),
+                                     float(softcap), PREFILL_EMU if emu is None else int(emu))
     return out
 
 

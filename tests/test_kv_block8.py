@@ -540,7 +540,7 @@ def test_prefill_captured_gpu():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 32, 256])
 def test_prefill_copy_of_a_wide_table_is_bounded_gpu(D):
     """Tables far wider than their rows need: the copy stays within 1 GiB and the sequences go in groups; without a work
     list and with one (which the groups leave unused), a row without queries and one without tokens among them."""
