@@ -524,6 +524,51 @@ GOLLEK_DEVICE int stretch_grid(const DecArgs& p, int64_t total) { return (int)mi
 GOLLEK_DEVICE int64_t stretch_begin(int64_t c, int64_t total, int grid) { return c * total / grid; }
 GOLLEK_DEVICE int64_t stretch_of(int64_t x, int64_t total, int grid) { return ((x + 1) * grid - 1) / total; }
 
+// Rows as one list, row b with n(b) * X places: every lane sums the places of an equal range of rows. For whole warps.
+template <class N>
+struct RowList {
+  int B, X, per;
+  int64_t mine = 0, upto, total;  // places of this lane's range, and up to its end
+  N n;
+  GOLLEK_DEVICE RowList(int B, int X, N n) : B(B), X(X), n(n) {
+    const int lane = threadIdx.x & 31;
+    per = (B + 31) / 32;
+    const int r0 = min(B, lane * per), r1 = min(B, r0 + per);
+#pragma unroll 8
+    for (int i = r0; i < r1; ++i) mine += n(i);
+    mine *= X;
+    upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  // The row that place x < total lies in; x becomes its place in that row. First the range, then the row in it.
+  GOLLEK_DEVICE int find(int64_t& x) const {
+    const int lane = threadIdx.x & 31;
+    const int range = __ffs(__ballot_sync(0xffffffffu, upto > x)) - 1;
+    int64_t before = __shfl_sync(0xffffffffu, upto - mine, range);
+    for (int b0 = range * per;; b0 += 32) {
+      const int k = b0 + lane < B ? n(b0 + lane) : 0;
+      int sum = k;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, k > 0 && before + (int64_t)sum * X > x);
+      if (hit) {
+        const int li = __ffs(hit) - 1;
+        x -= before + (int64_t)__shfl_sync(0xffffffffu, sum - k, li) * X;
+        return b0 + li;
+      }
+      before += (int64_t)__shfl_sync(0xffffffffu, sum, 31) * X;
+    }
+  }
+};
+
 // A place in the list of steps: step s of head tile hg of KV head kh of row b.
 struct DecPlace {
   int b, kh, hg, s;
@@ -559,49 +604,22 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
   for (int b = blockIdx.x; b < p.B; b += p.grid)
     if (p.lens[b] <= 0 || p.mb == 0)
       for (int i = threadIdx.x; i < p.H * D / 2; i += S::kThreads) reinterpret_cast<uint32_t*>(p.out + (int64_t)b * p.H * D)[i] = 0u;
-  // this CTA's stretch of the list: every lane sums the steps of an equal range of rows; then the range, and in it the row,
-  // that the stretch begins in
-  const int per = (p.B + 31) / 32, r0 = min(p.B, lane * per), r1 = min(p.B, r0 + per);
-  int64_t mine = 0;
-#pragma unroll 8
-  for (int i = r0; i < r1; ++i) mine += dec_row(p, i, T).n;
-  int64_t upto = mine * X;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += y;
-  }
-  const int64_t total = __shfl_sync(0xffffffffu, upto, 31);
+  // this CTA's stretch of the list
+  auto row_steps = [&](int b) { return dec_row(p, b, T).n; };
+  const RowList<decltype(row_steps)> list(p.B, X, row_steps);
+  const int64_t total = list.total;
   const int grid = stretch_grid(p, total);
   if ((int)blockIdx.x >= grid) return;
   const int64_t first = stretch_begin(blockIdx.x, total, grid);
   const int count = (int)(stretch_begin(blockIdx.x + 1, total, grid) - first);
   DecPlace at;  // of the next step to issue
   {
-    const int range = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
-    int64_t before = __shfl_sync(0xffffffffu, upto - mine * X, range);
-    at.b = 0;
-    for (int b0 = range * per;; b0 += 32) {
-      const int n = b0 + lane < p.B ? dec_row(p, b0 + lane, T).n : 0;
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += y;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, n > 0 && before + (int64_t)sum * X > first);
-      if (hit) {
-        const int li = __ffs(hit) - 1;
-        at.b = b0 + li;
-        before += (int64_t)__shfl_sync(0xffffffffu, sum - n, li) * X;
-        break;
-      }
-      before += (int64_t)__shfl_sync(0xffffffffu, sum, 31) * X;
-    }
+    int64_t place = first;
+    at.b = list.find(place);
     at.r = dec_row(p, at.b, T);
-    const int x = (int)((first - before) / at.r.n);
+    const int x = (int)(place / at.r.n);
     at.kh = x / p.NG, at.hg = x % p.NG;
-    at.s = (int)((first - before) % at.r.n);
+    at.s = (int)(place % at.r.n);
   }
 
   // block ids of this warp's tiles are read 32 at a time, one batch ahead of their use
@@ -1017,21 +1035,21 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
 }
 
 // Joins the parts of the head tiles that several CTAs shared: CTA c < grid the one that leaves the decode kernel's
-// CTA c; the others add the softmax weights of kMassTokens tokens of a (row, kv head) to mass, summed over the
-// head group in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
+// CTA c; the others share the batch's (row, kv head, kMassTokens tokens) by their lengths, however wide the table, and
+// add the tokens' softmax weights to mass, summed over the head group in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
 // share a block.
 // Measured: the weights of 64 rows of up to 4k, 32 heads, add 17 us to the 61 us of the attention (the scores, 4 bytes a head
 // and token, go out to memory and come back).
 constexpr int kJoinThreads = 256, kMassTokens = 1024;
 
 template <int GV>  // heads per KV head where they are 1, 2, 4 or 8, else 0
-__global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB, int mass_tiles) {
+__global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB) {
   __shared__ float sm[128];
   __shared__ float4 others[kJoinThreads];
   __shared__ float2 others_ml[kJoinThreads];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
   if ((int)blockIdx.x < p.grid) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
     const int4 sp = *reinterpret_cast<const int4*>(p.splits + blockIdx.x * 4);  // row, head tile, first part, parts
     if (sp.x < 0) return;
     const int kh = sp.y / p.NG, h0 = (sp.y - kh * p.NG) * HB, nh = min(p.G - h0, HB);
@@ -1082,53 +1100,60 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
     }
     return;
   }
-  const int i = blockIdx.x - p.grid;
-  const int bk = i / mass_tiles, b = bk / p.Hk, kh = bk - b * p.Hk;
-  const int L = min(max(p.lens[b], 0), p.mb << p.bs_log2), lo = p.window > 0 ? max(0, L - p.window) : 0;
-  const int first = (i - bk * mass_tiles) * kMassTokens;
-  if (first >= L || first + kMassTokens <= lo) return;
-  const float* sc = p.scores + (int64_t)bk * (p.mb << p.bs_log2) * p.G;
-  const int* bt = p.tables + (int64_t)b * p.bt_stride;
-  float* mass = p.mass + (kh << p.bs_log2);
+  auto row_pieces = [&](int b) { return dec_row(p, b, kMassTokens).n; };
+  const RowList<decltype(row_pieces)> list(p.B, p.Hk, row_pieces);  // lengths are inputs: no wait
   const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
   constexpr int GN = GV > 0 ? GV : 1, N = kMassTokens / kJoinThreads;
-  // the tokens' scores and blocks are on their way while the heads' sums are joined
-  float v[N][GN];
-  int id[N];
+  bool waited = false;
+  for (int64_t x = (int)blockIdx.x - p.grid; x < list.total; x += (int)gridDim.x - p.grid) {
+    int64_t place = x;
+    const int b = list.find(place);
+    const DecRow r = dec_row(p, b, kMassTokens);
+    const int kh = (int)(place / r.n), first = r.t0 + (int)(place % r.n) * kMassTokens;
+    const float* sc = p.scores + ((int64_t)b * p.Hk + kh) * (p.mb << p.bs_log2) * p.G;
+    const int* bt = p.tables + (int64_t)b * p.bt_stride;
+    float* mass = p.mass + (kh << p.bs_log2);
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    else __syncthreads();  // the last piece's readers of sm are done
+    waited = true;
+    // the tokens' scores and blocks are on their way while the heads' sums are joined
+    float v[N][GN];
+    int id[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    const int t = first + threadIdx.x + k * kJoinThreads;
-    id[k] = t >= lo && t < L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
-    if (GV > 0 && id[k] >= 0) {
-      if constexpr (GV == 1) v[k][0] = sc[t];
-      if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
-      if constexpr (GV >= 4)
+    for (int k = 0; k < N; ++k) {
+      const int t = first + threadIdx.x + k * kJoinThreads;
+      id[k] = t >= r.lo && t < r.L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
+      if (GV > 0 && id[k] >= 0) {
+        if constexpr (GV == 1) v[k][0] = sc[t];
+        if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
+        if constexpr (GV >= 4)
 #pragma unroll
-        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[((int64_t)t * GV + h) / 4];
+          for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[((int64_t)t * GV + h) / 4];
+      }
     }
-  }
-  for (int h = warp; h < p.G; h += kJoinThreads / 32) {
-    const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
-    const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
-                                  : join_ml(p, span.x, span.y, HB, h % HB);
-    if (lane == 0) sm[h] = ml.x + log2f(ml.y);
-  }
-  __syncthreads();
-  float lse[GN];
-#pragma unroll
-  for (int h = 0; h < GN; ++h) lse[h] = sm[h];
-#pragma unroll
-  for (int k = 0; k < N; ++k) {
-    if (id[k] < 0) continue;
-    const int t = first + threadIdx.x + k * kJoinThreads;
-    float w = 0.f;
-    if constexpr (GV > 0) {
-#pragma unroll
-      for (int h = 0; h < GN; ++h) w += ex2(v[k][h] - lse[h]);
-    } else {
-      for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
+    for (int h = warp; h < p.G; h += kJoinThreads / 32) {
+      const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
+      const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
+                                    : join_ml(p, span.x, span.y, HB, h % HB);
+      if (lane == 0) sm[h] = ml.x + log2f(ml.y);
     }
-    atomicAdd(mass + (int64_t)id[k] * row + (t & mask), w);
+    __syncthreads();
+    float lse[GN];
+#pragma unroll
+    for (int h = 0; h < GN; ++h) lse[h] = sm[h];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (id[k] < 0) continue;
+      const int t = first + threadIdx.x + k * kJoinThreads;
+      float w = 0.f;
+      if constexpr (GV > 0) {
+#pragma unroll
+        for (int h = 0; h < GN; ++h) w += ex2(v[k][h] - lse[h]);
+      } else {
+        for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
+      }
+      atomicAdd(mass + (int64_t)id[k] * row + (t & mask), w);
+    }
   }
 }
 
@@ -1648,9 +1673,9 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.cap = softcap > 0.f ? 2.f / softcap : 0.f;  // scores are in log2 units: e^(2 x / cap) = 2^(2 x log2(e) / cap)
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
-  const int mass_tiles = mass ? ((mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
-  const int64_t join = plan.grid + (int64_t)B * Hk * mass_tiles;
-  throw_if(join > 0x7fffffff, "block-scaled decode attention: grid too large");
+  // for the weights twice what the GPU holds at once, or fewer where even full tables would not need them
+  const int64_t pieces = mass ? (int64_t)B * Hk * (((int64_t)mb << p.bs_log2) / kMassTokens + 1) : 0;
+  const int64_t join = plan.grid + std::min<int64_t>(pieces, 16 * device_num_sms());
 #define GOLLEK_B8_M(DD, NN, E, M)                                                                          \
   do {                                                                                                     \
     using S = DecShape<DD, NN>;                                                                            \
@@ -1683,7 +1708,7 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   if (mass && p.G == 2) join_kernel = block8_join_kernel<2>;
   if (mass && p.G == 4) join_kernel = block8_join_kernel<4>;
   if (mass && p.G == 8) join_kernel = block8_join_kernel<8>;
-  launch_after(join_kernel, dim3((unsigned)join), kJoinThreads, 0, s, p, D, 8 * plan.nt, mass_tiles);
+  launch_after(join_kernel, dim3((unsigned)join), kJoinThreads, 0, s, p, D, 8 * plan.nt);
 }
 
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,

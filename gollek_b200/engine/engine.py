@@ -19,6 +19,7 @@ from typing import Callable, Dict, Iterable, List, Optional, Sequence as Seq, Un
 
 import torch
 
+from .. import ops
 from ..config import EngineConfig, ModelConfig, PRESETS, preset
 from ..models.llama import LlamaModel, TPComm
 from ..native import host_ext
@@ -126,6 +127,12 @@ class LLMEngine:
         bpb = self.model.kv_bytes_per_block(cfg.block_size)
         if weigh:  # fp32 attention weight per token, layer and KV head
             bpb += max(1, self.model.num_kv_layers) * self.model.Hk * cfg.block_size * 4
+            if self.device.type == "cuda":
+                # scores of the largest step, held once for every layer and captured batch; the pool gets what is left
+                width = -(-cfg.max_model_len // cfg.block_size) * cfg.block_size
+                self.model.kv_workspace = torch.empty(
+                    ops.block8_workspace(cfg.max_num_seqs, self.model.H, self.model.Hk, self.model.D, width, mass=True),
+                    dtype=torch.float32, device=self.device)
         nb = num_blocks or cfg.num_gpu_blocks
         if nb is None:
             if self.device.type == "cuda":

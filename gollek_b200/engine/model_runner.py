@@ -70,6 +70,7 @@ class _DecodeGraph:
         self.slots = None
         self.block_tables = None
         self.seq_lens = None
+        self.workspace = None
         self.out_ids = None
         self.logits = None
         self.launches = 0
@@ -618,9 +619,10 @@ class ModelRunner:
         g.block_tables = torch.zeros(bs, self.max_blocks, dtype=torch.int32, device=dev)
         # the warm-up rows own no block: length 1 reads block 0, or length 0 where reading would also weigh it
         g.seq_lens = torch.full((bs,), self.pad_len, dtype=torch.int32, device=dev)
-        splits = self._decode_splits(bs, self.cfg.max_model_len)
-        g.workspace = torch.empty(bs * self.model.H * max(1, splits) * (self.model.D + 2),
-                                  dtype=torch.float32, device=dev)
+        if not self.model.kv_block8:  # decode attention over a block-scaled cache has its own
+            splits = self._decode_splits(bs, self.cfg.max_model_len)
+            g.workspace = torch.empty(bs * self.model.H * max(1, splits) * (self.model.D + 2),
+                                      dtype=torch.float32, device=dev)
         meta = self._decode_meta(g)
         # warm up (lazy kernel attributes, allocator) outside capture
         s = torch.cuda.Stream(device=dev)

@@ -228,6 +228,7 @@ class LlamaModel:
         # the attention weight each token has drawn from decoding queries (eviction by attention)
         self.kv_block8 = False
         self.kv_mass: Optional[torch.Tensor] = None
+        self.kv_workspace: Optional[torch.Tensor] = None  # of weighing decode attention (CUDA)
         self.E_loc, self.e0, self.moe_F = 0, 0, self.F
         if cfg.is_moe:
             E = cfg.num_local_experts
@@ -656,7 +657,7 @@ class LlamaModel:
         if nd > 0:
             ops.paged_decode_attention(q[:nd], cache, meta.decode_block_tables, meta.decode_seq_lens, self.scale,
                                        0 if self.kv_block8 else meta.decode_splits, out=out[:nd],
-                                       workspace=None if self.kv_block8 else meta.decode_workspace,
+                                       workspace=self.kv_workspace if self.kv_block8 else meta.decode_workspace,
                                        window=window, softcap=cap, kv_scales=kv_scales, mass=mass)
         if meta.num_prefill_tokens > 0:
             ops.paged_prefill_attention(q[nd:], cache, meta.prefill_block_tables, meta.prefill_seq_lens,
@@ -665,7 +666,8 @@ class LlamaModel:
             if mass is not None:  # a prompt weighs its tokens through its chunk's last query
                 last = (meta.prefill_query_start[1:] - 1).long()
                 ops.paged_decode_attention(q[nd:][last], cache, meta.prefill_block_tables, meta.prefill_seq_lens,
-                                           self.scale, 0, window=window, softcap=cap, kv_scales=kv_scales, mass=mass)
+                                           self.scale, 0, workspace=self.kv_workspace, window=window, softcap=cap,
+                                           kv_scales=kv_scales, mass=mass)
         return out
 
     def _row_linear(self, a: torch.Tensor, w, li: int, lora_kind: Optional[str] = None) -> torch.Tensor:

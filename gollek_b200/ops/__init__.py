@@ -189,7 +189,8 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
     ``kv_scales`` fp32 [NB, 2, Hk]: block-scaled cache (see ``kv_quant_blocks``; head_dim 32, 64, 96,
     128 or 256). A sequence of length 0 gives zeros. The CTAs share the batch's tokens evenly:
     ``num_splits`` 0 fills the GPU, n > 0 takes n CTAs per sequence and KV head on average; without a
-    ``workspace`` one is allocated per call. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
+    ``workspace`` (``block8_workspace`` fp32 elements; with ``mass`` it holds a score for every query head and token of
+    the table's width) one is allocated per call. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
     heads of its KV head, is added to it; where rows share a block all of them are added, and only
     then the last bits depend on their order."""
     if kv_scales is not None and kv_scales.dim() == 3:
@@ -212,6 +213,13 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
                                                           int(num_splits), workspace, bool(tensor_cores),
                                                           int(window), float(softcap), kv_scales)
     return out
+
+
+def block8_workspace(rows: int, heads: int, kv_heads: int, head_dim: int, width: int, num_splits: int = 0,
+                     mass: bool = False) -> int:
+    """fp32 elements that decode attention over a block-scaled cache needs as ``workspace`` for at most ``rows`` sequences and
+    tables of at most ``width`` tokens."""
+    return cuda_ext().block8_workspace(rows, heads, kv_heads, head_dim, width, num_splits, mass)
 
 
 def _decode_block8(q, cache, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap, scales, mass):

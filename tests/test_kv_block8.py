@@ -446,6 +446,37 @@ def test_large_pool_offsets_gpu():
         assert torch.equal(cache[NB - 1 - i].cpu(), want[0][0, i])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("G", [1, 3])
+def test_weights_share_their_work_by_the_lengths_gpu(G):
+    """More pieces of 1024 tokens than the join has CTAs for them, rows of no and of one token among them; and a table
+    64 times wider than the rows need gives the same, to the bit."""
+    g = torch.Generator().manual_seed(87)
+    lens = [0, 1, 1023, 1024, 1025] + torch.randint(1, 2600, (420,), generator=g).tolist() + [0]
+    Hk, D = 4, 32
+    cache, scales, mass, bt, sl = filled("int8", lens, Hk, D, 16, 89)
+    q = torch.randn(len(lens), Hk * G, D, generator=g).bfloat16()
+    out, weights, absv, big = attend(q, cache[0], scales[0], bt, sl, 0.2)
+    wide = torch.zeros(len(lens), bt.shape[1] * 64, dtype=torch.int32, device="cuda")
+    wide[:, :bt.shape[1]] = bt.cuda()
+    ends = []
+    for table in (bt.cuda(), wide):
+        m = mass[0].cuda()
+        got = ops.paged_decode_attention(q.cuda(), cache[0].cuda(), table, sl.cuda(), 0.2, 0, kv_scales=scales[0].cuda(), mass=m)
+        ends.append((got.cpu(), m.cpu()))
+    check_out(ends[0][0], out, absv)
+    want, tol, seen = mass[0].double(), torch.zeros_like(mass[0], dtype=torch.float64), torch.zeros_like(mass[0], dtype=torch.bool)
+    for b, w in enumerate(weights):                                    # as check_mass, a row at a time
+        at = torch.arange(w.shape[1])
+        ids, off = bt[b].long()[at // 16], at % 16
+        want[ids, :, off] += w.T
+        tol[ids, :, off] = (2.0 ** -20 + 2 * D * 2.0 ** -24 * big) * w.T + 2.0 ** -23 * want[ids, :, off]
+        seen[ids, :, off] = True
+    got = ends[0][1].double()
+    assert bool(((got - want).abs() <= tol).all()) and torch.equal(got[~seen], mass[0].double()[~seen])
+    assert torch.equal(ends[0][0], ends[1][0]) and torch.equal(ends[0][1], ends[1][1])
+
+
 # ------------------------------------------------------------------------------------------- prompts
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))

@@ -244,3 +244,24 @@ def test_tables_are_as_wide_as_their_own_rows(tiny_cfg, tiny_weights, halves):
     assert {k for k, *_, mixed in seen if mixed} == {"decode", "prefill"} or halves
     assert all(w == need for _, w, need, _ in seen), seen
     assert any(w < 3 for _, w, *_ in seen) and any(w > 18 for _, w, *_ in seen)
+
+
+@pytest.mark.gpu
+def test_scores_are_held_before_the_pool_is_sized_gpu():
+    """Weighing decode attention keeps a score for every head and token of the table's width: one buffer for all captured
+    batches, allocated before the pool, and no captured batch brings one of its own."""
+    cfg = preset("llama-3-8b", num_hidden_layers=1, vocab_size=4096)
+    w = init_random_weights(cfg, seed=7)
+    eng = engine(cfg, w, device="cuda", num_blocks=64, kv_eviction=True, kv_eviction_policy="attention", max_num_seqs=32,
+                 max_model_len=32768, cuda_graph_batch_sizes=(8, 16, 32))
+    scores = 32 * 32768 * cfg.num_attention_heads * 4
+    assert eng.model.kv_workspace.numel() * 4 >= scores
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_reserved()
+    eng.runner.capture_all()
+    assert len(eng.runner.graphs) == 3 and torch.cuda.memory_reserved() - before < scores
+    g = torch.Generator().manual_seed(4)
+    prompts = [torch.randint(0, 4096, (n,), generator=g).tolist() for n in (40, 20, 130)]
+    outs = eng.generate(prompts, SamplingParams(temperature=0.0, max_tokens=6, ignore_eos=True))
+    for p, o in zip(prompts, outs):
+        assert float(gaps(cfg, w, p, o.output_token_ids).max()) < 0.25
