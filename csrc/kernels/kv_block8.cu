@@ -1035,20 +1035,69 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
 }
 
 // Joins the parts of the head tiles that several CTAs shared: CTA c < grid the one that leaves the decode kernel's
-// CTA c; the others share the batch's (row, kv head, kMassTokens tokens) by their lengths, however wide the table, and
-// add the tokens' softmax weights to mass, summed over the head group in head order. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
+// CTA c; the others add the softmax weights of the batch's pieces (row, kv head, kMassTokens tokens) to mass, summed over
+// the head group in head order: a CTA for each of the `tiles` pieces that a full table would hold, or (0: those would be
+// more than twice what the GPU holds at once) the pieces that the lengths have in turn. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
 // share a block.
 // Measured: the weights of 64 rows of up to 4k, 32 heads, add 17 us to the 61 us of the attention (the scores, 4 bytes a head
 // and token, go out to memory and come back).
 constexpr int kJoinThreads = 256, kMassTokens = 1024;
 
+// The weights of kMassTokens tokens from `first` on of a row and KV head, by a CTA; sm: a float for each head of the group.
 template <int GV>  // heads per KV head where they are 1, 2, 4 or 8, else 0
-__global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB) {
+GOLLEK_DEVICE void weigh_piece(const DecArgs& p, const DecRow& r, int b, int kh, int first, int HB, float* sm) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
+  const float* sc = p.scores + ((int64_t)b * p.Hk + kh) * (p.mb << p.bs_log2) * p.G;
+  const int* bt = p.tables + (int64_t)b * p.bt_stride;
+  float* mass = p.mass + (kh << p.bs_log2);
+  const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
+  constexpr int GN = GV > 0 ? GV : 1, N = kMassTokens / kJoinThreads;
+  // the tokens' scores and blocks are on their way while the heads' sums are joined
+  float v[N][GN];
+  int id[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int t = first + threadIdx.x + k * kJoinThreads;
+    id[k] = t >= r.lo && t < r.L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
+    if (GV > 0 && id[k] >= 0) {
+      if constexpr (GV == 1) v[k][0] = sc[t];
+      if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
+      if constexpr (GV >= 4)
+#pragma unroll
+        for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[((int64_t)t * GV + h) / 4];
+    }
+  }
+  for (int h = warp; h < p.G; h += kJoinThreads / 32) {
+    const int2 span = reinterpret_cast<const int2*>(p.spans)[(int64_t)b * X + kh * p.NG + h / HB];
+    const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
+                                  : join_ml(p, span.x, span.y, HB, h % HB);
+    if (lane == 0) sm[h] = ml.x + log2f(ml.y);
+  }
+  __syncthreads();
+  float lse[GN];
+#pragma unroll
+  for (int h = 0; h < GN; ++h) lse[h] = sm[h];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (id[k] < 0) continue;
+    const int t = first + threadIdx.x + k * kJoinThreads;
+    float w = 0.f;
+    if constexpr (GV > 0) {
+#pragma unroll
+      for (int h = 0; h < GN; ++h) w += ex2(v[k][h] - lse[h]);
+    } else {
+      for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
+    }
+    atomicAdd(mass + (int64_t)id[k] * row + (t & mask), w);
+  }
+}
+
+template <int GV>  // as weigh_piece's; -1: no weights
+__global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs p, int D, int HB, int tiles) {
   __shared__ float sm[128];
   __shared__ float4 others[kJoinThreads];
   __shared__ float2 others_ml[kJoinThreads];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, X = p.Hk * p.NG;
-  if ((int)blockIdx.x < p.grid) {
+  if (GV < 0 || (int)blockIdx.x < p.grid) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the decode kernel still runs
     const int4 sp = *reinterpret_cast<const int4*>(p.splits + blockIdx.x * 4);  // row, head tile, first part, parts
     if (sp.x < 0) return;
@@ -1060,39 +1109,38 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
       const int gr = threadIdx.x / quads, q = q0 + (groups > 1 ? threadIdx.x % quads : threadIdx.x);
       float M = -INFINITY, sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto add = [&](const float2& ml, const float4& o) {
+        const float m = fmaxf(M, ml.x), d0 = m == -INFINITY ? 0.f : M - m, d1 = m == -INFINITY ? 0.f : ml.x - m;
+        const float f0 = ex2(d0), f1 = ex2(d1);
+        M = m;
+        sum = shift_sum(sum, d0) + shift_sum(ml.y, d1);
+        acc.x = f0 * acc.x + f1 * o.x;
+        acc.y = f0 * acc.y + f1 * o.y;
+        acc.z = f0 * acc.z + f1 * o.z;
+        acc.w = f0 * acc.w + f1 * o.w;
+      };
       if (q < quads && (groups == 1 || gr < groups)) {
         const int hh = q * 4 / D;
-#pragma unroll 4
-        for (int i = groups > 1 ? gr : 0; i < sp.w; i += groups) {
-          const int64_t k = part_slot(sp.z, i) * HB + hh;
-          const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[k];
-          const float4 o = *reinterpret_cast<const float4*>(p.part_o + k * D + (q * 4 - hh * D));
-          const float m = fmaxf(M, ml.x), d0 = m == -INFINITY ? 0.f : M - m, d1 = m == -INFINITY ? 0.f : ml.x - m;
-          const float f0 = ex2(d0), f1 = ex2(d1);
-          M = m;
-          sum = shift_sum(sum, d0) + shift_sum(ml.y, d1);
-          acc.x = f0 * acc.x + f1 * o.x;
-          acc.y = f0 * acc.y + f1 * o.y;
-          acc.z = f0 * acc.z + f1 * o.z;
-          acc.w = f0 * acc.w + f1 * o.w;
+        constexpr int N = 4;  // parts whose loads are in flight together
+        for (int i = groups > 1 ? gr : 0; i < sp.w; i += N * groups) {
+          float2 ml[N];
+          float4 o[N];
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const int64_t k = part_slot(sp.z, min(i + e * groups, sp.w - 1)) * HB + hh;
+            ml[e] = reinterpret_cast<const float2*>(p.part_ml)[k];
+            o[e] = *reinterpret_cast<const float4*>(p.part_o + k * D + (q * 4 - hh * D));
+          }
+#pragma unroll
+          for (int e = 0; e < N; ++e)
+            if (i + e * groups < sp.w) add(ml[e], o[e]);
         }
       }
       if (groups > 1) {
         if (gr > 0 && gr < groups) others[threadIdx.x] = acc, others_ml[threadIdx.x] = make_float2(M, sum);
         __syncthreads();
         if (gr > 0) return;
-        for (int g = 1; g < groups; ++g) {
-          const float4 o = others[threadIdx.x + g * quads];
-          const float2 ml = others_ml[threadIdx.x + g * quads];
-          const float m = fmaxf(M, ml.x), d0 = m == -INFINITY ? 0.f : M - m, d1 = m == -INFINITY ? 0.f : ml.x - m;
-          const float f0 = ex2(d0), f1 = ex2(d1);
-          M = m;
-          sum = shift_sum(sum, d0) + shift_sum(ml.y, d1);
-          acc.x = f0 * acc.x + f1 * o.x;
-          acc.y = f0 * acc.y + f1 * o.y;
-          acc.z = f0 * acc.z + f1 * o.z;
-          acc.w = f0 * acc.w + f1 * o.w;
-        }
+        for (int g = 1; g < groups; ++g) add(others_ml[threadIdx.x + g * quads], others[threadIdx.x + g * quads]);
       }
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
       if (q < quads)
@@ -1100,59 +1148,26 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
     }
     return;
   }
-  auto row_pieces = [&](int b) { return dec_row(p, b, kMassTokens).n; };
-  const RowList<decltype(row_pieces)> list(p.B, p.Hk, row_pieces);  // lengths are inputs: no wait
-  const int row = p.Hk << p.bs_log2, mask = (1 << p.bs_log2) - 1;
-  constexpr int GN = GV > 0 ? GV : 1, N = kMassTokens / kJoinThreads;
-  bool waited = false;
-  for (int64_t x = (int)blockIdx.x - p.grid; x < list.total; x += (int)gridDim.x - p.grid) {
-    int64_t place = x;
-    const int b = list.find(place);
-    const DecRow r = dec_row(p, b, kMassTokens);
-    const int kh = (int)(place / r.n), first = r.t0 + (int)(place % r.n) * kMassTokens;
-    const float* sc = p.scores + ((int64_t)b * p.Hk + kh) * (p.mb << p.bs_log2) * p.G;
-    const int* bt = p.tables + (int64_t)b * p.bt_stride;
-    float* mass = p.mass + (kh << p.bs_log2);
-    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-    else __syncthreads();  // the last piece's readers of sm are done
-    waited = true;
-    // the tokens' scores and blocks are on their way while the heads' sums are joined
-    float v[N][GN];
-    int id[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int t = first + threadIdx.x + k * kJoinThreads;
-      id[k] = t >= r.lo && t < r.L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
-      if (GV > 0 && id[k] >= 0) {
-        if constexpr (GV == 1) v[k][0] = sc[t];
-        if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
-        if constexpr (GV >= 4)
-#pragma unroll
-          for (int h = 0; h < GV; h += 4) *reinterpret_cast<float4*>(v[k] + h) = reinterpret_cast<const float4*>(sc)[((int64_t)t * GV + h) / 4];
-      }
+  if constexpr (GV >= 0) {
+    if (tiles > 0) {
+      const int x = (int)blockIdx.x - p.grid, bk = x / tiles, b = bk / p.Hk, first = (x - bk * tiles) * kMassTokens;
+      const DecRow r = dec_row(p, b, kMassTokens);
+      if (first >= r.L || first + kMassTokens <= r.lo) return;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      weigh_piece<GV>(p, r, b, bk - b * p.Hk, first, HB, sm);
+      return;
     }
-    for (int h = warp; h < p.G; h += kJoinThreads / 32) {
-      const int2 span = reinterpret_cast<const int2*>(p.spans)[b * X + kh * p.NG + h / HB];
-      const float2 ml = span.y == 1 ? reinterpret_cast<const float2*>(p.row_ml)[(int64_t)b * p.H + kh * p.G + h]
-                                    : join_ml(p, span.x, span.y, HB, h % HB);
-      if (lane == 0) sm[h] = ml.x + log2f(ml.y);
-    }
-    __syncthreads();
-    float lse[GN];
-#pragma unroll
-    for (int h = 0; h < GN; ++h) lse[h] = sm[h];
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if (id[k] < 0) continue;
-      const int t = first + threadIdx.x + k * kJoinThreads;
-      float w = 0.f;
-      if constexpr (GV > 0) {
-#pragma unroll
-        for (int h = 0; h < GN; ++h) w += ex2(v[k][h] - lse[h]);
-      } else {
-        for (int h = 0; h < p.G; ++h) w += ex2(sc[(int64_t)t * p.G + h] - sm[h]);
-      }
-      atomicAdd(mass + (int64_t)id[k] * row + (t & mask), w);
+    auto row_pieces = [&](int b) { return dec_row(p, b, kMassTokens).n; };
+    const RowList<decltype(row_pieces)> list(p.B, p.Hk, row_pieces);  // lengths are inputs: no wait
+    bool waited = false;
+    for (int64_t x = (int)blockIdx.x - p.grid; x < list.total; x += (int)gridDim.x - p.grid) {
+      int64_t place = x;
+      const int b = list.find(place);
+      const DecRow r = dec_row(p, b, kMassTokens);
+      if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+      else __syncthreads();  // the last piece's readers of sm are done
+      waited = true;
+      weigh_piece<GV>(p, r, b, (int)(place / r.n), r.t0 + (int)(place % r.n) * kMassTokens, HB, sm);
     }
   }
 }
@@ -1673,9 +1688,9 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.cap = softcap > 0.f ? 2.f / softcap : 0.f;  // scores are in log2 units: e^(2 x / cap) = 2^(2 x log2(e) / cap)
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
-  // for the weights twice what the GPU holds at once, or fewer where even full tables would not need them
-  const int64_t pieces = mass ? (int64_t)B * Hk * (((int64_t)mb << p.bs_log2) / kMassTokens + 1) : 0;
-  const int64_t join = plan.grid + std::min<int64_t>(pieces, 16 * device_num_sms());
+  const int64_t tiles = mass ? (((int64_t)mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
+  const int64_t pieces = B * Hk * tiles, most = 16 * device_num_sms();  // the GPU holds eight join CTAs an SM
+  const int64_t join = plan.grid + std::min(pieces, most);
 #define GOLLEK_B8_M(DD, NN, E, M)                                                                          \
   do {                                                                                                     \
     using S = DecShape<DD, NN>;                                                                            \
@@ -1703,12 +1718,13 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
 #undef GOLLEK_B8_N
 #undef GOLLEK_B8_M
   check_launch("block8_decode");
-  auto join_kernel = block8_join_kernel<0>;
+  auto join_kernel = mass ? block8_join_kernel<0> : block8_join_kernel<-1>;
   if (mass && p.G == 1) join_kernel = block8_join_kernel<1>;
   if (mass && p.G == 2) join_kernel = block8_join_kernel<2>;
   if (mass && p.G == 4) join_kernel = block8_join_kernel<4>;
   if (mass && p.G == 8) join_kernel = block8_join_kernel<8>;
-  launch_after(join_kernel, dim3((unsigned)join), kJoinThreads, 0, s, p, D, 8 * plan.nt);
+  launch_after(join_kernel, dim3((unsigned)join), kJoinThreads, 0, s, p, D, 8 * plan.nt,
+               pieces <= most ? (int)tiles : 0);
 }
 
 void launch_kv_evict(void* cache, float* scales, float* mass, const int* tables, int64_t bt_stride, int mb,
