@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kQuantThreads, D <= 64 ? 6 : D <= 128 ? 5 : 3)
       while (back >= 0 && p.slots[back] < 0) --back;
       if (back >= 0 && (p.slots[back] >> p.bs_log2) == blk) continue;
     }
-    if (checked_index(blk, p.num_blocks, p.bounds, -1) < 0) continue;  // beyond the pool: skipped
+    if (checked_index(blk, p.num_blocks, p.bounds, -1) < 0) continue;  // beyond the pool (where bounds are checked): skipped
     const int64_t row = ((int64_t)blk * 2 + w) * p.Hk + h;
     uint8_t* codes = p.cache + (row << p.bs_log2) * D;
     // the run's tokens among the lanes, and whether they are all of it
@@ -1058,7 +1058,7 @@ GOLLEK_DEVICE void weigh_piece(const DecArgs& p, const DecRow& r, int b, int kh,
 #pragma unroll
   for (int k = 0; k < N; ++k) {
     const int t = first + threadIdx.x + k * kJoinThreads;
-    id[k] = t >= r.lo && t < r.L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds) : -1;
+    id[k] = t >= r.lo && t < r.L ? checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds, -1) : -1;  // beyond the pool: none
     if (GV > 0 && id[k] >= 0) {
       if constexpr (GV == 1) v[k][0] = sc[t];
       if constexpr (GV == 2) *reinterpret_cast<float2*>(v[k]) = reinterpret_cast<const float2*>(sc)[t];
@@ -1410,19 +1410,21 @@ GOLLEK_DEVICE void move_masses(const EvictArgs& p, const EvictRow& r, int h, int
   const int* bt = p.tables + (int64_t)b * p.bt_stride;
   float* mass = p.mass + (((int64_t)ly * p.num_blocks * p.Hk + h) << p.bs_log2);
   const int mask = (1 << p.bs_log2) - 1;
-  auto at = [&](int t) {
-    const int id = checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds);
-    return mass + (uint64_t)(uint32_t)id * (p.Hk << p.bs_log2) + (t & mask);
-  };
+  auto at = [&](int t, int id) { return mass + (uint64_t)(uint32_t)id * (p.Hk << p.bs_log2) + (t & mask); };
+  auto from = [&](int t) { return at(t, checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds)); };
   for (int base = threadIdx.x; base - (int)threadIdx.x < r.K; base += N * kMoveThreads) {
     float v[N];
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (base + k * kMoveThreads < r.K) v[k] = *at(kept[base + k * kMoveThreads]);
+      if (base + k * kMoveThreads < r.K) v[k] = *from(kept[base + k * kMoveThreads]);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (base + k * kMoveThreads < r.K) *at(base + k * kMoveThreads) = v[k];
+    for (int k = 0; k < N; ++k) {
+      const int t = base + k * kMoveThreads;
+      if (t >= r.K) continue;
+      const int id = checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds, -1);
+      if (id >= 0) *at(t, id) = v[k];
+    }
   }
 }
 
@@ -1464,7 +1466,8 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
   const uint32_t row_stride = (uint32_t)(2 * p.Hk << p.bs_log2) * D;
   uint8_t* codes = p.cache + ((int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h) * ((int64_t)D << p.bs_log2);
   float* scales = p.scales + (int64_t)ly * p.num_blocks * 2 * p.Hk + w * p.Hk + h;
-  auto block_of = [&](int t) { return checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds); };
+  // beyond the pool: block 0 to read from, none to write to
+  auto block_of = [&](int t, int safe) { return checked_index(bt[t >> p.bs_log2], p.num_blocks, p.bounds, safe); };
   auto scale_at = [&](int id) { return scales + (uint64_t)(uint32_t)id * (2 * p.Hk); };
   const int own = warp * TW + (lane & (TW - 1));  // the token of a chunk whose index and block ids this lane keeps
   const int piece = lane % P * 16;
@@ -1474,7 +1477,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
   // indices of a chunk, block ids of a chunk, codes and scales of a chunk: each one step behind the one before
   int src2, src1, id1;
   auto load_src = [&](int c) { return own < r.K - c * kChunk ? kept[c * kChunk + own] : -1; };
-  auto load_id = [&](int src) { return src >= 0 ? block_of(src) : 0; };
+  auto load_id = [&](int src) { return src >= 0 ? block_of(src, 0) : 0; };
   auto load_codes = [&](int c, int src, int id) {
     const uint32_t st = smem_u32(ring) + (c % kMoveStages) * S::kStage;
 #pragma unroll
@@ -1502,7 +1505,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
   for (int c = 0; c < chunks; ++c) {
     const int base = c * kChunk, n = min(kChunk, r.K - base);
     load_codes(c + 2, src1, id1);
-    const int to_id = own < n ? block_of(base + own) : 0;  // destination block
+    const int to_id = own < n ? block_of(base + own, -1) : -1;  // destination block
     src1 = src2;
     id1 = load_id(src1);
     src2 = load_src(c + 4);
@@ -1539,7 +1542,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       const int d = __shfl_sync(0xffffffffu, to_id, tok(i) & 31), to = base + warp * TW + tok(i);
-      if (!mine(i) || to - base >= n) continue;
+      if (!mine(i) || to - base >= n || d < 0) continue;
       const float z = s[i * R / 16 % GR];
       rescale<E4M3, 4>(code[i], sc[i] * __uint_as_float((254u << 23) - __float_as_uint(z)));  // sc / z, z = 2^e
       *reinterpret_cast<uint4*>(codes + (uint64_t)(uint32_t)d * row_stride + (to & (bs - 1)) * D + piece) =

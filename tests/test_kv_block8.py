@@ -828,3 +828,29 @@ def test_bad_indices_are_reported_gpu():
         out = ops.paged_decode_attention(torch.randn(2, 4, 64, device="cuda").bfloat16(), cache, bad, lens, 0.1,
                                          num_splits=0, kv_scales=scales)
         assert bc.status() == (4, NB + 7) and bool(torch.isfinite(out).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_bad_indices_write_to_no_other_block_gpu(kind):
+    """With bounds checking on, a block id beyond the pool is reported, and neither weights nor an eviction's tokens go to
+    block 0 in its place, which may be somebody's."""
+    cache, scales, mass, bt, lens = [x.cuda() for x in filled(kind, [100, 90], 2, 64, 16, 53)]
+    cache, scales, mass = cache[0].clamp(max=126), scales[0].nan_to_num(0.5), mass[0]
+    NB, mine = cache.shape[0], bt[1, :6].long()
+    bad = bt.clone()
+    bad[0, 1] = NB + 7
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    keep = torch.tensor([50, 50], dtype=torch.int32).cuda()
+    good = [x.clone() for x in (cache, scales, mass)]
+    ops.paged_decode_attention(q, good[0], bt, lens, 0.1, 0, kv_scales=good[1], mass=good[2])
+    ops.kv_evict(*good, bt, lens, keep, 4, 8)
+    with ops.BoundsCheck() as bc:
+        got = [x.clone() for x in (cache, scales, mass)]
+        ops.paged_decode_attention(q, got[0], bad, lens, 0.1, 0, kv_scales=got[1], mass=got[2])
+        assert bc.status() == (4, NB + 7) and torch.equal(got[2][0], mass[0])
+        bc.reset()
+        ops.kv_evict(*got, bad, lens, keep, 4, 8)
+        assert bc.status() == (4, NB + 7)
+    for x, y, z in zip(got, (cache, scales, mass), good):
+        assert torch.equal(x[0], y[0]) and torch.equal(x[mine], z[mine])
