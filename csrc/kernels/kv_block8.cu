@@ -994,10 +994,10 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
           if (whole)
             *reinterpret_cast<uint32_t*>(p.out + row * D + d) = pack_bf16x2(o[i][nt][e] * inv, o[i][nt][e + 2] * inv);
           else
-            *reinterpret_cast<float2*>(p.part_o + (part * HB + hh) * D + d) = make_float2(o[i][nt][e], o[i][nt][e + 2]);
+            *reinterpret_cast<float2*>(p.part_o + ((int64_t)part * HB + hh) * D + d) = make_float2(o[i][nt][e], o[i][nt][e + 2]);
         }
         if (warp == 0 && g == 0) {
-          if (!whole) *reinterpret_cast<float2*>(p.part_ml + (part * HB + hh) * 2) = make_float2(m[nt][e], sum);
+          if (!whole) *reinterpret_cast<float2*>(p.part_ml + ((int64_t)part * HB + hh) * 2) = make_float2(m[nt][e], sum);
           else if (MASS) *reinterpret_cast<float2*>(p.row_ml + row * 2) = make_float2(m[nt][e], sum);
         }
       }
@@ -1005,7 +1005,7 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
       int parts = 1;
       if (!last) {
         parts = (int)(stretch_of(first + j - step + cur.r.n - 1, total, grid) - blockIdx.x) + 1;
-        *reinterpret_cast<int4*>(p.splits + blockIdx.x * 4) = make_int4(b, kh * p.NG + cur.hg, (int)part, parts);
+        *reinterpret_cast<int4*>(p.splits + (int64_t)blockIdx.x * 4) = make_int4(b, kh * p.NG + cur.hg, (int)part, parts);
       }
       if (MASS) *reinterpret_cast<int2*>(p.spans + ((int64_t)b * X + kh * p.NG + cur.hg) * 2) = make_int2((int)part, parts);
     }

@@ -418,6 +418,23 @@ def test_decode_strides_stream_graph_and_shared_blocks_gpu():
 
 
 @pytest.mark.gpu
+def test_large_workspace_offsets_gpu():
+    """64 CTAs a sequence over 8200 sequences: the parts' sums lie up to 2^32 floats and more behind the workspace's start."""
+    B, L, G, D = 8200, 4096, 16, 256
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    cache, scales, _, bt, sl = filled("int8", [L], 1, D, 16, 97)
+    q = torch.randn(8, G, D, generator=torch.Generator().manual_seed(5)).bfloat16()
+    out, _, absv, _ = attend(q, cache[0], scales[0], bt.expand(8, -1), sl.expand(8), 0.05)
+    rows = torch.arange(B) % 8
+    got = ops.paged_decode_attention(q[rows].cuda(), cache[0].cuda(), bt.cuda().expand(B, -1).contiguous(),
+                                     torch.full((B,), L, dtype=torch.int32, device="cuda"), 0.05, 64, kv_scales=scales[0].cuda())
+    check_out(got[:8], out, absv)
+    assert torch.equal(got.view(-1, 8, G, D), got[:8].expand(B // 8, -1, -1, -1))   # every row splits alike
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
 def test_large_pool_offsets_gpu():
     """Blocks whose byte offsets pass 2^32."""
     Hk, D, bs = 8, 128, 16
