@@ -425,8 +425,9 @@ struct FaItem {
 // what its Q load, first scores and epilogue cost. An item that crosses a border leaves unnormalised sums per CTA, joined by
 // prefill_join_kernel. plan: int64 [B + 1], list position of each sequence's first KV tile, then the list's length.
 // Measured: eight chunks of 30 to 100 tokens behind 6000 cached ones, 32 heads, 8 KV heads of 64: 71 us, and 10 us for the joins;
-// the list form takes 100 us for the same. Exponentials bound it: at 16 a cycle and SM they take 45 us of it (more of them on
-// the FMA pipe: the call takes 8 % longer), the rest is the latency of a softmax warp's other steps.
+// the list form takes 100 us for the same. Latency bounds it: 94 M exponentials run (warps without a query skip theirs), 16 us of
+// the MUFU with a quarter of them on the FMA pipe (a larger share there: the call takes 8 % longer); issue slots are 37 % and the
+// matrix pipe 22 % busy, and the two slots' step over a KV tile takes 2.5 us (2.7 at head size 128, with twice the products): a softmax warp's steps.
 constexpr int kFaLead = 3;
 struct FaStretch {
   const long long* plan;

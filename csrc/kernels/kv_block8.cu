@@ -74,9 +74,13 @@ GOLLEK_DEVICE void decode4(uint32_t w, float* f) {
 // first slot starts the block anew, any other can only raise the scale), rounds the codes already
 // there to a raised scale, and stores the run's codes. Memory-bound: 3 bytes a value. A run of at most 16 tokens stays
 // in registers between its magnitude and its codes (16-byte loads, all of them in flight at once); a longer one is read twice.
-// Measured (8 heads of 128): 48 rows of one token 3.2 us, the latency of slot, first code and scale one behind the other;
-// 8190 prompt tokens 14.7 us, 3.4 TB/s: bytes in flight, with the 20 warps an SM holds at 96 registers (16 at 126: 16.4 us; 24
-// at 80 spill: 18 us).
+// Measured (8 heads of 128): 48 rows of one token 3.2 us, the latency of slot, first code and scale one behind the other (4.1 to
+// 4.8 us where every scale grows); 8190 prompt tokens in blocks of 16 14.6 us, 3.4 TB/s: bytes in flight, with the 20 warps an SM
+// holds at 96 registers (16 at 126: 16.4 us; 24 at 80 spill: 18 us). A run that does not stay in registers is stored a token at
+// a time, behind the load of its slot: in blocks of 32 and 64, whose runs are longer, the same tokens take 45 and 49 us. So are
+// the runs of a prompt whose first tokens are the last of their warps' 16 (lane 16), for the next block's first token is not seen: 38
+// us behind 15 decode rows. And in a step of 1024 tokens a warp takes up to 16 decode rows one behind the other: a prompt behind
+// 16 to 256 of them takes 30 us.
 // ---------------------------------------------------------------------------------------------
 GOLLEK_DEVICE uint32_t clean2(uint32_t w) {  // two bf16: NaN -> 0, infinities -> the largest bf16
   uint32_t r = 0;
@@ -378,8 +382,9 @@ __global__ void __launch_bounds__(256, 4)
 // uses p alone. m only moves when a score passes it by 2^8: the vote rides on the barrier that the
 // exchange needs anyway.
 // Measured: 16 rows of 32k (64 heads, 8 KV heads of 128, int8; 1.07 GB) 167 us, 6.4 TB/s: the bytes. 64 rows of up to 4k (32
-// heads, e4m3; 329 MB) 61 us, 5.4 TB/s: 8 us of start, joins and end beside the bytes. One row of 1000 tokens 8.8 us: the
-// latency of two launches, block ids, codes and a join.
+// heads, e4m3; 329 MB) 61 us, 5.4 TB/s: 8 us of start, joins and end beside the bytes. One row of 1000 tokens 8.4 us: the
+// latency of two launches, block ids, codes and a join. Smaller heads lie further from their bytes, for scores, votes and
+// barriers are per token: 64 rows of up to 4k take 51 us at head size 64 (bytes: 29 us) and 42 us at 32 (15 us).
 // ---------------------------------------------------------------------------------------------
 constexpr float kSlack = 8.f;  // p * scale <= 2^9: within f16
 
@@ -1039,8 +1044,10 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
 // the head group in head order: a CTA for each of the `tiles` pieces that a full table would hold, or (0: those would be
 // more than twice what the GPU holds at once) the pieces that the lengths have in turn. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
 // share a block.
-// Measured: the weights of 64 rows of up to 4k, 32 heads, add 17 us to the 61 us of the attention (the scores, 4 bytes a head
-// and token, go out to memory and come back).
+// Measured: the weights of 64 rows of up to 4k, 32 heads, add 16 us to the 61 us of the attention: 20 MB of scores, 4 bytes a head
+// and token, go out and come back (3 us each way at most), but this pass begins when the whole decode kernel has ended and loads
+// block ids, scores and sums one behind the other. Under a table 32 times wider than the rows: 101 us by events, as under one of
+// their own width, where a CTA for every piece of the table took 153 us.
 constexpr int kJoinThreads = 256, kMassTokens = 1024;
 
 // The weights of kMassTokens tokens from `first` on of a row and KV head, by a CTA; sm: a float for each head of the group.
@@ -1332,7 +1339,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const Evic
 // into a ring; a thread only touches the codes that it loaded itself), the indices and block ids they hang on earlier
 // still. Each destination block gets the smallest power-of-two scale for what it then holds: one barrier a chunk, for its
 // largest magnitude.
-// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 176 us with step 1. A (layer,
+// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 176 us with step 1 where earlier evictions have drawn
+// the rows' survivors together, 202 us for the first one of rows as they were written. A (layer,
 // sequence, head) is one chain of chunks, and 512 chains are three or four an SM: latency. With two threads a token, whose
 // loads and stores touch 32 bytes of 16 rows at a time, the way to L2 was the bound (209 us); copies by the bulk engine, a row
 // each, took 313 us.
@@ -1629,7 +1637,6 @@ Block8Plan plan_for(int B, int H, int Hk, int64_t width, int splits, bool mass) 
   using S = DecShape<D, NT>;
   Block8Plan p;
   p.nt = NT;
-  p.tokens = S::kTokens;
   const int G = H / Hk, HB = 8 * NT;
   p.ng = (G + HB - 1) / HB;
   const int64_t tiles = (int64_t)B * Hk * p.ng;

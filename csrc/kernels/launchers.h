@@ -295,7 +295,7 @@ void launch_kv_dequant_scaled(const void* cache, const float* scales, const int*
 // Decode attention over it: a grid of CTAs that share the batch's steps evenly, and the fp32 workspace (counts of
 // floats, in this order) for what they share.
 struct Block8Plan {
-  int grid = 1, nt = 1, ng = 1, tokens = 0;
+  int grid = 1, nt = 1, ng = 1;
   int64_t n_o = 0, n_ml = 0, n_scores = 0, n_row = 0, n_span = 0;
   int64_t floats() const { return n_o + n_ml + n_scores + n_row + n_span; }
 };

@@ -192,7 +192,8 @@ def paged_decode_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables
     ``workspace`` (``block8_workspace`` fp32 elements; with ``mass`` it holds a score for every query head and token of
     the table's width) one is allocated per call. ``mass`` (fp32 [NB, Hk, bs]): each attended token's softmax weight, summed over the query
     heads of its KV head, is added to it; where rows share a block all of them are added, and only
-    then the last bits depend on their order."""
+    then the last bits depend on their order. Probabilities times their block's value scale are f16 numbers
+    against the largest of them: a token whose product is 2^-14 of that or less is off by up to 2^-25 of it."""
     if kv_scales is not None and kv_scales.dim() == 3:
         return _decode_block8(q, kv_cache, block_tables, seq_lens, scale, num_splits, out, workspace, window, softcap,
                               kv_scales, mass)
@@ -405,7 +406,7 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
                             out: Optional[torch.Tensor] = None, tensor_cores: bool = True,
                             window: int = 0, softcap: float = 0.0, emu: Optional[int] = None,
                             kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Varlen causal attention of new tokens q [T, H, D] over the paged KV (prefix + new).
+    """Varlen causal attention of new tokens q [T, H, D] over the paged KV (prefix + new); head_dim 32, 64, 128 or 256.
     head_dim 64 / 128 runs on tcgen05/TMEM (the two-tile kernel when ``tiles`` is a ``prefill_schedule``
     work list); other sizes on mma.sync (64-row tiles). ``window`` > 0: sliding-window attention;
     ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (8-bit cache, scales per token or per
