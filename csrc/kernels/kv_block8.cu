@@ -8,7 +8,8 @@
 //
 // The scales that are written are powers of two (at least 2^-100), so value / scale and its rounding
 // are exact in any precision: a code is a function of the inputs alone, requantizing a block whose
-// scale grows is a shift, and the bf16 copy that prompt attention reads holds every value exactly.
+// scale grows is a shift, and the bf16 copy that prompt attention reads holds every value exactly (but for 2^128, what
+// the largest bf16's code rounds to, in whose place it holds the largest bf16).
 #include <cuda_fp8.h>
 
 #include <algorithm>
@@ -123,6 +124,13 @@ GOLLEK_DEVICE uint2 encode8(const uint4& u, float inv) {
     }
   }
   return make_uint2(c[0], c[1]);
+}
+
+// Two bf16: infinities -> the largest bf16 (NaN stays). Its code rounds up to 2^128, so a value read back may pass fp32's range.
+GOLLEK_DEVICE uint32_t saturate2(uint32_t w) {
+  asm("min.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0x7f7f7f7fu));
+  asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0xff7fff7fu));
+  return w;
 }
 
 struct QuantArgs {
@@ -351,7 +359,9 @@ __global__ void __launch_bounds__(256, 4)
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] *= s[k];
       const int rowi = v / vec;
-      reinterpret_cast<uint4*>(dst)[(row0 + (rowi >> 4) * hrow + (rowi & 15)) * vec + v % vec] = float_to_bf16x8(f);
+      uint4 u = float_to_bf16x8(f);
+      u = make_uint4(saturate2(u.x), saturate2(u.y), saturate2(u.z), saturate2(u.w));  // an infinity would reach masked queries
+      reinterpret_cast<uint4*>(dst)[(row0 + (rowi >> 4) * hrow + (rowi & 15)) * vec + v % vec] = u;
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");  // launched beside the plan: it is done when this kernel is

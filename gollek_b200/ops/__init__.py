@@ -297,7 +297,7 @@ def kv_quant_blocks(kv: torch.Tensor, slots: torch.Tensor, cache: torch.Tensor, 
 
     A write to a block's first slot starts the block anew: its scale is the smallest that holds the
     written rows. Any other write can only raise the scale; the codes already there are then rounded
-    to it. NaN is stored as 0, infinities as the largest bf16. ``mass`` (fp32 [NB, Hk, bs]), the
+    to it. NaN is stored as 0, infinities as the largest bf16 (its code rounds to 2^128 and reads back as the largest bf16). ``mass`` (fp32 [NB, Hk, bs]), the
     attention weight the tokens have drawn, becomes 0 at the written slots. The rows of one block must be
     neighbours in ``slots`` (skipped rows aside), as the engine's batches are; of two rows with the
     same slot the later one stays."""

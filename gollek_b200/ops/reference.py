@@ -130,6 +130,11 @@ def block8_decode_codes(codes: torch.Tensor) -> torch.Tensor:
     return codes.float() if codes.dtype == torch.int8 else codes.view(torch.float8_e4m3fn).float()
 
 
+def _block8_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """codes * scales; 2^128, what the largest bf16's code rounds to, reads as the largest bf16."""
+    return (block8_decode_codes(codes) * scales).clamp(-_BF16_MAX, _BF16_MAX)
+
+
 def block8_encode(y: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """8-bit codes of y = value / scale, to nearest, ties to even, saturating."""
     if dtype == torch.int8:
@@ -203,7 +208,7 @@ def block8_gather(cache: torch.Tensor, scales: torch.Tensor, block_tables: torch
     NB, _, Hk, bs, D = cache.shape
     n, mb = block_tables.shape
     ids = block_tables.long().clamp(0, NB - 1)
-    x = block8_decode_codes(cache[ids]) * scales[ids][..., None, None]          # [n, mb, 2, Hk, bs, D]
+    x = _block8_values(cache[ids], scales[ids][..., None, None])                # [n, mb, 2, Hk, bs, D]
     if seq_lens is not None:
         pos = torch.arange(mb * bs).view(1, mb, 1, 1, bs, 1)
         x = torch.where(pos < seq_lens[:n].long().view(n, 1, 1, 1, 1, 1), x, torch.zeros(()))
@@ -229,7 +234,7 @@ def block8_decode(q: torch.Tensor, cache: torch.Tensor, scales: torch.Tensor, bl
             continue
         at = torch.arange(lo, L)
         ids = block_tables[b].long()[at // bs]
-        kv = block8_decode_codes(cache[ids, :, :, at % bs]) * scales[ids][..., None]   # [n, 2, Hk, D]
+        kv = _block8_values(cache[ids, :, :, at % bs], scales[ids][..., None])  # [n, 2, Hk, D]
         s = torch.einsum("kgd,nkd->kgn", q[b].float().view(Hk, H // Hk, D), kv[:, 0]) * scale
         if softcap > 0:
             s = softcap * torch.tanh(s / softcap)
@@ -266,7 +271,7 @@ def block8_evict(cache: torch.Tensor, scales: torch.Tensor, mass: torch.Tensor, 
                 mid = w[a:L - r].nan_to_num(0.0).sort(descending=True, stable=True).indices[: K - a - r].sort().values + a
                 src = torch.cat([at[:a], mid, at[L - r:]])
                 kept[ly, b, h, :K] = src.int()
-                x = block8_decode_codes(cache[ly, ids[src], :, h, off[src]]) * scales[ly, ids[src], :, h][..., None]
+                x = _block8_values(cache[ly, ids[src], :, h, off[src]], scales[ly, ids[src], :, h][..., None])
                 for j in range(0, K, bs):
                     blk, n = ids[j], min(bs, K - j)
                     s = block8_scale(x[j:j + n].abs().amax((0, 2)), cache.dtype)               # [2]

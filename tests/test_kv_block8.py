@@ -616,6 +616,56 @@ def test_prefill_copy_of_a_wide_table_is_bounded_gpu(D):
                 assert bool(((x[qs[b]:qs[b + 1]] - out).abs() <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all())
 
 
+def infinite_values(kind, D=64):
+    """80 tokens written through the operator, the 41st with infinities in V (and a NaN), and 64-bit values of them all."""
+    g = torch.Generator().manual_seed(31)
+    kv = torch.randn(80, 2, 2, D, generator=g)
+    kv[40, 1, 0, 3], kv[40, 1, 0, 4], kv[40, 1, 1, 5] = math.inf, -math.inf, math.nan
+    cache = torch.zeros(6, 2, 2, 16, D, dtype=KINDS[kind])
+    scales, bt = torch.zeros(6, 2, 2), torch.tensor([[3, 5, 1, 0, 4]], dtype=torch.int32)
+    at = torch.arange(80)
+    ops.kv_quant_blocks(kv.bfloat16(), (bt[0].long()[at // 16] * 16 + at % 16).int(), cache, scales)
+    return cache, scales, bt, g
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", list(KINDS))
+def test_infinities_stay_finite_when_read(kind, device):
+    """The code of the largest bf16 rounds to 2^128. Read as an infinity it would spoil queries that it is masked from (0 times
+    infinity), and an eviction's scales."""
+    cache, scales, bt, g = infinite_values(kind)
+    big = values(cache, scales).abs().max()
+    assert float(big) == 2.0 ** 128
+    c, s, t = cache.clone().to(device), scales.clone().to(device), bt.to(device)
+    copy, _ = ops.kv_dequant_blocks(c, s, t)
+    assert float(copy.double().abs().max()) == float(torch.finfo(torch.bfloat16).max)
+    assert torch.equal(copy.double().cpu().sign(), values(cache, scales)[bt[0].long()].sign().view_as(copy))
+    # prompts: the queries of tokens 30 .. 79; p in bf16, and 2^128 as the largest bf16: half a step 2^-8 each, and the output's
+    q = torch.randn(50, 4, 64, generator=g).bfloat16()
+    lens = torch.arange(31, 81, dtype=torch.int32)
+    out, _, absv, _ = attend(q, cache, scales, bt.expand(50, -1), lens, 0.2)
+    got = ops.paged_prefill_attention(q.to(device), c, t, torch.tensor([80], dtype=torch.int32, device=device),
+                                      torch.tensor([0, 50], dtype=torch.int32, device=device), 0.2, kv_scales=s)
+    err = (got.double().cpu() - out).abs()
+    assert bool(torch.isfinite(got).all()) and bool((err <= 2.0 ** -8 * out.abs() + (2.0 ** -7 + 2.0 ** -8) * absv).all())
+    # eviction: token 40's block keeps its code and gets the scale that holds it
+    mass = torch.rand(6, 2, 16, generator=g)
+    mass[1, :, 8] = 2.0
+    m = mass.to(device)
+    kept = ops.kv_evict(c, s, m, t, torch.tensor([80], dtype=torch.int32, device=device),
+                        torch.tensor([50], dtype=torch.int32, device=device), 4, 8).cpu()
+    for h in range(2):
+        src = kept[0, h, :50].long()
+        x = values(cache, scales)[bt[0].long()[src // 16], :, h, src % 16]                  # [50, 2, D]
+        for j in range(0, 50, 16):
+            for w in range(2):
+                scale = least_scale(min(float(x[j:j + 16, w].abs().max()), 2.0 ** 128 * (1 - 2.0 ** -8)), kind)
+                blk = int(bt[0, j // 16])
+                n = len(x[j:j + 16])
+                assert float(s[blk, w, h]) == scale
+                assert torch.equal(numbers(c.cpu()[blk, w, h, :n]), nearest(x[j:j + 16, w] / scale, kind))
+
+
 def test_gather_cpu_behind_the_end():
     cache, scales, _, bt, lens = filled("e4m3", [5, 70], 2, 32, 32, 23)
     tmp, table = ops.kv_dequant_blocks(cache[0], scales[0], bt, lens)
