@@ -495,6 +495,11 @@ GOLLEK_DEVICE float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 2^(2 x), below fp32's normal numbers too: beside value scales of 2^122 a weight of 2^-20 is a probability of 2^-142
+GOLLEK_DEVICE float ex2_twice(float x) {
+  const float y = ex2(x);
+  return y * y;
+}
 // l * 2^d in two steps: l reaches 2^108 beside value scales of 2^-100, where 2^d alone would underflow
 GOLLEK_DEVICE float shift_sum(float l, float d) {
   const float h = ex2(0.5f * d);
@@ -906,7 +911,7 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
         for (int q = 0; q < TW; ++q) {
           float e4[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) e4[e] = ex2(s[q][nt][e] - m[nt][e & 1]);  // a masked score is -inf
+          for (int e = 0; e < 4; ++e) e4[e] = ex2_twice(fmaf(s[q][nt][e], 0.5f, -0.5f * m[nt][e & 1]));  // a masked score is -inf
           sum[nt][0] += e4[0] + e4[2];
           sum[nt][1] += e4[1] + e4[3];
           const __half2 u = __floats2half2_rn(e4[0] * vs[q], e4[1] * vs[q]);
@@ -1007,7 +1012,7 @@ __global__ void __launch_bounds__(DecShape<D, NT>::kThreads, DecShape<D, NT>::kC
         for (int i = 0; i < OWN; ++i) {
           const int d = (warp * OWN + i) * 16 + 2 * g;
           if (whole)
-            *reinterpret_cast<uint32_t*>(p.out + row * D + d) = pack_bf16x2(o[i][nt][e] * inv, o[i][nt][e + 2] * inv);
+            *reinterpret_cast<uint32_t*>(p.out + row * D + d) = saturate2(pack_bf16x2(o[i][nt][e] * inv, o[i][nt][e + 2] * inv));
           else
             *reinterpret_cast<float2*>(p.part_o + ((int64_t)part * HB + hh) * D + d) = make_float2(o[i][nt][e], o[i][nt][e + 2]);
         }
@@ -1161,7 +1166,8 @@ __global__ void __launch_bounds__(kJoinThreads) block8_join_kernel(const DecArgs
       }
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
       if (q < quads)
-        *reinterpret_cast<uint2*>(out + q * 4) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+        *reinterpret_cast<uint2*>(out + q * 4) =
+            make_uint2(saturate2(pack_bf16x2(acc.x * inv, acc.y * inv)), saturate2(pack_bf16x2(acc.z * inv, acc.w * inv)));
     }
     return;
   }

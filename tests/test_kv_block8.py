@@ -666,6 +666,30 @@ def test_infinities_stay_finite_when_read(kind, device):
                 assert torch.equal(numbers(c.cpu()[blk, w, h, :n]), nearest(x[j:j + 16, w] / scale, kind))
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("splits", [0, 64])
+def test_decode_over_the_largest_values(kind, splits, device):
+    """Value scales up to 2^122 beside ordinary ones: the weights of the block's own tokens may not drown, down to 2^-20 of
+    the largest, nor the sum they are divided by; a token of the largest bf16 alone reads as that."""
+    cache, scales, bt, g = infinite_values(kind)
+    q = torch.randn(50, 4, 64, generator=g).bfloat16()
+    lens = torch.arange(31, 81, dtype=torch.int32)
+    out, _, absv, _ = attend(q, cache, scales, bt.expand(50, -1), lens, 0.2)
+    dev = [x.to(device) for x in (q, cache, bt.expand(50, -1).contiguous(), lens)]
+    got = ops.paged_decode_attention(*dev, 0.2, splits, kv_scales=scales.to(device)).double().cpu()
+    # p times its block's scale is held in f16 against the largest of them: rows that see a token of token 40's block (32 .. 47)
+    # are off by up to 2^-25 of that a token and unit of code (as in test_decode_uneven_scales_gpu); the codes there are
+    # zero but for token 40's, at most 64 (256 in e4m3), whose product 2^128 stands for, so 2^-25 2^128 a token; and 2^128
+    # reads as the largest bf16, 2^-8 less
+    floor = torch.where(lens > 32, 80 * 2.0 ** -25 * 2.0 ** 128, 0.0)[:, None, None]
+    assert bool(((got - out).abs() <= 2.0 ** -8 * out.abs() + (2.0 ** -10 + 2.0 ** -8) * absv + floor).all())
+    one = torch.full((1,), 41, dtype=torch.int32, device=device)
+    got = ops.paged_decode_attention(dev[0][:1], dev[1], dev[2][:1], one, 0.2, splits, kv_scales=scales.to(device), window=1)
+    top = float(torch.finfo(torch.bfloat16).max)
+    assert float(got[0, 0, 3]) == top and float(got[0, 1, 4]) == -top and float(got[0, 2, 5]) == 0.0
+
+
 def test_gather_cpu_behind_the_end():
     cache, scales, _, bt, lens = filled("e4m3", [5, 70], 2, 32, 32, 23)
     tmp, table = ops.kv_dequant_blocks(cache[0], scales[0], bt, lens)
