@@ -1568,7 +1568,8 @@ __global__ void __launch_bounds__(kMoveThreads, 4) kv_evict_move_kernel(const Ev
       const int d = __shfl_sync(0xffffffffu, to_id, tok(i) & 31), to = base + warp * TW + tok(i);
       if (!mine(i) || to - base >= n || d < 0) continue;
       const float z = s[i * R / 16 % GR];
-      rescale<E4M3, 4>(code[i], sc[i] * __uint_as_float((254u << 23) - __float_as_uint(z)));  // sc / z, z = 2^e
+      // sc / z, z = 2^e. A code that is not zero has a ratio of 2^18 at most; beside a scale of 2^120, zeros would meet an infinity
+      rescale<E4M3, 4>(code[i], fminf(sc[i] * __uint_as_float((254u << 23) - __float_as_uint(z)), 0x1p100f));
       *reinterpret_cast<uint4*>(codes + (uint64_t)(uint32_t)d * row_stride + (to & (bs - 1)) * D + piece) =
           make_uint4(code[i][0], code[i][1], code[i][2], code[i][3]);
       if ((to & (bs - 1)) == 0 && piece == 0) *scale_at(d) = z;

@@ -762,6 +762,35 @@ def test_evict_cpu(kind, sink, recent, max_keep):
     assert same(c[1].double(), want[2]) and same(c[2], want[3])
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("K", [4, 20])
+def test_evict_zeros_out_of_a_large_scale(kind, K, device):
+    """The neighbours of an infinity are zeros at a scale of 2^120 or more. Once that token is dropped they go to a scale of 2^-100
+    (among themselves) or of ordinary tokens, and stay zeros."""
+    g = torch.Generator().manual_seed(37)
+    kv = torch.randn(48, 2, 2, 128, generator=g)
+    kv[5, :, :, 7] = math.inf
+    cache, scales, bt = torch.zeros(4, 2, 2, 16, 128, dtype=KINDS[kind]), torch.zeros(4, 2, 2), torch.tensor([[2, 0, 3]], dtype=torch.int32)
+    at = torch.arange(48)
+    ops.kv_quant_blocks(kv.bfloat16(), (bt[0].long()[at // 16] * 16 + at % 16).int(), cache, scales)
+    mass = torch.rand(4, 2, 16, generator=g)
+    mass[2, :, 5] = 0.0
+    x = values(cache, scales)[bt[0].long()].permute(1, 2, 0, 3, 4).reshape(2, 2, 48, 128)
+    c, s = cache.clone().to(device), scales.clone().to(device)
+    kept = ops.kv_evict(c, s, mass.clone().to(device), bt.to(device), torch.tensor([48], dtype=torch.int32, device=device),
+                        torch.tensor([K], dtype=torch.int32, device=device), 4, 0).cpu()
+    for h in range(2):
+        src = kept[0, h, :K].long()
+        assert 5 not in src.tolist() and src[:4].tolist() == [0, 1, 2, 3]
+        for w in range(2):
+            for j in range(0, K, 16):
+                y = x[w, h, src[j:j + 16]]
+                scale, blk = least_scale(float(y.abs().max()), kind), int(bt[0, j // 16])
+                assert float(s[blk, w, h]) == scale
+                assert torch.equal(numbers(c.cpu()[blk, w, h, :len(y)]), nearest(y / scale, kind))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", list(KINDS))
 @pytest.mark.parametrize("D,bs", [(128, 16), (64, 32), (64, 16), (96, 16), (256, 64), (32, 16), (160, 16), (192, 32), (224, 16)])
