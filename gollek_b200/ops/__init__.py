@@ -411,7 +411,8 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
     work list); other sizes on mma.sync (64-row tiles). ``window`` > 0: sliding-window attention;
     ``softcap`` > 0: tanh soft-capped scores. With ``kv_scales`` (8-bit cache, scales per token or per
     block) the referenced blocks are dequantized into a bf16 copy first, as wide as the table; with scales per block the
-    copy stays within 1 GiB (or twice the queries' bytes, or one sequence's): more sequences go in groups."""
+    copy stays within 1 GiB (or twice the queries' bytes, or one sequence's): more sequences go in groups. There a length
+    beyond the table is cut to it, and queries in front of their sequence's first token give zeros."""
     if kv_scales is not None and kv_scales.dim() == 3 and q.is_cuda and tensor_cores and q.shape[2] in (64, 128):
         # by an estimate of both: over the work list, or the CTAs share the KV tiles evenly by the lengths on the device
         return _C(4).block8_prefill(q, kv_cache, kv_scales, block_tables, seq_lens, query_start, scale, tiles,
@@ -420,6 +421,8 @@ def paged_prefill_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_table
         return _prefill_block8_mma(q, kv_cache, block_tables, seq_lens, query_start, scale, tiles, out, tensor_cores, window,
                                    softcap, emu, kv_scales)
     if kv_scales is not None:
+        if kv_scales.dim() == 3:
+            seq_lens = seq_lens.clamp(0, block_tables.shape[1] * kv_cache.shape[3])
         kv_cache, block_tables = kv_dequant_blocks(kv_cache, kv_scales, block_tables,
                                                    seq_lens if kv_scales.dim() == 3 else None)
     if not q.is_cuda:
@@ -449,7 +452,9 @@ def _prefill_block8_mma(q, cache, block_tables, seq_lens, query_start, scale, ti
     if tiles is None:
         tiles = prefill_schedule(query_start.tolist(), seq_lens.tolist(), q.shape[1], cache.shape[2], q.shape[2],
                                  tensor_cores).to(q.device)
-    row = block_tables.shape[1] * cache.shape[3] * 2 * cache.shape[2] * cache.shape[4] * 2
+    width = block_tables.shape[1] * cache.shape[3]
+    seq_lens = seq_lens[:n].clamp(0, width)  # the copy's table has no columns beyond
+    row = width * 2 * cache.shape[2] * cache.shape[4] * 2
     group = max(1, min(n, max(PROMPT_COPY_BYTES, 4 * q.numel()) // max(1, row)))
     for b0 in range(0, n, group):
         b1 = min(n, b0 + group)

@@ -116,7 +116,8 @@ def paged_attention(q: torch.Tensor, kv_cache: torch.Tensor, block_tables: torch
         if window > 0:
             masked = masked | (kpos[None, None, :] <= qpos[None, :, None] - window)
         sc = sc.masked_fill(masked, float("-inf"))
-        out[s:e] = torch.einsum("hqk,khd->qhd", torch.softmax(sc, -1), v).to(q.dtype)
+        p = torch.softmax(sc, -1).masked_fill(masked.all(-1, keepdim=True), 0.0)  # a query that sees no token: zeros
+        out[s:e] = torch.einsum("hqk,khd->qhd", p, v).to(q.dtype)
     return out
 
 

@@ -568,6 +568,25 @@ def test_prefill_lengths_beside_the_queries_gpu(D, tiles):
         assert bool(((got[qs[b]:qs[b + 1]] - out).abs() <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all())
 
 
+@pytest.mark.parametrize("device,D", [("cpu", 32), ("cpu", 64), *(pytest.param("cuda", D, marks=pytest.mark.gpu) for D in (32, 256))])
+def test_prefill_lengths_beside_the_queries_elsewhere(device, D):
+    """The same on the CPU and at the head sizes that go through the work list over a copy."""
+    lens, new, H = [0, 100, 7, 300], [150, 400, 7, 20], 4
+    cache, scales, _, bt, sl = filled("int8", lens, 2, D, 16, 79)
+    bt, sl[3] = bt[:, :16], 1000                                       # 256 tokens fit the table
+    qs = torch.tensor([0] + new).cumsum(0).int()
+    q = torch.randn(int(qs[-1]), H, D, generator=torch.Generator().manual_seed(6)).bfloat16()
+    c, s, t, l, st = (x.to(device) for x in (cache[0], scales[0], bt, sl, qs))
+    got = ops.paged_prefill_attention(q.to(device), c, t, l, st, 0.1, out=torch.full_like(q, math.nan, device=device),
+                                      kv_scales=s).double().cpu()
+    assert not bool(got[:150].any()) and not bool(got[150:450].any())
+    for b, n in enumerate(new):
+        L = min(lens[b] if b < 3 else 1000, 256)
+        rows = torch.arange(L - n + 1, L + 1).clamp(min=0).int()
+        out, _, absv, _ = attend(q[qs[b]:qs[b + 1]], cache[0], scales[0], bt[b:b + 1].expand(n, -1), rows, 0.1)
+        assert bool(((got[qs[b]:qs[b + 1]] - out).abs() <= 2.0 ** -8 * out.abs() + 2.0 ** -7 * absv).all())
+
+
 @pytest.mark.gpu
 def test_prefill_captured_gpu():
     """A captured step replayed with other lengths and chunk borders."""
