@@ -427,7 +427,8 @@ struct FaItem {
 // Measured: eight chunks of 30 to 100 tokens behind 6000 cached ones, 32 heads, 8 KV heads of 64: 71 us, and 10 us for the joins;
 // the list form takes 100 us for the same. Latency bounds it: 94 M exponentials run (warps without a query skip theirs), 16 us of
 // the MUFU with a quarter of them on the FMA pipe (a larger share there: the call takes 8 % longer); issue slots are 37 % and the
-// matrix pipe 22 % busy, and the two slots' step over a KV tile takes 2.5 us (2.7 at head size 128, with twice the products): a softmax warp's steps.
+// matrix pipe 22 % busy, and the two slots' step over a KV tile takes 2.5 us (2.7 at head size 128, with twice the products): a
+// softmax warp's steps, one behind the other.
 constexpr int kFaLead = 3;
 struct FaStretch {
   const long long* plan;

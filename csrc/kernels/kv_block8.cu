@@ -1057,12 +1057,12 @@ GOLLEK_DEVICE float2 join_ml(const DecArgs& p, int first, int n, int HB, int hh)
 // Joins the parts of the head tiles that several CTAs shared: CTA c < grid the one that leaves the decode kernel's
 // CTA c; the others add the softmax weights of the batch's pieces (row, kv head, kMassTokens tokens) to mass, summed over
 // the head group in head order: a CTA for each of the `tiles` pieces that a full table would hold, or (0: those would be
-// more than twice what the GPU holds at once) the pieces that the lengths have in turn. An entry gets one add per call, so sums do not depend on the order of the CTAs unless rows
-// share a block.
+// more than 16 an SM, several times what it holds at once) the pieces that the lengths have in turn. An entry gets one add
+// per call, so sums do not depend on the order of the CTAs unless rows share a block.
 // Measured: the weights of 64 rows of up to 4k, 32 heads, add 16 us to the 61 us of the attention: 20 MB of scores, 4 bytes a head
 // and token, go out and come back (3 us each way at most), but this pass begins when the whole decode kernel has ended and loads
-// block ids, scores and sums one behind the other. Under a table 32 times wider than the rows: 101 us by events, as under one of
-// their own width, where a CTA for every piece of the table took 153 us.
+// block ids, scores and sums one behind the other. Under a table 32 times wider than the rows: 101 us by events, where a
+// CTA for every piece of the table took 153 us; where the pieces fit the grid, to search for them costs 2 us (87 us, not 85).
 constexpr int kJoinThreads = 256, kMassTokens = 1024;
 
 // The weights of kMassTokens tokens from `first` on of a row and KV head, by a CTA; sm: a float for each head of the group.
@@ -1355,8 +1355,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_evict_select_kernel(const Evic
 // into a ring; a thread only touches the codes that it loaded itself), the indices and block ids they hang on earlier
 // still. Each destination block gets the smallest power-of-two scale for what it then holds: one barrier a chunk, for its
 // largest magnitude.
-// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 176 us with step 1 where earlier evictions have drawn
-// the rows' survivors together, 202 us for the first one of rows as they were written. A (layer,
+// Measured: 8 layers x 4 sequences of 8192 tokens to 60 % (8 heads of 128, e4m3; 660 MB at least) 176 us with step 1 where
+// earlier evictions have drawn the rows' survivors together, 202 us for the first one of rows as they were written. A (layer,
 // sequence, head) is one chain of chunks, and 512 chains are three or four an SM: latency. With two threads a token, whose
 // loads and stores touch 32 bytes of 16 rows at a time, the way to L2 was the bound (209 us); copies by the bulk engine, a row
 // each, took 313 us.
@@ -1716,7 +1716,7 @@ void launch_block8_decode(void* out, const void* q, int64_t q_stride, const void
   p.cap_log2 = softcap * kLog2e;
   p.bounds = bounds_status();
   const int64_t tiles = mass ? (((int64_t)mb << p.bs_log2) + kMassTokens - 1) / kMassTokens : 0;
-  const int64_t pieces = B * Hk * tiles, most = 16 * device_num_sms();  // the GPU holds eight join CTAs an SM
+  const int64_t pieces = B * Hk * tiles, most = 16 * device_num_sms();
   const int64_t join = plan.grid + std::min(pieces, most);
 #define GOLLEK_B8_M(DD, NN, E, M)                                                                          \
   do {                                                                                                     \
